@@ -11,7 +11,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 # FLINT_ATTN_LIB names another build of the same library (an A/B comparison, a debug build)
 LIB_PATH = os.environ.get("FLINT_ATTN_LIB") or os.path.join(HERE, "libflint_attn.so")
 
-F32, BF16 = 0, 1
+F32, BF16, F16 = 0, 1, 2  # F16: rows of store_kv_dev / load_kv_dev only
+KV_F16, KV_INT4 = 0, 1
 N_HEAD, N_HEAD_KV, HEAD_DIM = 32, 4, 128
 QKV_DIM, OUT_DIM, PARTIAL_DIM = 5120, 4096, 130
 ERR_LEN = 1024  # server/src/ffi.rs:38
@@ -27,7 +28,16 @@ class _Config(C.Structure):
                 ("kv_rank", C.c_int32), ("kv_ranks", C.c_int32), ("kv_pages", C.c_int32)]
 
 
+class _KvOptions(C.Structure):
+    _fields_ = [("kv_format", C.c_int32), ("first_tokens", C.c_int32)]
+
+
+_KV_ROWS = [C.c_void_p, C.c_int32, C.c_int32, C.POINTER(C.c_int32), C.POINTER(C.c_int32), C.c_int32, C.c_void_p, C.c_void_p,
+            C.c_int32, C.c_void_p, C.c_char_p, C.c_int32]
 SYMBOLS = {
+    "flint_attn_open_kv": (C.c_void_p, [C.POINTER(_Config), C.POINTER(_KvOptions), C.c_char_p, C.c_int32]),
+    "flint_attn_store_kv_dev": (C.c_int32, _KV_ROWS),
+    "flint_attn_load_kv_dev": (C.c_int32, _KV_ROWS),
     "flint_attn_open": (C.c_void_p, [C.POINTER(_Config), C.c_char_p, C.c_int32]),
     "flint_attn_close": (None, [C.c_void_p]),
     "flint_attn_n_ctx": (C.c_int32, [C.c_void_p]),
@@ -166,14 +176,16 @@ class Attn:
     """One attention handle on one GPU. Single owner, not thread-safe (src/capi.h:1)."""
 
     def __init__(self, layer_is_swa: Sequence[bool], layer_has_rope: Sequence[bool], max_seqs: int, n_ctx: int,
-                 device: int = 0, kv_rank: int = 0, kv_ranks: int = 1, kv_pages: int = 0):
+                 device: int = 0, kv_rank: int = 0, kv_ranks: int = 1, kv_pages: int = 0, kv_format: int = KV_F16,
+                 first_tokens: int = 0):
         self._lib = load_library()
         self._err = C.create_string_buffer(ERR_LEN)
         self.n_layers = len(layer_is_swa)
         swa, rope = _i32([int(b) for b in layer_is_swa]), _i32([int(b) for b in layer_has_rope])
         cfg = _Config(device, self.n_layers, swa, rope, max_seqs, n_ctx, kv_rank, kv_ranks, kv_pages)
         err = C.create_string_buffer(ERR_LEN)
-        self._h = self._lib.flint_attn_open(C.byref(cfg), err, ERR_LEN)
+        opt = _KvOptions(kv_format, first_tokens)
+        self._h = self._lib.flint_attn_open_kv(C.byref(cfg), C.byref(opt), err, ERR_LEN)
         if not self._h:
             raise FlintAttnError(err.value.decode(errors="replace"))
         self.layer_is_swa = [bool(b) for b in layer_is_swa]
@@ -360,6 +372,35 @@ class Attn:
         k, v = np.ascontiguousarray(k, np.uint16), np.ascontiguousarray(v, np.uint16)
         assert k.shape == v.shape and k.shape[0] == N_HEAD_KV and k.shape[2] == HEAD_DIM
         self._call("flint_attn_write_kv", layer, seq, slot0, k.shape[1], k.ctypes.data, v.ctypes.data)
+
+    def _kv_rows(self, name, layer, seqs, pos0, n_rows, k_dev, v_dev, dtype, stream):
+        """f() that enqueues the call, with every argument converted once."""
+        if len(seqs) != len(pos0):
+            raise ValueError("one start position per sequence")
+        fn, h, err = getattr(self._lib, name), self._h, self._err
+        args = (layer, len(seqs), _i32(seqs), _i32(pos0), n_rows, _ptr(k_dev), _ptr(v_dev), dtype, stream)
+
+        def call():
+            if fn(h, *args, err, ERR_LEN) != 0:
+                raise FlintAttnError(err.value.decode(errors="replace"))
+
+        return call
+
+    def store_kv_dev(self, layer, seqs, pos0, n_rows, k_dev, v_dev, dtype, stream: int = 0):
+        """Rows [len(seqs)][4][n_rows][128] of K and V on the device into the cache, sequence i from position pos0[i] on."""
+        self._kv_rows("flint_attn_store_kv_dev", layer, seqs, pos0, n_rows, k_dev, v_dev, dtype, stream)()
+
+    def load_kv_dev(self, layer, seqs, pos0, n_rows, k_dev, v_dev, dtype, stream: int = 0):
+        """The reverse of store_kv_dev: the values that the cache stands for."""
+        self._kv_rows("flint_attn_load_kv_dev", layer, seqs, pos0, n_rows, k_dev, v_dev, dtype, stream)()
+
+    def prepared_store_kv_dev(self, layer, seqs, pos0, n_rows, k_dev, v_dev, dtype, stream: int = 0):
+        """f() that enqueues store_kv_dev with these arguments, for a caller that makes the same call again."""
+        return self._kv_rows("flint_attn_store_kv_dev", layer, seqs, pos0, n_rows, k_dev, v_dev, dtype, stream)
+
+    def prepared_load_kv_dev(self, layer, seqs, pos0, n_rows, k_dev, v_dev, dtype, stream: int = 0):
+        """f() that enqueues load_kv_dev with these arguments."""
+        return self._kv_rows("flint_attn_load_kv_dev", layer, seqs, pos0, n_rows, k_dev, v_dev, dtype, stream)
 
     def kv_dev(self, layer: int, which: int) -> int:
         return int(self._lib.flint_attn_kv_dev(self._h, layer, which) or 0)

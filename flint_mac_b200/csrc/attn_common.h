@@ -27,6 +27,7 @@ constexpr int kMergeFan = 16;                  // splits folded by one CTA in th
 
 constexpr int kDtypeF32 = 0;
 constexpr int kDtypeBf16 = 1;
+constexpr int kDtypeF16 = 2;  // cache rows only (store / load)
 
 // One unit of decode work: the 8 query heads of one KV head of one token against cached keys [j0, j1).
 struct DecItem {

@@ -13,6 +13,7 @@
 
 #include "../../include/flint_attn.h"
 #include "attn_common.h"
+#include "kv4.h"
 #include "prefill_attn.h"
 #include "proj.h"
 
@@ -40,6 +41,7 @@ struct Layer {
     int n_slots = 0;
     int kv_lo = 0, kv_hi = 0;  // positions a full layer holds on this device: [kv_lo, kv_hi)
     __half *k = nullptr, *v = nullptr;
+    Kv4Cache kv4;  // the cache of a handle that keeps K/V in 4 bits (k and v are null then)
     float *q_norm = nullptr, *k_norm = nullptr, *sinks = nullptr;  // device copies
     // projections either side of attention (optional): attn_norm [n_embd] fp32, W_qkv [5120][n_embd] bf16 (q rows,
     // then k rows, then v rows: the packed row of src/metal/fused.metal:211), W_o [n_embd][4096] bf16
@@ -228,6 +230,7 @@ struct flint_attn {
     std::vector<int32_t> seq_blocks;   // blocks each sequence holds
     std::vector<int32_t> free_pages;   // stack of free page numbers
     int32_t *table_dev = nullptr;
+    int kv_format = FLINT_ATTN_KV_F16, first_tokens = 0;
     int *dec_err = nullptr;  // device word the decode kernel sets when a bounded wait runs out
     std::vector<Layer> layers;
     std::vector<int32_t> pos;
@@ -272,7 +275,7 @@ struct flint_attn {
     ~flint_attn() {
         cudaSetDevice(device);
         for (auto &L : layers) {
-            cudaFree(L.k); cudaFree(L.v); cudaFree(L.q_norm); cudaFree(L.k_norm); cudaFree(L.sinks);
+            cudaFree(L.k); cudaFree(L.v); cudaFree(L.kv4.blocks); cudaFree(L.q_norm); cudaFree(L.k_norm); cudaFree(L.sinks);
             cudaFree(L.attn_norm); cudaFree(L.w_qkv); cudaFree(L.w_o); cudaFree(L.kv_maps);
         }
         cudaFree(dec_err);
@@ -413,6 +416,7 @@ struct flint_attn {
         check_seqs(n, seqs);
         if (qkv_dtype != kDtypeF32 && qkv_dtype != kDtypeBf16) throw std::runtime_error("bad qkv dtype");
         if (mode == 0 && out_dtype != kDtypeF32 && out_dtype != kDtypeBf16) throw std::runtime_error("bad out dtype");
+        if (mode != 0 && L.kv4.blocks) throw std::runtime_error("partial records are not kept for a 4-bit cache");
         if (mode == 0 && kv_ranks > 1 && !L.is_swa)
             throw std::runtime_error("full layers of a KV-sharded handle need decode_partial + combine");
         std::vector<int32_t> &p = batch_pos;
@@ -475,6 +479,25 @@ struct flint_attn {
         }
         ensure_scratch(n_records, n_subs, n_groups);
         const bool inline_items = items.size() <= size_t(kMaxParamItems);
+        if (L.kv4.blocks) {
+            Dec4Params dp{};
+            dp.items = inline_items ? nullptr : upload_items(items, st);
+            dp.qkv = qkv;
+            dp.out = out;
+            dp.q_norm = L.q_norm; dp.k_norm = L.k_norm; dp.sinks = L.sinks; dp.inv_freq = inv_freq;
+            dp.cache = L.kv4;
+            dp.scratch = scratch; dp.scratch2 = scratch2;
+            dp.tickets = tickets; dp.tickets2 = tickets + n_subs;
+            dp.is_swa = L.is_swa; dp.has_rope = L.has_rope;
+            dp.qkv_dtype = qkv_dtype; dp.out_dtype = out_dtype;
+            dp.error_flag = dec_err;
+            time_mark(st);
+            CK(launch_decode_kv4(dp, inline_items ? items.data() : nullptr, int(items.size()), st));
+            time_mark(st);
+            launches++;
+            if (!inline_items) mark_ring_used(dp.items, st);
+            return;
+        }
         DecParams dp{};
         dp.items = inline_items ? nullptr : upload_items(items, st);
         dp.qkv = qkv;
@@ -531,9 +554,22 @@ struct flint_attn {
 extern "C" {
 
 flint_attn *flint_attn_open(const flint_attn_config *cfg, char *err, int32_t err_len) {
+    return flint_attn_open_kv(cfg, nullptr, err, err_len);
+}
+
+flint_attn *flint_attn_open_kv(const flint_attn_config *cfg, const flint_attn_kv_options *opt, char *err,
+                               int32_t err_len) {
     flint_attn *a = nullptr;
     try {
         if (!cfg) throw std::runtime_error("null config");
+        const int kv_format = opt ? opt->kv_format : int(FLINT_ATTN_KV_F16), first_tokens = opt ? opt->first_tokens : 0;
+        if (kv_format != FLINT_ATTN_KV_F16 && kv_format != FLINT_ATTN_KV_INT4) throw std::runtime_error("bad kv_format");
+        if (first_tokens < 0 || first_tokens > kMaxFirstTokens)
+            throw std::runtime_error("first_tokens must be 0 to " + std::to_string(kMaxFirstTokens));
+        if (first_tokens > 0 && kv_format != FLINT_ATTN_KV_INT4)
+            throw std::runtime_error("first tokens are kept by handles with a 4-bit cache only");
+        if (kv_format == FLINT_ATTN_KV_INT4 && cfg->kv_ranks > 1)
+            throw std::runtime_error("a 4-bit KV cache cannot be sharded by key range");
         if (cfg->n_layers <= 0 || !cfg->layer_is_swa || !cfg->layer_has_rope) throw std::runtime_error("bad layer table");
         if (cfg->max_seqs <= 0 || cfg->n_ctx <= 0) throw std::runtime_error("max_seqs and n_ctx must be positive");
         const int ranks = cfg->kv_ranks > 1 ? cfg->kv_ranks : 1;
@@ -555,6 +591,8 @@ flint_attn *flint_attn_open(const flint_attn_config *cfg, char *err, int32_t err
         a->n_ctx = cfg->n_ctx;
         a->kv_rank = cfg->kv_rank;
         a->kv_ranks = ranks;
+        a->kv_format = kv_format;
+        a->first_tokens = first_tokens;
         a->sm_count = prop.multiProcessorCount;
         a->target_items = a->sm_count * 2;
         a->pos.assign(cfg->max_seqs, 0);
@@ -572,6 +610,7 @@ flint_attn *flint_attn_open(const flint_attn_config *cfg, char *err, int32_t err
         for (int i = 0; i < kRing; i++) CK(cudaEventCreateWithFlags(&a->ring_ev[i], cudaEventDisableTiming));
         CK(decode_kernel_setup());
         CK(prefill_kernel_setup());
+        CK(decode_kv4_setup());
         CK(cudaMalloc(&a->dec_err, sizeof(int)));
         CK(cudaMemset(a->dec_err, 0, sizeof(int)));
         float freq[kHeadDim / 2];
@@ -596,6 +635,25 @@ flint_attn *flint_attn_open(const flint_attn_config *cfg, char *err, int32_t err
                 L.n_slots = std::max(1, L.kv_hi - L.kv_lo);
             }
             L.paged = !L.is_swa && cfg->kv_pages > 0;
+            CK(cudaMalloc(&L.q_norm, kHeadDim * sizeof(float)));
+            CK(cudaMalloc(&L.k_norm, kHeadDim * sizeof(float)));
+            CK(cudaMalloc(&L.sinks, kNHead * sizeof(float)));
+            if (kv_format == FLINT_ATTN_KV_INT4) {
+                L.kv4.first_tokens = L.is_swa ? first_tokens : 0;
+                L.kv4.blocks_per_seq = L.is_swa ? kKv4RingBlocks + (first_tokens > 0 ? 1 : 0)
+                                                : (L.n_slots + kKv4BlockKeys - 1) / kKv4BlockKeys;
+                L.kv4.block_mask = L.is_swa ? uint32_t(kKv4RingBlocks - 1) : 0xFFFFFFFFu;
+                if (L.is_swa) L.n_slots += first_tokens;
+                if (L.paged) {
+                    L.kv4.block_table = a->table_dev;
+                    L.kv4.table_stride = a->pages_per_seq;
+                }
+                const size_t bytes = (L.paged ? size_t(cfg->kv_pages) : size_t(cfg->max_seqs) * L.kv4.blocks_per_seq) *
+                                     kNHeadKv * kKv4BlockBytes;
+                CK(cudaMalloc(&L.kv4.blocks, bytes));
+                CK(cudaMemset(L.kv4.blocks, 0, bytes));
+                continue;
+            }
             const size_t bytes = L.paged ? size_t(cfg->kv_pages) * kNHeadKv * kPageKeys * kHeadDim * sizeof(__half)
                                          : size_t(cfg->max_seqs) * kNHeadKv * L.n_slots * kHeadDim * sizeof(__half);
             CK(cudaMalloc(&L.k, bytes));
@@ -618,9 +676,6 @@ flint_attn *flint_attn_open(const flint_attn_config *cfg, char *err, int32_t err
                     CK(cudaMemcpy(L.kv_maps, maps, sizeof(maps), cudaMemcpyHostToDevice));
                 }
             }
-            CK(cudaMalloc(&L.q_norm, kHeadDim * sizeof(float)));
-            CK(cudaMalloc(&L.k_norm, kHeadDim * sizeof(float)));
-            CK(cudaMalloc(&L.sinks, kNHead * sizeof(float)));
         }
         CK(cudaDeviceSynchronize());
         return a;
@@ -863,6 +918,7 @@ static void prefill_impl(flint_attn *a, int layer, int seq, int n_tok, const voi
     if (a->kv_ranks > 1 && !L.is_swa && !partial_o)
         throw std::runtime_error("full layers of a KV-sharded handle need prefill_partial + prefill_combine");
     if (partial_o && L.is_swa) throw std::runtime_error("sliding-window layers are not sharded: use prefill_dev");
+    if (partial_o && L.kv4.blocks) throw std::runtime_error("partial records are not kept for a 4-bit cache");
     if (partial_o && !partial_ml) throw std::runtime_error("null partial buffer");
     if ((qkv_dtype != kDtypeF32 && qkv_dtype != kDtypeBf16) ||
         (!partial_o && out_dtype != kDtypeF32 && out_dtype != kDtypeBf16))
@@ -872,9 +928,16 @@ static void prefill_impl(flint_attn *a, int layer, int seq, int n_tok, const voi
     pp.qkv = qkv; pp.out = out;
     pp.qkv_dtype = qkv_dtype; pp.out_dtype = out_dtype;
     pp.q_norm = L.q_norm; pp.k_norm = L.k_norm; pp.sinks = L.sinks; pp.inv_freq = a->inv_freq;
-    pp.k_cache = L.k + (L.paged ? 0 : size_t(seq) * kNHeadKv * L.n_slots * kHeadDim);
-    pp.v_cache = L.v + (L.paged ? 0 : size_t(seq) * kNHeadKv * L.n_slots * kHeadDim);
-    if (L.paged) {
+    if (L.kv4.blocks) {
+        pp.kv4 = L.kv4;
+        pp.seq = seq;
+        if (!L.is_swa) pp.stage_rows = a->n_ctx;
+        if (L.paged) a->ensure_pages(seq, p0 + n_tok - 1, st);
+    } else {
+        pp.k_cache = L.k + (L.paged ? 0 : size_t(seq) * kNHeadKv * L.n_slots * kHeadDim);
+        pp.v_cache = L.v + (L.paged ? 0 : size_t(seq) * kNHeadKv * L.n_slots * kHeadDim);
+    }
+    if (L.paged && !L.kv4.blocks) {
         a->ensure_pages(seq, p0 + n_tok - 1, st);
         pp.block_table = a->table_dev + size_t(seq) * a->pages_per_seq;
         pp.n_pages = a->kv_pages;
@@ -1088,6 +1151,91 @@ int32_t flint_attn_n_slots(const flint_attn *a, int32_t layer) {
     return a->layers[layer].n_slots;
 }
 
+// Rows of n sequences between a layer's cache and dense arrays [n][4][n_rows][128] on the device.
+static void kv_rows(flint_attn *a, int layer, int n, const int32_t *seqs, const int32_t *pos0, int n_rows, void *k, void *v,
+                    int dtype, cudaStream_t st, bool store) {
+    CK(cudaSetDevice(a->device));
+    if (layer < 0 || layer >= int(a->layers.size())) throw std::runtime_error("layer index out of range");
+    Layer &L = a->layers[layer];
+    if (!seqs || !pos0 || !k || !v) throw std::runtime_error("null pointer");
+    a->check_seqs(n, seqs);
+    if (dtype != kDtypeF32 && dtype != kDtypeBf16 && dtype != kDtypeF16) throw std::runtime_error("bad dtype");
+    if (a->kv_ranks > 1 && !L.is_swa) throw std::runtime_error("rows of a layer sharded by key range are not moved by position");
+    if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)
+        throw std::runtime_error("K/V rows must start on a 16-byte boundary");
+    if (n_rows <= 0) throw std::runtime_error("row count out of range");
+    for (int i = 0; i < n; i++)
+        if (pos0[i] < 0 || pos0[i] > a->n_ctx - n_rows) throw std::runtime_error("row range out of the context");
+    if (store) {
+        std::vector<int32_t> sorted(seqs, seqs + n);
+        std::sort(sorted.begin(), sorted.end());
+        if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
+            throw std::runtime_error("a sequence appears twice in one store");
+    }
+    if (store && L.paged) {  // all or nothing, as in decode
+        size_t want = 0;
+        for (int i = 0; i < n; i++) want += size_t(std::max(0, (pos0[i] + n_rows - 1) / kPageKeys + 1 - a->seq_blocks[seqs[i]]));
+        if (want > a->free_pages.size())
+            throw std::runtime_error("KV page pool exhausted (" + std::to_string(a->kv_pages) + " pages of 64 keys)");
+        for (int i = 0; i < n; i++) a->ensure_pages(seqs[i], pos0[i] + n_rows - 1, st);
+    }
+    KvRowsParams kp{};
+    kp.cache = L.kv4;
+    kp.k_cache = L.k; kp.v_cache = L.v;
+    if (L.paged) {
+        kp.cache.block_table = a->table_dev;
+        kp.cache.table_stride = a->pages_per_seq;
+    }
+    kp.n_slots = L.n_slots;
+    kp.is_swa = L.is_swa;
+    kp.dtype = dtype;
+    kp.n_rows = n_rows;
+    kp.head_stride = (long long)n_rows * kHeadDim;
+    kp.seq_stride = kp.head_stride * kNHeadKv;
+    const size_t step = size_t(kKvRowsSeqs) * kp.seq_stride * (dtype == kDtypeF32 ? 4 : 2);
+    for (int i0 = 0; i0 < n; i0 += kKvRowsSeqs) {
+        const int m = std::min(kKvRowsSeqs, n - i0);
+        KvRowsSeqs ks;
+        memcpy(ks.seq, seqs + i0, size_t(m) * sizeof(int32_t));
+        memcpy(ks.pos0, pos0 + i0, size_t(m) * sizeof(int32_t));
+        kp.k = static_cast<char *>(k) + size_t(i0 / kKvRowsSeqs) * step;
+        kp.v = static_cast<char *>(v) + size_t(i0 / kKvRowsSeqs) * step;
+        CK(store ? launch_kv_store(kp, ks, m, st) : launch_kv_load(kp, ks, m, st));
+        a->launches++;
+    }
+}
+
+// read_kv / write_kv of a 4-bit cache: the rows go through a half-precision staging buffer on the device.
+static void kv4_copy(flint_attn *a, Layer &L, int seq, int slot0, int n, uint16_t *k, uint16_t *v, bool to_host) {
+    if (n == 0) return;
+    const size_t bytes = size_t(kNHeadKv) * n * kHeadDim * 2;
+    a->ensure_io(2 * bytes);
+    char *dk = static_cast<char *>(a->io_dev), *dv = dk + bytes;
+    if (L.paged && !to_host) a->ensure_pages(seq, slot0 + n - 1, nullptr);
+    KvRowsParams kp{};
+    kp.cache = L.kv4;
+    kp.is_swa = L.is_swa;
+    kp.raw_slots = 1;
+    kp.dtype = kDtypeF16;
+    kp.n_rows = n;
+    kp.head_stride = (long long)n * kHeadDim;
+    kp.k = dk; kp.v = dv;
+    KvRowsSeqs ks{};
+    ks.seq[0] = seq;
+    ks.pos0[0] = slot0;
+    if (!to_host) {
+        CK(cudaMemcpy(dk, k, bytes, cudaMemcpyHostToDevice));
+        CK(cudaMemcpy(dv, v, bytes, cudaMemcpyHostToDevice));
+        CK(launch_kv_store(kp, ks, 1, nullptr));
+    } else {
+        CK(launch_kv_load(kp, ks, 1, nullptr));
+        CK(cudaMemcpy(k, dk, bytes, cudaMemcpyDeviceToHost));
+        CK(cudaMemcpy(v, dv, bytes, cudaMemcpyDeviceToHost));
+    }
+    a->launches++;
+    CK(cudaDeviceSynchronize());
+}
+
 static void kv_copy(flint_attn *a, int layer, int seq, int slot0, int n, uint16_t *k, uint16_t *v, bool to_host) {
     CK(cudaSetDevice(a->device));
     if (layer < 0 || layer >= int(a->layers.size())) throw std::runtime_error("layer index out of range");
@@ -1095,6 +1243,10 @@ static void kv_copy(flint_attn *a, int layer, int seq, int slot0, int n, uint16_
     if (seq < 0 || seq >= a->max_seqs) throw std::runtime_error("sequence index out of range");
     if (slot0 < 0 || n < 0 || slot0 + n > L.n_slots) throw std::runtime_error("slot range out of bounds");
     CK(cudaDeviceSynchronize());
+    if (L.kv4.blocks) {
+        kv4_copy(a, L, seq, slot0, n, k, v, to_host);
+        return;
+    }
     if (L.paged) {  // block by block through the table; writing allocates the pages it needs
         if (!to_host && n > 0) {
             a->ensure_pages(seq, slot0 + n - 1, nullptr);
@@ -1154,7 +1306,27 @@ int32_t flint_attn_write_kv(flint_attn *a, int32_t layer, int32_t seq, int32_t s
 
 void *flint_attn_kv_dev(flint_attn *a, int32_t layer, int32_t which) {
     if (layer < 0 || layer >= int(a->layers.size())) return nullptr;
+    if (a->layers[layer].kv4.blocks) return which == 0 ? static_cast<void *>(a->layers[layer].kv4.blocks) : nullptr;
     return which == 0 ? static_cast<void *>(a->layers[layer].k) : static_cast<void *>(a->layers[layer].v);
+}
+
+int32_t flint_attn_store_kv_dev(flint_attn *a, int32_t layer, int32_t n, const int32_t *seqs, const int32_t *pos0,
+                                int32_t n_rows, const void *k_dev, const void *v_dev, int32_t dtype, void *cuda_stream,
+                                char *err, int32_t err_len) {
+    API_TRY
+    kv_rows(a, layer, n, seqs, pos0, n_rows, const_cast<void *>(k_dev), const_cast<void *>(v_dev), dtype,
+            cudaStream_t(cuda_stream), true);
+    return 0;
+    API_CATCH(-1)
+}
+
+int32_t flint_attn_load_kv_dev(flint_attn *a, int32_t layer, int32_t n, const int32_t *seqs, const int32_t *pos0,
+                               int32_t n_rows, void *k_dev, void *v_dev, int32_t dtype, void *cuda_stream, char *err,
+                               int32_t err_len) {
+    API_TRY
+    kv_rows(a, layer, n, seqs, pos0, n_rows, k_dev, v_dev, dtype, cudaStream_t(cuda_stream), false);
+    return 0;
+    API_CATCH(-1)
 }
 
 int32_t flint_attn_seq_release(flint_attn *a, int32_t seq) {

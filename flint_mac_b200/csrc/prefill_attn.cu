@@ -25,6 +25,7 @@
 #include <utility>
 #include <vector>
 
+#include "kv4.cuh"
 #include "ptx.cuh"
 #include "tc5.cuh"
 
@@ -84,7 +85,13 @@ struct PfArgs {
     // Key-range shard of a full layer (context-parallel prefill): this device holds keys [kr_lo, kr_hi) only; a unit's
     // keys are clipped to it, the sink enters on the device that says so, and the output is an un-normalised partial.
     int kr_lo, kr_hi, with_sink, cp_partial;
+    // Sliding-window layer with first tokens that stay visible: rows [0, first_rows) of the K/V staging hold positions
+    // [0, first_tokens), the window's rows follow.
+    int first_tokens, first_rows;
 };
+
+// What a query sees, beyond the causal limit; the attention kernel is compiled for each.
+enum { kFull = 0, kWindow = 1, kWindowFirst = 2 };
 
 // ------------------------------------------------------------------------------------------------- prologue
 // Packed two-float arithmetic (sm_100): a 64-bit register holds two floats.
@@ -122,11 +129,15 @@ struct PrologueArgs {
     const float *q_norm, *k_norm, *inv_freq;
     __half *k_cache, *v_cache;  // [4][n_slots][128] of this sequence
     __half *q_st;               // [32][n_tok][128], pre-scaled by log2(e)/sqrt(128)
-    __half *k_st, *v_st;        // [4][n_hist + n_tok][128] (ring layers only; null otherwise)
+    __half *k_st, *v_st;        // [4][st_rows][128] (ring layers and 4-bit caches; null otherwise); new token t in row st_new + t
     int n_slots, is_swa, has_rope, qkv_dtype;
     int p0, n_tok, n_hist;
     const int32_t *block_table;  // paged full layer: k_cache / v_cache are page pools, slot = page * 64 + pos % 64
     int kv_lo, kv_hi;            // full layer: positions this device's cache holds (slot = pos - kv_lo); others are not stored
+    int st_rows, st_new;
+    Kv4Cache kv4;                // 4-bit cache (the other cache pointers are null), and the sequence's index into it
+    int seq;
+    int first_rows;              // rows of the staging in front of the history that take positions [0, first_tokens)
 };
 
 // A lane's share of an input row of 128: dims 4*sub..4*sub+3 and the four 64 further on, the partners of the first
@@ -204,12 +215,46 @@ __device__ __forceinline__ void pf_norm_rope8(float (&x)[8], const unsigned long
     for (int i = 0; i < 4; i++) unpack_f32x2(v[i], x[2 * i], x[2 * i + 1]);
 }
 
+// A new token's K or V row with a 4-bit cache: half-precision values to the staging, codes to the cache.  The lane's eight
+// values belong to two groups: dims 4 sub .. + 3 to group sub / 8, the four 64 further on to the group two after it; each
+// group lives in eight neighbouring lanes.
+__device__ __forceinline__ void store_row_kv4(const PrologueArgs &a, const float (&x)[8], int pos, int t, int kvh, bool is_v,
+                                              int sub, bool to_cache) {
+    __half *st = is_v ? a.v_st : a.k_st;
+    pf_store_half44(st + (size_t(kvh) * a.st_rows + a.st_new + t) * kHeadDim + 4 * sub, x);
+    const bool to_first = a.is_swa && pos < a.kv4.first_tokens;
+    if (to_first && a.first_rows > 0) pf_store_half44(st + (size_t(kvh) * a.st_rows + pos) * kHeadDim + 4 * sub, x);
+    if (!to_cache && !to_first) return;  // (the same for the whole token)
+    unsigned char *block = kv4_block(a.kv4, a.seq, kvh, pos >> 6);
+#pragma unroll
+    for (int hi = 0; hi < 2; hi++) {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = __half2float(__float2half_rn(x[4 * hi + j]));
+        __half2 dl;
+        const uint32_t codes = kv4_quantise4(v, dl);
+        const int g = (sub >> 3) + 2 * hi;
+        auto put = [&](unsigned char *blk, int row) {
+            *reinterpret_cast<uint16_t *>(blk + (is_v ? kKv4VCodes : kKv4KCodes) + kv4_chunk(row, g) + (sub & 7) * 2) = uint16_t(codes);
+            if ((sub & 7) != 0) return;
+            if (is_v) {
+                *reinterpret_cast<__half *>(blk + kv4_v_group(row, g)) = __low2half(dl);
+                *reinterpret_cast<__half *>(blk + kv4_v_group(row, g) + 16) = __high2half(dl);
+            } else {
+                *reinterpret_cast<__half2 *>(blk + kv4_k_group(row, g)) = dl;
+            }
+        };
+        if (to_cache) put(block, pos & 63);
+        if (to_first) put(kv4_first_block(a.kv4, a.seq, kvh), pos);
+    }
+}
+
 constexpr int kProRows = 10;  // input rows (heads) per warp: a token's 40 rows (32 q, 4 k, 4 v) take the four warps of a CTA
 
 // New-token pass: one CTA of four warps per token, each warp with ten of its 40 head rows, two rows per pass (one per
 // half-warp).  All loads of a warp go out before the first row is touched.  The token's 64 (cos, sin) pairs are
 // evaluated once, by the first warp, and shared through shared memory.
-template <bool kBf16>
+template <bool kBf16, bool kKv4>
 __device__ __forceinline__ void prologue_rows(const PrologueArgs &a) {
     __shared__ float2 s_cs[kHeadDim / 2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -241,6 +286,15 @@ __device__ __forceinline__ void prologue_rows(const PrologueArgs &a) {
     // On a ring layer tokens t and t + 1024 of one launch share a slot: only the last token that maps to a slot
     // stores there, so the ring's final contents do not depend on the order in which the CTAs run.
     const bool to_cache = mine && (!a.is_swa || t + kSwaRing >= a.n_tok);
+    if (kKv4 && a.first_rows > 0 && t == 0) {  // the product takes the first tokens' rows 16 at a time: those past them count as 0
+        const int from = a.kv4.first_tokens, to = (from + 15) & ~15;
+        for (int i = threadIdx.x; i < (to - from) * kNHeadKv * (kHeadDim / 8); i += 128) {
+            const int c = i % (kHeadDim / 8), r = from + i / (kHeadDim / 8) / kNHeadKv, kvh = i / (kHeadDim / 8) % kNHeadKv;
+            const size_t off = (size_t(kvh) * a.st_rows + r) * kHeadDim + 8 * c;
+            *reinterpret_cast<uint4 *>(a.k_st + off) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(a.v_st + off) = make_uint4(0, 0, 0, 0);
+        }
+    }
     // paged layer: [page][kv head][64 slots][128] instead of [kv head][slot][128]
     const size_t page = a.block_table ? size_t(a.block_table[pos >> 6]) : 0;
     __syncthreads();
@@ -276,6 +330,10 @@ __device__ __forceinline__ void prologue_rows(const PrologueArgs &a) {
                                               pack_f32x2(k1.z, k1.w)};
             pf_norm_rope8(x, wk, cs, sn, nsn, rope, 1.0f);
         }
+        if (kKv4) {
+            store_row_kv4(a, x, pos, t, kvh, !is_k, sub, to_cache);
+            continue;
+        }
         if (to_cache) {
             __half *cache = is_k ? a.k_cache : a.v_cache;
             const size_t crow = a.block_table ? (page * kNHeadKv + kvh) * 64 + (pos & 63) : size_t(kvh) * a.n_slots + slot;
@@ -283,7 +341,7 @@ __device__ __forceinline__ void prologue_rows(const PrologueArgs &a) {
         }
         if (a.k_st) {
             __half *st = is_k ? a.k_st : a.v_st;
-            pf_store_half44(st + (size_t(kvh) * (a.n_hist + a.n_tok) + a.n_hist + t) * kHeadDim + 4 * sub, x);
+            pf_store_half44(st + (size_t(kvh) * a.st_rows + a.st_new + t) * kHeadDim + 4 * sub, x);
         }
     }
 }
@@ -299,18 +357,18 @@ __global__ void __launch_bounds__(256) k_prefill_history(const PrologueArgs a) {
     const int r = int(row / kNHeadKv), kvh = int(row % kNHeadKv);
     const int pos = a.p0 - a.n_hist + r, slot = pos & (kSwaRing - 1);
     const size_t src = (size_t(kvh) * a.n_slots + slot) * kHeadDim + 4 * lane;
-    const size_t dst = (size_t(kvh) * (a.n_hist + a.n_tok) + r) * kHeadDim + 4 * lane;
+    const size_t dst = (size_t(kvh) * a.st_rows + r) * kHeadDim + 4 * lane;
     *reinterpret_cast<uint2 *>(a.k_st + dst) = *reinterpret_cast<const uint2 *>(a.k_cache + src);
     *reinterpret_cast<uint2 *>(a.v_st + dst) = *reinterpret_cast<const uint2 *>(a.v_cache + src);
 }
 
 // (one kernel per input type: the bf16 one holds half the registers in flight and fits eight CTAs on an SM)
-template <bool kBf16>
+template <bool kBf16, bool kKv4>
 __global__ void __launch_bounds__(128, kBf16 ? 8 : 5) k_prefill_prologue(const PrologueArgs a) {
     // the attention kernel of this prefill may be scheduled as soon as SMs come free: it waits for this grid's
     // completion (griddepcontrol.wait) before it reads anything written here
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-    prologue_rows<kBf16>(a);
+    prologue_rows<kBf16, kKv4>(a);
 }
 
 // ------------------------------------------------------------------------------------------------- attention
@@ -352,12 +410,13 @@ enum {
 // key range is split, one range of its key tiles.
 struct Unit {
     int t0, kvh, q_first, q_last, klo, n_keys, n_tiles, split;
+    int first;  // 1: tile 0 holds the first tokens, the window's tiles follow
 };
 // Units are handed out longest first: late query blocks (full 544-key bands) before the first 16 blocks of the
 // prompt, whose bands are shorter, so that the CTAs that get one unit more than the others get short ones.
 // (Host and device: the host's schedule uses the same tile counts.)
 __host__ __device__ inline Unit unit_geom_of(int u, int n_tok, int p0, int is_swa, int key_row0, int n_ksplit,
-                                             int kr_lo = 0, int kr_hi = 0x7fffffff) {
+                                             int kr_lo = 0, int kr_hi = 0x7fffffff, int first_tokens = 0) {
     Unit g;
     const int uq = u / n_ksplit;
     g.split = u % n_ksplit;
@@ -379,10 +438,15 @@ __host__ __device__ inline Unit unit_geom_of(int u, int n_tok, int p0, int is_sw
         g.n_keys = left < (kt_b - kt_a) * kBN ? left : (kt_b - kt_a) * kBN;
         g.n_tiles = kt_b - kt_a;
     }
+    // a query at q sees the first tokens below q - 512 through the extra tile, those from there on through its window
+    g.first = first_tokens > 0 && g.q_last > kHist ? 1 : 0;
+    g.n_tiles += g.first;
     return g;
 }
+template <int kKind>
 __device__ __forceinline__ Unit unit_geom(const PfArgs &a, int u) {
-    return unit_geom_of(u, a.n_tok, a.p0, a.is_swa, a.key_row0, a.n_ksplit, a.kr_lo, a.kr_hi);
+    return unit_geom_of(u, a.n_tok, a.p0, a.is_swa, a.key_row0, a.n_ksplit, a.kr_lo, a.kr_hi,
+                        kKind == kWindowFirst ? a.first_tokens : 0);
 }
 
 // The i-th unit of this CTA, or -1.  The host balances the units over the CTAs by their tile counts and lays each
@@ -408,12 +472,13 @@ __device__ __forceinline__ int unit_at(const PfArgs &a, const int *local, int i)
 // run at half rate).
 // (compiled per layer kind and output type: the code of the other three combinations would only take up
 // instruction cache, which the softmax warps are short of)
-template <bool kSwa, bool kOutF32>
+template <int kKind, bool kOutF32>
 __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_constant__ CUtensorMap tm_q,
                                                                   const __grid_constant__ CUtensorMap tm_k,
                                                                   const __grid_constant__ CUtensorMap tm_v,
                                                                   const __grid_constant__ CUtensorMap tm_o,
                                                                   const PfArgs a) {
+    constexpr bool kSwa = kKind != kFull;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t base = smem_u32(smem_raw);
     unsigned char *gen = smem_raw;
@@ -478,7 +543,8 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
                 g++;
                 if (use >= 1 && !wait_bar(bar(kBarSlotEmpty + slot), (use - 1) & 1)) return false;
                 const uint32_t dst = base + kOffKV + slot * kTileBytes, full = bar(kBarSlotFull + slot);
-                const int row = un.klo + kt * kBN - a.key_row0;
+                int row = un.klo + kt * kBN - a.key_row0;
+                if (kKind == kWindowFirst) row = kt < un.first ? 0 : row + a.first_rows - un.first * kBN;
                 tc5::mbar_expect_tx(full, kTileBytes);
                 if (a.block_table) {
                     // a 128-key tile is two pages; a page past the sequence's last one holds only keys that every
@@ -508,7 +574,7 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
             for (int i = 0; ok; i++) {
                 const int u = unit_at(a, sched_local, i);
                 if (u < 0) break;
-                const Unit un = unit_geom(a, u);
+                const Unit un = unit_geom<kKind>(a, u);
                 // order of need: Q0, K(0), Q1, V(0), K(1), V(1), ...
                 ok = load_q(un, 0, i) && load_tile(&tm_k, un, 0) && load_q(un, 1, i);
                 for (int kt = 0; kt < un.n_tiles && ok; kt++) {
@@ -542,7 +608,13 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
             Unit un;
         };
         // keys of a tile that any query of the unit can see, rounded up to the MMA's N granularity
-        auto tile_n = [&](const Cursor &c) { return min(kBN, (c.un.n_keys - c.kt * kBN + 15) & ~15); };
+        auto tile_n = [&](const Cursor &c) {
+            if (kKind == kWindowFirst) {
+                if (c.kt < c.un.first) return (a.first_tokens + 15) & ~15;
+                return min(kBN, (c.un.n_keys - (c.kt - c.un.first) * kBN + 15) & ~15);
+            }
+            return min(kBN, (c.un.n_keys - c.kt * kBN + 15) & ~15);
+        };
         auto advance = [&](Cursor &c) {  // returns false at the end of the stream
             if (c.kt + 1 < c.un.n_tiles) {
                 c.kt++;
@@ -551,7 +623,7 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
                 if (u < 0) return false;
                 c.i++;
                 c.kt = 0;
-                c.un = unit_geom(a, u);
+                c.un = unit_geom<kKind>(a, u);
             }
             c.j++;
             return true;
@@ -592,7 +664,7 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
             return true;
         };
         if (unit_at(a, sched_local, 0) >= 0) {
-            Cursor cur{0, 0, 0, unit_geom(a, unit_at(a, sched_local, 0))};
+            Cursor cur{0, 0, 0, unit_geom<kKind>(a, unit_at(a, sched_local, 0))};
             ok = issue_qk(cur);
             while (ok) {
                 Cursor nxt = cur;
@@ -621,7 +693,7 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
         for (int i = 0; ok; i++) {
         const int u = unit_at(a, sched_local, i);
         if (u < 0) break;
-        const Unit un = unit_geom(a, u);
+        const Unit un = unit_geom<kKind>(a, u);
         const int kvh = un.kvh, t0 = un.t0, klo = un.klo, n_keys = un.n_keys, n_tiles = un.n_tiles;
         const int qt_first = un.q_first + w * kQPos;  // first / last position of this Q tile
         const int qt_last = min(qt_first + kQPos - 1, un.q_last);
@@ -636,17 +708,23 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
             ok = __all_sync(0xffffffffu, wait_bar(bar(kBarSReady + w), j & 1));  // warp-uniform for tcgen05.ld
             if (!ok) break;
             tc5::fence_after_sync();
-            const int kbase = klo + kt * kBN;
-            const int n_cols = min(kBN, (n_keys - kt * kBN + 15) & ~15);  // columns the MMA wrote (same as the issuer)
+            const bool first_tile = kKind == kWindowFirst && kt < un.first;
+            const int kw = kKind == kWindowFirst ? kt - un.first : kt;  // tile of the window
+            const int kbase = first_tile ? 0 : klo + kw * kBN;
+            // columns the MMA wrote (same as the issuer)
+            const int n_cols = first_tile ? (a.first_tokens + 15) & ~15 : min(kBN, (n_keys - kw * kBN + 15) & ~15);
             const int n_chunks = (n_cols + 31) >> 5;
             // visible columns of this row form one range [c_lo, c_hi] (prefill.metal:212); on a key-range shard the
             // unit's keys also end with the shard (k_end), before the causal limit of later queries
             const int k_end = klo + n_keys - 1;
-            const int c_hi = min(qpos, k_end) - kbase;
-            const int c_lo = kSwa ? qpos - kHist - kbase : -(1 << 30);
+            // (in the tile of the first tokens: those in front of the row's window, which may be none)
+            const int n_front = min(a.first_tokens, qpos - kHist);
+            const int c_hi = first_tile ? (n_front > 0 ? n_front - 1 : 1 << 20) : min(qpos, k_end) - kbase;
+            const int c_lo = first_tile ? (n_front > 0 ? 0 : 1 << 20) : kSwa ? qpos - kHist - kbase : -(1 << 30);
             // Per 32-column chunk, for the whole Q tile: 0 = every row sees every key (no per-element mask),
             // 1 = mixed, 2 = no row sees any key.  Only the two ends of the band are mixed.
             auto chunk_kind = [&](int ch) {
+                if (first_tile) return 1;
                 const int key_lo = kbase + ch * 32, key_hi = key_lo + 31;
                 if (key_lo > qt_last || key_lo > k_end || (kSwa && key_hi < qt_first - kHist)) return 2;
                 if (key_hi <= qt_first && key_hi <= k_end && (!kSwa || key_lo >= qt_last - kHist)) return 0;
@@ -939,13 +1017,14 @@ cudaError_t make_out_map(CUtensorMap *map, void *base, int n_tok, int out_dtype)
 // tiles than others.  Greedy longest-first assignment to the least loaded CTA by (key tiles + one tile of per-unit
 // overhead); unit indices are already ordered longest first.  The table is kept until the geometry changes.
 cudaError_t build_schedule(PrefillWorkspace &ws, const PfArgs &a, int n_units, int grid, cudaStream_t stream) {
-    const int key[5] = {a.n_tok, a.p0, a.is_swa * 256 + a.n_ksplit, a.key_row0 ^ (a.kr_hi * 31), grid};
+    const int key[5] = {a.n_tok, a.p0, (a.first_tokens << 16) + a.is_swa * 256 + a.n_ksplit, a.key_row0 ^ (a.kr_hi * 31), grid};
     if (ws.sched && memcmp(key, ws.sched_key, sizeof(key)) == 0) return cudaSuccess;
     std::vector<std::vector<int>> lists(grid);
     std::priority_queue<std::pair<int, int>, std::vector<std::pair<int, int>>, std::greater<std::pair<int, int>>> heap;
     for (int b = 0; b < grid; b++) heap.push({0, b});
     for (int u = 0; u < n_units; u++) {
-        const int tiles = unit_geom_of(u, a.n_tok, a.p0, a.is_swa, a.key_row0, a.n_ksplit, a.kr_lo, a.kr_hi).n_tiles;
+        const int tiles = unit_geom_of(u, a.n_tok, a.p0, a.is_swa, a.key_row0, a.n_ksplit, a.kr_lo, a.kr_hi,
+                                       a.first_tokens).n_tiles;
         const auto [load, b] = heap.top();
         heap.pop();
         lists[b].push_back(u);
@@ -986,10 +1065,12 @@ cudaError_t prefill_kernel_setup() {
     }
     int dev = 0;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&g_sm_count, cudaDevAttrMultiProcessorCount, dev);
-    cudaError_t e = cudaFuncSetAttribute(k_prefill_attn<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_prefill_attn<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_prefill_attn<true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_prefill_attn<true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    cudaError_t e = cudaFuncSetAttribute(k_prefill_attn<kFull, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_prefill_attn<kFull, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_prefill_attn<kWindow, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_prefill_attn<kWindow, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_prefill_attn<kWindowFirst, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_prefill_attn<kWindowFirst, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     return e;
 }
 
@@ -1002,10 +1083,16 @@ void prefill_workspace_free(PrefillWorkspace &ws) {
 cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStream_t stream, int *n_launches) {
     *n_launches = 0;
     const int T = p.n_tok;
-    const int n_hist = p.is_swa ? (p.p0 < kHist ? p.p0 : kHist) : 0;
+    const bool kv4 = p.kv4.blocks != nullptr;
+    const bool staged = p.is_swa || kv4;  // K/V rows come from linear staging, not from the cache itself
+    const int n_hist = p.is_swa ? (p.p0 < kHist ? p.p0 : kHist) : kv4 ? p.p0 : 0;
+    // (only queries past the first 512 + 1 have first tokens in front of their window)
+    const int first_tokens = p.is_swa && kv4 && p.p0 + T - 1 > kHist ? p.kv4.first_tokens : 0;
+    const int first_rows = first_tokens > 0 ? kMaxFirstTokens : 0;
+    const int st_new = first_rows + n_hist, st_rows = st_new + T;
     auto up = [](size_t x) { return (x + 1023) / 1024 * 1024; };
     const size_t q_bytes = up(size_t(kNHead) * T * kHeadDim * 2);
-    const size_t kv_bytes = p.is_swa ? up(size_t(kNHeadKv) * (n_hist + T) * kHeadDim * 2) : 0;
+    const size_t kv_bytes = staged ? up(size_t(kNHeadKv) * std::max(st_rows, p.stage_rows) * kHeadDim * 2) : 0;
     // Key-range split: a chunk on a full layer with fewer units than SMs and a long history leaves most of the GPU
     // idle (512 tokens = 64 units) while every unit walks hundreds of key tiles.  Each unit is then cut into ranges
     // of at least 4 key tiles, as many as fit the SMs, and a small kernel merges the partials.
@@ -1046,8 +1133,8 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
     char *wbase = static_cast<char *>(ws.buf);
     int *err_flag = reinterpret_cast<int *>(wbase);
     __half *q_st = reinterpret_cast<__half *>(wbase + 1024);
-    __half *k_st = p.is_swa ? reinterpret_cast<__half *>(wbase + 1024 + q_bytes) : nullptr;
-    __half *v_st = p.is_swa ? reinterpret_cast<__half *>(wbase + 1024 + q_bytes + kv_bytes) : nullptr;
+    __half *k_st = staged ? reinterpret_cast<__half *>(wbase + 1024 + q_bytes) : nullptr;
+    __half *v_st = staged ? reinterpret_cast<__half *>(wbase + 1024 + q_bytes + kv_bytes) : nullptr;
     float *part_o = reinterpret_cast<float *>(wbase + 1024 + q_bytes + 2 * kv_bytes);
     float2 *part_ml = reinterpret_cast<float2 *>(wbase + 1024 + q_bytes + 2 * kv_bytes + part_o_bytes);
 
@@ -1060,18 +1147,45 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
     pa.block_table = p.block_table;
     pa.kv_lo = p.is_swa ? 0 : p.kv_lo;
     pa.kv_hi = p.is_swa ? 0x7fffffff : p.kv_hi;
+    pa.st_rows = st_rows; pa.st_new = st_new;
+    pa.kv4 = p.kv4; pa.seq = p.seq; pa.first_rows = first_rows;
     cudaError_t e;
     // The prologue is launched last, directly in front of the attention kernel, so that the two are neighbours on the
     // stream: the attention kernel is launched with programmatic stream serialisation and sets itself up (tensor
     // memory, barriers, work list) on SMs the prologue has already left.
     auto launch_prologue = [&]() -> cudaError_t {
-        if (n_hist > 0) {
+        if (kv4 && p.p0 > 0) {  // the values of earlier tokens, as the cache holds them
+            KvRowsParams rows{};
+            rows.cache = p.kv4;
+            rows.is_swa = p.is_swa;
+            rows.dtype = kDtypeF16;
+            rows.head_stride = (long long)st_rows * kHeadDim;
+            KvRowsSeqs one{};
+            one.seq[0] = p.seq;
+            one.pos0[0] = p.p0 - n_hist;
+            rows.n_rows = n_hist;
+            rows.k = k_st + size_t(first_rows) * kHeadDim;
+            rows.v = v_st + size_t(first_rows) * kHeadDim;
+            if (cudaError_t le = launch_kv_load(rows, one, 1, stream); le != cudaSuccess) return le;
+            (*n_launches)++;
+            if (first_tokens > 0) {
+                one.pos0[0] = 0;
+                rows.n_rows = std::min(first_tokens, p.p0);
+                rows.k = k_st;
+                rows.v = v_st;
+                if (cudaError_t le = launch_kv_load(rows, one, 1, stream); le != cudaSuccess) return le;
+                (*n_launches)++;
+            }
+        } else if (n_hist > 0) {
             k_prefill_history<<<unsigned((n_hist * kNHeadKv + 7) / 8), 256, 0, stream>>>(pa);
             if (cudaError_t le = cudaGetLastError(); le != cudaSuccess) return le;
             (*n_launches)++;
         }
-        if (pa.qkv_dtype == kDtypeBf16) k_prefill_prologue<true><<<unsigned(T), 128, 0, stream>>>(pa);
-        else k_prefill_prologue<false><<<unsigned(T), 128, 0, stream>>>(pa);
+        const bool bf16 = pa.qkv_dtype == kDtypeBf16;
+        if (kv4 && bf16) k_prefill_prologue<true, true><<<unsigned(T), 128, 0, stream>>>(pa);
+        else if (kv4) k_prefill_prologue<false, true><<<unsigned(T), 128, 0, stream>>>(pa);
+        else if (bf16) k_prefill_prologue<true, false><<<unsigned(T), 128, 0, stream>>>(pa);
+        else k_prefill_prologue<false, false><<<unsigned(T), 128, 0, stream>>>(pa);
         if (cudaError_t le = cudaGetLastError(); le != cudaSuccess) return le;
         (*n_launches)++;
         return cudaSuccess;
@@ -1087,9 +1201,9 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
     else e = make_out_map(&tm_o, p.out, T, p.out_dtype);
     if (e != cudaSuccess) return e;
     if ((e = make_map(&tm_q, q_st, T, kNHead, kQPos, kGqa)) != cudaSuccess) return e;
-    const void *kb = p.is_swa ? static_cast<const void *>(k_st) : static_cast<const void *>(p.k_cache);
-    const void *vb = p.is_swa ? static_cast<const void *>(v_st) : static_cast<const void *>(p.v_cache);
-    const int kv_rows = p.is_swa ? n_hist + T : p.n_slots;
+    const void *kb = staged ? static_cast<const void *>(k_st) : static_cast<const void *>(p.k_cache);
+    const void *vb = staged ? static_cast<const void *>(v_st) : static_cast<const void *>(p.v_cache);
+    const int kv_rows = staged ? st_rows : p.n_slots;
     if (p.block_table) {  // page pool: {128 dims, 64 rows of a page, pages x KV heads}, one 64-row box per load
         if ((e = make_map(&tm_k, kb, 64, p.n_pages * kNHeadKv, 64, 1)) != cudaSuccess) return e;
         if ((e = make_map(&tm_v, vb, 64, p.n_pages * kNHeadKv, 64, 1)) != cudaSuccess) return e;
@@ -1111,6 +1225,7 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
     a.with_sink = p.with_sink;
     a.cp_partial = cp ? 1 : 0;
     a.block_table = p.block_table; a.table_len = p.table_len;
+    a.first_tokens = first_tokens; a.first_rows = first_rows;
     const int n_units = n_units_q * n_ksplit;
     const dim3 grid(n_units < g_sm_count ? n_units : g_sm_count);
     a.n_units = n_units;
@@ -1141,10 +1256,12 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
         cfg.attrs = &attr;
         cfg.numAttrs = no_pdl ? 0 : 1;
         const bool f32 = a.out_dtype == kDtypeF32;
-        if (a.is_swa) e = f32 ? cudaLaunchKernelEx(&cfg, k_prefill_attn<true, true>, tm_q, tm_k, tm_v, tm_o, a)
-                              : cudaLaunchKernelEx(&cfg, k_prefill_attn<true, false>, tm_q, tm_k, tm_v, tm_o, a);
-        else e = f32 ? cudaLaunchKernelEx(&cfg, k_prefill_attn<false, true>, tm_q, tm_k, tm_v, tm_o, a)
-                     : cudaLaunchKernelEx(&cfg, k_prefill_attn<false, false>, tm_q, tm_k, tm_v, tm_o, a);
+        if (first_tokens > 0) e = f32 ? cudaLaunchKernelEx(&cfg, k_prefill_attn<kWindowFirst, true>, tm_q, tm_k, tm_v, tm_o, a)
+                                      : cudaLaunchKernelEx(&cfg, k_prefill_attn<kWindowFirst, false>, tm_q, tm_k, tm_v, tm_o, a);
+        else if (a.is_swa) e = f32 ? cudaLaunchKernelEx(&cfg, k_prefill_attn<kWindow, true>, tm_q, tm_k, tm_v, tm_o, a)
+                                   : cudaLaunchKernelEx(&cfg, k_prefill_attn<kWindow, false>, tm_q, tm_k, tm_v, tm_o, a);
+        else e = f32 ? cudaLaunchKernelEx(&cfg, k_prefill_attn<kFull, true>, tm_q, tm_k, tm_v, tm_o, a)
+                     : cudaLaunchKernelEx(&cfg, k_prefill_attn<kFull, false>, tm_q, tm_k, tm_v, tm_o, a);
     }
     if (e != cudaSuccess) return e;
     (*n_launches)++;

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "attn_common.h"
+#include "kv4.h"
 
 namespace flint {
 
@@ -27,6 +28,13 @@ struct PrefillParams {
     // launch_prefill_combine after the devices have exchanged them.
     float *partial_o = nullptr;
     float *partial_ml = nullptr;
+    // Layer whose cache is held in 4 bits (k_cache, v_cache, block_table above are null then): the K/V rows that the
+    // launch attends to are all staged in half precision, what the cache holds of earlier tokens as the values that it
+    // stands for, this call's own rows as they are; those are quantised into the cache on the way.  A sliding-window layer
+    // with kv4.first_tokens > 0 keeps those first tokens visible to every later query.
+    Kv4Cache kv4;
+    int seq = 0;         // the sequence's index into kv4
+    int stage_rows = 0;  // rows of K/V staging to allocate for at least (a full layer's context length)
 };
 
 // Device scratch that lives with the handle and grows on demand: half-precision staging of the normalised,

@@ -34,7 +34,7 @@ typedef struct flint_attn flint_attn;
 
 /* Element types of the qkv input rows and of the attention output rows.  Row buffers start on a 16-byte boundary
  * (any device allocation does; so does every row of one, a row being 10240 or 20480 bytes). */
-enum { FLINT_ATTN_F32 = 0, FLINT_ATTN_BF16 = 1 };
+enum { FLINT_ATTN_F32 = 0, FLINT_ATTN_BF16 = 1, FLINT_ATTN_F16 = 2 /* rows of flint_attn_store_kv_dev / load_kv_dev only */ };
 
 enum {
     FLINT_ATTN_N_HEAD = 32,
@@ -63,6 +63,30 @@ typedef struct {
 /* src/capi.h:20-21. NULL + message on failure. */
 flint_attn *flint_attn_open(const flint_attn_config *cfg, char *err, int32_t err_len);
 void flint_attn_close(flint_attn *a);
+
+/* ---- K/V caches held in 4 bits, first tokens that stay visible ------------------------------------------
+ * No counterpart in the reference, which caches K and V in half precision (src/engine.mm:509-511).  flint_attn_open_kv
+ * is flint_attn_open with options (NULL: the defaults, all zero):
+ *   kv_format     FLINT_ATTN_KV_INT4: every layer's cache in 4 bits, 80 bytes a row where half precision takes 256.
+ *     A row is one token's 128 values of one KV head, K after norm and rotation, rounded to half as in a half-precision
+ *     cache, in four groups of 32.  A group keeps lo = min, d = half((max - lo) / 15) and codes
+ *     round-half-even((x - lo) / d) limited to 0..15 (0 where d is 0), and stands for lo + code d.  A group with an
+ *     infinity or a NaN in it reads back as NaN.  All calls below work as on a half-precision handle, contiguous and
+ *     paged; a call's own tokens are attended as their half-precision rows, what the cache held before the call as the
+ *     values that it stands for.  Not with kv_ranks > 1, and no partial records (decode_partial, prefill_partial, xchg).
+ *     A prefill behind a cached context on a full layer brings that context into half-precision scratch of the handle
+ *     (n_ctx rows, 2 KB each, once for all layers).
+ *   first_tokens  0 to 64 (4-bit caches only): on sliding-window layers a query at position p sees, besides the last 513
+ *     positions, positions below first_tokens.  Each sequence keeps those rows outside the ring; n_slots is
+ *     1024 + first_tokens there, slots from 1024 on being the first tokens' rows.
+ * A 4-bit cache's device memory (flint_attn_kv_dev, which = 0; which = 1 is NULL) is in the library's own block format. */
+enum { FLINT_ATTN_KV_F16 = 0, FLINT_ATTN_KV_INT4 = 1 };
+typedef struct {
+    int32_t kv_format;
+    int32_t first_tokens;
+} flint_attn_kv_options;
+flint_attn *flint_attn_open_kv(const flint_attn_config *cfg, const flint_attn_kv_options *opt, char *err,
+                               int32_t err_len);
 
 /* src/capi.h:23,25 (per sequence here: the reference is single-session). */
 int32_t flint_attn_n_ctx(const flint_attn *a);
@@ -202,6 +226,21 @@ int32_t flint_attn_write_kv(flint_attn *a, int32_t layer, int32_t seq, int32_t s
 /* Device addresses of a layer's K (which = 0) or V (1) cache, for zero-copy fills by a co-resident producer (the
  * page pool [kv_pages][4][64][128] of a paged layer). */
 void *flint_attn_kv_dev(flint_attn *a, int32_t layer, int32_t which);
+/* Rows of K and V in and out of a layer's cache on the device, for a co-resident producer or consumer: n sequences, n_rows
+ * consecutive positions each, from pos0[i] (host array) on.  k_dev / v_dev: [n][4][n_rows][128] of `dtype` (F32, BF16 or
+ * F16), starting on a 16-byte boundary, K already normalised and rotated.  store rounds the values to half and writes them
+ * in the cache's format (quantised on a 4-bit handle); on a ring layer a position goes to its slot, and below
+ * first_tokens to the first tokens' rows too; of positions that share a slot the last one is kept.  A paged layer takes
+ * the pages it needs, or fails with "KV page pool exhausted" and changes nothing.  No sequence twice in one store.
+ * load reads back the values that the cache stands for (4-bit: rounded once to `dtype`); positions on pages a sequence
+ * does not hold read as zeros, positions that a ring has given to others read as those.  The sequences' positions are
+ * neither read nor moved (flint_attn_set_pos).  Asynchronous on `cuda_stream`; not for layers sharded by key range. */
+int32_t flint_attn_store_kv_dev(flint_attn *a, int32_t layer, int32_t n, const int32_t *seqs, const int32_t *pos0,
+                                int32_t n_rows, const void *k_dev, const void *v_dev, int32_t dtype, void *cuda_stream,
+                                char *err, int32_t err_len);
+int32_t flint_attn_load_kv_dev(flint_attn *a, int32_t layer, int32_t n, const int32_t *seqs, const int32_t *pos0,
+                               int32_t n_rows, void *k_dev, void *v_dev, int32_t dtype, void *cuda_stream, char *err,
+                               int32_t err_len);
 /* Declare that a sequence's caches already hold `pos` tokens (after flint_attn_write_kv / a device-side fill). */
 int32_t flint_attn_set_pos(flint_attn *a, int32_t seq, int32_t pos);
 
