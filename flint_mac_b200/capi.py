@@ -32,10 +32,12 @@ class _KvOptions(C.Structure):
     _fields_ = [("kv_format", C.c_int32), ("first_tokens", C.c_int32)]
 
 
+_I32P = C.POINTER(C.c_int32)
 _KV_ROWS = [C.c_void_p, C.c_int32, C.c_int32, C.POINTER(C.c_int32), C.POINTER(C.c_int32), C.c_int32, C.c_void_p, C.c_void_p,
             C.c_int32, C.c_void_p, C.c_char_p, C.c_int32]
 SYMBOLS = {
     "flint_attn_open_kv": (C.c_void_p, [C.POINTER(_Config), C.POINTER(_KvOptions), C.c_char_p, C.c_int32]),
+    "flint_attn_plan_decode_int4": (C.c_int32, [C.c_int32, _I32P, C.c_int32, C.c_int32, C.c_int32, _I32P, C.c_int32]),
     "flint_attn_store_kv_dev": (C.c_int32, _KV_ROWS),
     "flint_attn_load_kv_dev": (C.c_int32, _KV_ROWS),
     "flint_attn_open": (C.c_void_p, [C.POINTER(_Config), C.c_char_p, C.c_int32]),
@@ -154,6 +156,18 @@ def plan_decode(pos: Sequence[int], is_swa: bool, kv_lo: int = 0, kv_hi: int = 2
         if n >= 0:
             return np.ctypeslib.as_array(out)[: 8 * n].reshape(n, 8).copy()
         cap *= 4
+
+
+def plan_decode_int4(pos: Sequence[int], is_swa: bool, first_tokens: int = 0, target_items: int = 296):
+    """Host-only: the pieces of a decode launch over a 4-bit cache as an int32 array [n][8] =
+    (token, tile0, tile1, split, n_split, first_record, launch, records_of_launch)."""
+    lib = load_library()
+    cap = 4096 + 4 * len(pos)
+    out = (C.c_int32 * (8 * cap))()
+    n = lib.flint_attn_plan_decode_int4(len(pos), _i32(pos), int(is_swa), first_tokens, target_items, out, cap)
+    if n < 0:
+        raise FlintAttnError("bad batch for a plan")
+    return np.ctypeslib.as_array(out)[: 8 * n].reshape(n, 8).copy()
 
 
 def rollback_restart(cached_len: int, pos: int) -> int:

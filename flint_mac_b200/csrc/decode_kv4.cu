@@ -8,15 +8,18 @@
 // sliding-window layer, and the token itself.  The token itself enters at half precision, as its own record of the final
 // merge; its row is quantised into the cache by the same launch.
 //
-// The codes go to the tensor cores as they are: a nibble masked out of a 16-bit lane is the half-precision number
-// c * 2^-24 (or c * 2^-20 for the second nibble: the lane holds c * 16 subnormal steps), which the products take exactly.
-// Q is stored for the first and second nibbles with factors 4 and 1/4, so that both come out as q c 2^-22; outputs of
-// the second nibbles are 16 times too large and are put right at the end.  That is 5 logical operations for 8 codes.
-// On the K side d multiplies the 32-dim partial scores (4 groups per key), on the V side it multiplies the
-// probabilities (4 operand pairs per 16 keys), and lo enters through one more product each.
+// The codes go to the tensor cores as they are: bits masked out of the low byte of a 16-bit lane are a half-precision
+// number, their value times 2^-24, which the products take exactly.  Of the four codes n0 .. n3 of a lane the operands are
+// n0, n0 + 16 n1, n2 and n2 + 16 n3: four logical operations for the eight codes of a register.  On the K side
+//   q0 n0 + q1 n1 = (q0 - q1 / 16) n0 + (q1 / 16) (n0 + 16 n1),
+// so Q is stored with those factors (times four, away from half's subnormals); on the V side the output of n1 is a sixteenth
+// of the difference of two outputs.  On the K side d multiplies the 32-dim partial scores (4 groups per key), on the V side
+// it multiplies the probabilities (4 operand pairs per 16 keys), and lo enters through one more product each.
 //
-// A warp works on whole blocks of 64 positions by itself, the four warps of a CTA on every fourth one; a block is one
-// 10 KB bulk copy on the warp's own mbarrier.
+// A CTA works on pieces (kv4_plan.h), one after the other: its own, then those of CTAs that have not started.  Its eight
+// warps take every eighth tile of a piece each and work alone: a tile is one 5 KB bulk copy for K and one for V, on
+// mbarriers of the warp's own; the next tile's K comes in while this one's V is worked on, and the other way round, and
+// the raw rows and the first K of the next piece while this one is worked on and ended.
 #include <cstring>
 
 #include "decode_common.cuh"
@@ -26,24 +29,33 @@ namespace flint {
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 2;       // blocks of a warp in flight or in use
+constexpr int kHalf = kKv4VCodes;    // a block's K part, and its V part: 5120 bytes each
+static_assert(kKv4BlockBytes == 2 * kHalf, "K and V part of a block are alike");
 constexpr int kORow = kHeadDim + 4;  // floats between heads of the merge buffer: the eight lanes of a store hit different banks
-constexpr uint32_t kNib0 = 0x000f000fu, kNib1 = 0x00f000f0u;
 
+template <int kWarps>
 struct __align__(128) Dec4Smem {
-    unsigned char tile[kWarps][kStages][kKv4BlockBytes];
-    alignas(8) unsigned long long full_bar[kWarps][kStages];
+    unsigned char k[kWarps][kHalf];
+    union {
+        unsigned char v[kWarps][kHalf];
+        float o[kWarps][kGqa][kORow];  // the warps' outputs of a piece, once all are through with its tiles
+    };
+    alignas(8) unsigned long long full_bar[kWarps][2];  // the K part, the V part has landed
+    alignas(16) uint4 next;                // answer of the scheduler: the next piece, if there is one
+    alignas(8) unsigned long long next_bar;
+    alignas(16) unsigned char raw[kGqa + 2][kHeadDim * 4];  // raw rows of the next piece: q heads, new k, new v
     alignas(16) __half q[kGqa][kHeadDim];  // normalised, rotated, scaled by log2(e) / sqrt(128)
-    float red_m[kWarps][kGqa], red_l[kWarps][kGqa], s_new[kGqa];
+    float red_m[kWarps][kGqa], red_l[kWarps][kGqa];
     alignas(16) __half knew[kHeadDim];
-    alignas(16) __half vnew[kHeadDim];
+    alignas(16) __half vnew[2][kHeadDim];  // (the present piece's is read while the next one's is written)
     alignas(16) float rope_cos[kHeadDim / 2], rope_sin[kHeadDim / 2];
-    int is_last;
+    alignas(16) float q_norm[kHeadDim], k_norm[kHeadDim], sinks[kNHead];
+    struct {  // a piece whose record is written: where it belongs, and whether it was the last of its run to arrive
+        int rec0, split, n_split, kvh, row, last;
+    } done[2];
+    int last2;
 };
-// The per-warp outputs are merged through the (by then idle) tiles.
-static_assert(sizeof(float) * kWarps * kGqa * kORow <= sizeof(Dec4Smem::tile), "merge buffer aliases the tiles");
+static_assert(sizeof(Dec4Smem<4>) * 4 <= 223 * 1024 && sizeof(Dec4Smem<8>) * 2 <= 225 * 1024, "CTAs of an SM");
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst),
@@ -62,99 +74,325 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
+// The operands n0, n0 + 16 n1, n2, n2 + 16 n3 of a register of eight codes.
+struct Codes {
+    uint32_t n0, n01, n2, n23;
+};
+__device__ __forceinline__ Codes split_codes(uint32_t w) {
+    Codes c;
+    c.n0 = w & 0x000f000fu;
+    c.n01 = w & 0x00ff00ffu;
+    c.n23 = __byte_perm(w, 0u, 0x4341);
+    c.n2 = c.n23 & 0x000f000fu;
+    return c;
+}
+// D(16x8, f32) = A(16x16, f16, row) * B(16x8, f16, col)
+__device__ __forceinline__ void mma_16816_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Packed two-float arithmetic
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void fma2(float &a, float &b, uint64_t m, float c0, float c1) {  // (a, b) = (a, b) * m + (c0, c1)
+    asm("{\n.reg .b64 x, y;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%3, %4};\nfma.rn.f32x2 x, x, %2, y;\nmov.b64 {%0, %1}, x;\n}\n"
+        : "+f"(a), "+f"(b)
+        : "l"(m), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ void sub2(float &a, float &b, uint64_t m) {  // (a, b) -= m
+    asm("{\n.reg .b64 x;\nmov.b64 x, {%0, %1};\nsub.rn.f32x2 x, x, %2;\nmov.b64 {%0, %1}, x;\n}\n" : "+f"(a), "+f"(b) : "l"(m));
+}
+__device__ __forceinline__ void add2(uint64_t &acc, float a, float b) {
+    asm("{\n.reg .b64 x;\nmov.b64 x, {%1, %2};\nadd.rn.f32x2 %0, %0, x;\n}\n" : "+l"(acc) : "f"(a), "f"(b));
+}
+
 __device__ __forceinline__ float low_half(uint32_t a) { return __low2float(*reinterpret_cast<const __half2 *>(&a)); }
 
-__device__ __forceinline__ void decode_item(const Dec4Params &p, const DecItem &it) {
+// Bounded by a count of polls (a quarter of a second or more), not by the clock: the loop is four instructions.
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+    for (uint32_t n = 0; n < (1u << 24); n++)
+        if (mbar_try_wait(bar, parity)) return true;
+    return false;
+}
+
+// Folds n partial records of one head into (M, L, a): the lane's four dims d0 .. d0 + 3.  Record i lies at rec(i).
+// Ten records a trip, their loads in flight together.
+struct Merged4 {
+    float M, L, a[4];
+};
+template <typename Rec>
+__device__ __forceinline__ Merged4 merge_records4(Rec rec, int n, int d0) {
+    constexpr int kTrip = 10;
+    Merged4 r;
+    r.M = -INFINITY;
+    r.L = r.a[0] = r.a[1] = r.a[2] = r.a[3] = 0.f;
+#pragma unroll 1
+    for (int s0 = 0; s0 < n; s0 += kTrip) {
+        float2 ml[kTrip];
+        float4 x[kTrip];
+#pragma unroll
+        for (int i = 0; i < kTrip; i++) {
+            const float *q = rec(min(s0 + i, n - 1));  // past the end: the last one again, unused
+            ml[i] = __ldcg(reinterpret_cast<const float2 *>(q + kHeadDim));
+            x[i] = __ldcg(reinterpret_cast<const float4 *>(q + d0));
+            if (s0 + i >= n) ml[i] = make_float2(-INFINITY, 0.f);
+        }
+        float cm = r.M;
+#pragma unroll
+        for (int i = 0; i < kTrip; i++) cm = fmaxf(cm, ml[i].x);
+        const float keep = r.M == -INFINITY ? 0.f : fast_exp2(r.M - cm);
+        r.L *= keep;
+#pragma unroll
+        for (int j = 0; j < 4; j++) r.a[j] *= keep;
+        r.M = cm;
+#pragma unroll
+        for (int i = 0; i < kTrip; i++) {
+            const float c = ml[i].y == 0.f ? 0.f : fast_exp2(ml[i].x - cm);
+            r.L += ml[i].y * c;
+            r.a[0] += x[i].x * c; r.a[1] += x[i].y * c; r.a[2] += x[i].z * c; r.a[3] += x[i].w * c;
+        }
+    }
+    return r;
+}
+
+__device__ __forceinline__ void store_out4(void *out, int dtype, size_t idx, float a, float b, float c, float d) {
+    if (dtype == kDtypeF32) {
+        *reinterpret_cast<float4 *>(static_cast<float *>(out) + idx) = make_float4(a, b, c, d);
+    } else {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
+        *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(out) + idx) =
+            make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
+    }
+}
+
+// Asks the scheduler for a CTA of this grid that has not started: it then never starts, and its work is the asker's.
+__device__ __forceinline__ void ask_next(uint32_t dst, uint32_t bar) {
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    mbar_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n" ::"r"(dst), "r"(bar)
+                 : "memory");
+}
+// The answer: the block index of the CTA, or -1 if none was left.
+__device__ __forceinline__ int next_index(uint32_t src) {
+    uint32_t ok, x;
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .b128 r;\n.reg .b64 a, b;\n"
+        "ld.shared.v2.b64 {a, b}, [%2];\n"
+        "mov.b128 r, {a, b};\n"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n"
+        "selp.b32 %0, 1, 0, p;\n"
+        "mov.b32 %1, 0;\n"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n}\n"
+        : "=r"(ok), "=r"(x)
+        : "r"(src)
+        : "memory");
+    return ok ? int(x) : -1;
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(dst), "l"(src) : "memory");
+}
+
+template <int kWarps>
+__device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Piece *pieces) {
     extern __shared__ __align__(128) unsigned char smem_raw[];
-    Dec4Smem &sm = *reinterpret_cast<Dec4Smem *>(smem_raw);
+    Dec4Smem<kWarps> &sm = *reinterpret_cast<Dec4Smem<kWarps> *>(smem_raw);
+    constexpr int kThreads = kWarps * 32, kHeads = kGqa / kWarps;  // kHeads: query heads of the group that a warp looks after
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int g = lane >> 2, t4 = lane & 3, d0 = 4 * lane;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-    const int mh = tid >> 4, md = (tid & 15) * 8;
-    const int head = it.kvh * kGqa + mh;
-    const float sink = p.sinks[head];
     const bool rope = p.has_rope != 0;
-    const bool fold_k = it.fold && warp == 0, fold_v = it.fold && warp == 1;
-    const float4 wq = reinterpret_cast<const float4 *>(p.q_norm)[lane];
-    float4 wk = wq;
-    if (fold_k) wk = reinterpret_cast<const float4 *>(p.k_norm)[lane];
     float freq = 0.f;
     if (rope && tid < kHeadDim / 2) freq = p.inv_freq[tid];
-    // the cached keys, 64 positions at a time: the block of first tokens if some lie before the window, then the range
-    const int n_first = p.is_swa ? min(p.cache.first_tokens, it.j0) : 0;
-    const int extra = n_first > 0 ? 1 : 0, b0 = it.j0 >> 6;
-    const int n_tiles = extra + (it.j1 > it.j0 ? ((it.j1 + 63) >> 6) - b0 : 0);
-    const uint32_t tiles = smem_u32(&sm.tile[warp][0][0]), bars = smem_u32(&sm.full_bar[warp][0]);
-    auto load_tile = [&](int t, int stage) {  // one lane
-        const unsigned char *block = t < extra ? kv4_first_block(p.cache, it.seq, it.kvh)
-                                               : kv4_block(p.cache, it.seq, it.kvh, b0 + t - extra);
-        mbar_expect_tx(bars + 8 * stage, kKv4BlockBytes);
-        bulk_load(tiles + stage * kKv4BlockBytes, block, kKv4BlockBytes, bars + 8 * stage);
-    };
+    // the layer's constants: read from shared memory at every piece (a load past a busy memory system takes microseconds)
+    for (int i = tid; i < kHeadDim; i += kThreads) {
+        sm.q_norm[i] = p.q_norm[i];
+        sm.k_norm[i] = p.k_norm[i];
+        if (i < kNHead) sm.sinks[i] = p.sinks[i];
+    }
+    const uint32_t k_tile = smem_u32(&sm.k[warp][0]), v_tile = smem_u32(&sm.v[warp][0]);
+    const uint32_t k_bar = smem_u32(&sm.full_bar[warp][0]), v_bar = k_bar + 8;
     if (lane == 0) {
-#pragma unroll
-        for (int i = 0; i < kStages; i++) mbar_init(bars + 8 * i, 1);
+        mbar_init(k_bar, 1);
+        mbar_init(v_bar, 1);
+        if (warp == 0) mbar_init(smem_u32(&sm.next_bar), 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
+
+    // ldmatrix addresses of a lane in the K and V codes of 16 rows (the chunk swizzle depends on the row mod 8 alone)
+    const int sw = (lane & 7) >> 1;
+    const uint32_t k_at = k_tile + (lane & 7) * kKv4RowBytes + (((lane >> 3) ^ sw) << 4);
+    const uint32_t v_at = v_tile + (((lane >> 3) & 1) * 8 + (lane & 7)) * kKv4RowBytes + (((lane >> 4) ^ sw) << 4);
+    const uint32_t kg_at = k_tile + kKv4KGroups + g * 16, vg_at = v_tile + (kKv4VGroups - kHalf) + t4 * 32;
+
+    // the present piece
+    Dec4Piece pc;
+    Dec4Range rg;
+    int kvh, ta, tb;
+    const unsigned char *seq_blocks;  // contiguous caches: the group's first block
+    bool ends;  // it ends its group: it also takes the new token
+    auto get_piece = [&](int index) {
+        pc = pieces[index >> 2];
+        kvh = index & 3;
+        rg = dec4_range(pc.pos, p.is_swa, p.cache.first_tokens);
+        ta = pc.t0;
+        tb = ta + pc.n;
+        ends = pc.split == pc.n_split - 1;
+        seq_blocks = p.cache.blocks + (size_t(pc.seq) * kNHeadKv + kvh) * p.cache.blocks_per_seq * kKv4BlockBytes;
+    };
+    auto load_part = [&](int t, int is_v) {  // one lane
+        const int extra = rg.n_first > 0 ? 1 : 0, b = (rg.j0 >> 6) + t - extra;
+        const unsigned char *block;
+        if (p.cache.block_table) block = kv4_block(p.cache, pc.seq, kvh, b);
+        else block = seq_blocks + size_t(t < extra ? uint32_t(kKv4RingBlocks) : uint32_t(b) & p.cache.block_mask) * kKv4BlockBytes;
+        const uint32_t bar = is_v ? v_bar : k_bar;
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // earlier accesses to the buffer come first
+        mbar_expect_tx(bar, kHalf);
+        bulk_load(is_v ? v_tile : k_tile, block + is_v * kHalf, kHalf, bar);
+    };
+    // Raw rows: its heads of the group by each warp, the new k and v by warps 0 and 1 too.  A warp reads what it fetched.
+    auto fetch_rows = [&](int index) {
+        const Dec4Piece &w = pieces[index >> 2];
+        const int head0 = (index & 3) * kGqa, tok = p.tok0 + w.tok;
+        const size_t es = p.qkv_dtype == kDtypeF32 ? 4 : 2;
+        const unsigned char *row = static_cast<const unsigned char *>(p.qkv) + size_t(tok) * kQkvDim * es;
+        auto fetch = [&](int at, int i) {
+            const uint32_t dst = smem_u32(&sm.raw[i][0]) + d0 * uint32_t(es);
+            if (es == 4) cp_async16(dst, row + (at + d0) * es, 16);
+            else cp_async8(dst, row + (at + d0) * es);
+        };
+#pragma unroll
+        for (int i = 0; i < kHeads; i++) fetch((head0 + warp * kHeads + i) * kHeadDim, warp * kHeads + i);
+        if (w.split == w.n_split - 1 && warp < 2) fetch(kQDim + warp * kKvDim + (index & 3) * kHeadDim, kGqa + warp);
+        cp_async_commit();
+    };
+    auto rope_table = [&](int index) {
+        if (!rope || tid >= kHeadDim / 2) return;
+        float sn, cs;
+        sincos_reduced(float(pieces[index >> 2].pos) * freq, &sn, &cs);
+        sm.rope_cos[tid] = cs;
+        sm.rope_sin[tid] = sn;
+    };
+    int flip = 0;
+    auto finish_rows = [&] {  // raw rows (and the rotation table, visible already) -> sm.q, the new token's rows, the cache
+        cp_async_wait<0>();
+        __syncwarp();
+        float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (rope) {
+            cs = reinterpret_cast<const float4 *>(sm.rope_cos)[lane & 15];
+            sn = reinterpret_cast<const float4 *>(sm.rope_sin)[lane & 15];
+        }
+        const float qscale = rsqrtf(float(kHeadDim)) * kLog2e;  // softmax runs in base 2
+#pragma unroll
+        for (int i = 0; i < kHeads; i++) {
+            const int h = warp * kHeads + i;
+            float4 x = norm_rope(load_row4(&sm.raw[h][0], p.qkv_dtype, 0, lane), reinterpret_cast<const float4 *>(sm.q_norm)[lane], cs, sn, lane, rope);
+            x.x *= qscale; x.y *= qscale; x.z *= qscale; x.w *= qscale;
+            store_half4(&sm.q[h][d0], x);
+        }
+        if (ends && warp < 2) {
+            float4 x = load_row4(&sm.raw[kGqa + warp][0], p.qkv_dtype, 0, lane);
+            if (warp == 0) x = norm_rope(x, reinterpret_cast<const float4 *>(sm.k_norm)[lane], cs, sn, lane, rope);
+            const uint2 h = make_uint2(pack_half2(x.x, x.y), pack_half2(x.z, x.w));
+            *reinterpret_cast<uint2 *>(warp == 0 ? &sm.knew[d0] : &sm.vnew[flip][d0]) = h;
+        }
+    };
+    auto store_new = [&] {  // the new token's rows -> the cache (warps 0 and 1)
+        if (!ends || warp >= 2) return;
+        const uint2 h = *reinterpret_cast<const uint2 *>(warp == 0 ? &sm.knew[d0] : &sm.vnew[flip][d0]);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&h.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
+        const float f[4] = {a.x, a.y, b.x, b.y};
+        kv4_store_lane(kv4_block(p.cache, pc.seq, kvh, pc.pos >> 6), pc.pos & 63, warp == 1, lane, f);
+        if (p.is_swa && pc.pos < p.cache.first_tokens)
+            kv4_store_lane(kv4_first_block(p.cache, pc.seq, kvh), pc.pos, warp == 1, lane, f);
+    };
+    // Split-K: merges the run of records that piece `w` was the last of to arrive, and if that was the group's last run, the
+    // runs (the whole CTA calls this).
+    auto merge_run = [&](int w) {
+        const auto &f = sm.done[w];
+        const int rec0 = f.rec0, fan = dec4_fan(f.n_split), sub = f.split / fan, n_sub = (f.n_split + fan - 1) / fan;
+        auto record = [&](float *base, int i, int h) { return base + (size_t(rec0 + i * kNHeadKv) * kGqa + h) * kRecStride; };
+        const int h0 = warp * kHeads, n = min(fan, f.n_split - sub * fan);
+        auto finish = [&](const Merged4 &r, int h) {
+            const int head = f.kvh * kGqa + h;
+            const float sink2 = sm.sinks[head] * kLog2e;
+            const float Mf = fmaxf(r.M, sink2), cf = fast_exp2(r.M - Mf);
+            const float inv = cf / (r.L * cf + fast_exp2(sink2 - Mf));
+            store_out4(p.out, p.out_dtype, size_t(f.row) * kQDim + head * kHeadDim + d0, r.a[0] * inv, r.a[1] * inv, r.a[2] * inv, r.a[3] * inv);
+        };
+#pragma unroll 1
+        for (int h = h0; h < h0 + kHeads; h++) {
+            const Merged4 r = merge_records4([&](int i) { return record(p.scratch, sub * fan + i, h); }, n, d0);
+            if (n_sub == 1) {
+                finish(r, h);
+                continue;
+            }
+            float *rec = record(p.scratch2, sub, h);
+            *reinterpret_cast<float4 *>(rec + d0) = make_float4(r.a[0], r.a[1], r.a[2], r.a[3]);
+            if (lane == 0) *reinterpret_cast<float2 *>(rec + kHeadDim) = make_float2(r.M, r.L);
+        }
+        if (n_sub == 1) return;
+        __syncthreads();
+        if (tid == 0) {
+            const bool last = ticket_acq_rel(&p.tickets2[rec0]) == n_sub - 1;
+            if (last) p.tickets2[rec0] = 0;
+            sm.last2 = last;
+        }
+        __syncthreads();
+        if (!sm.last2) return;
+#pragma unroll 1
+        for (int h = h0; h < h0 + kHeads; h++)
+            finish(merge_records4([&](int i) { return record(p.scratch2, i, h); }, n_sub, d0), h);
+    };
+
+    get_piece(int(blockIdx.x));
     // Nothing an earlier kernel of the stream produces (rows, cache contents, split-K records and counters) is read or
     // written before this wait.
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    if (lane == 0) {
-#pragma unroll
-        for (int i = 0; i < kStages; i++)
-            if (warp + i * kWarps < n_tiles) load_tile(warp + i * kWarps, i);
-    }
+    fetch_rows(int(blockIdx.x));
+    if (lane == 0 && ta + warp < tb) load_part(ta + warp, 0);
+    if (tid == 0) ask_next(smem_u32(&sm.next), smem_u32(&sm.next_bar));
+    rope_table(int(blockIdx.x));
+    __syncthreads();
+    finish_rows();
+    __syncthreads();
 
-    // ---- prologue: the group's q heads, and the new token's k and v
-    const size_t row0 = size_t(it.tok) * kQkvDim;
-    float4 q[2];
+    const uint64_t two22 = pack2(4194304.f, 4194304.f);
+    bool waiting = false;  // the last piece's record is out, its run not yet merged
+    int used = 0;  // tiles this warp has been through: the phase of its barriers
+    for (uint32_t turn = 0;; turn++) {
+    if (lane == 0 && ta + warp < tb) load_part(ta + warp, 1);
+    store_new();
+    float s_new[kHeads];  // the new token's score with the warp's heads
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-        q[i] = load_row4(p.qkv, p.qkv_dtype, row0 + size_t(it.kvh * kGqa + warp * 2 + i) * kHeadDim, lane);
-    float4 kv_new = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (fold_k) kv_new = load_row4(p.qkv, p.qkv_dtype, row0 + kQDim + size_t(it.kvh) * kHeadDim, lane);
-    if (fold_v) kv_new = load_row4(p.qkv, p.qkv_dtype, row0 + kQDim + kKvDim + size_t(it.kvh) * kHeadDim, lane);
-    const float qscale = rsqrtf(float(kHeadDim)) * kLog2e;  // softmax runs in base 2
-    if (rope && tid < kHeadDim / 2) {
-        float sn, cs;
-        sincos_reduced(float(it.pos) * freq, &sn, &cs);
-        sm.rope_cos[tid] = cs;
-        sm.rope_sin[tid] = sn;
-    }
-    __syncthreads();
-    float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (rope) {
-        cs = reinterpret_cast<const float4 *>(sm.rope_cos)[lane & 15];
-        sn = reinterpret_cast<const float4 *>(sm.rope_sin)[lane & 15];
-    }
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        q[i] = norm_rope(q[i], wq, cs, sn, lane, rope);
-        q[i].x *= qscale; q[i].y *= qscale; q[i].z *= qscale; q[i].w *= qscale;
-        store_half4(&sm.q[warp * 2 + i][4 * lane], q[i]);
-    }
-    if (fold_k || fold_v) {
-        if (fold_k) kv_new = norm_rope(kv_new, wk, cs, sn, lane, rope);
-        const uint2 h = make_uint2(pack_half2(kv_new.x, kv_new.y), pack_half2(kv_new.z, kv_new.w));
-        *reinterpret_cast<uint2 *>(fold_k ? &sm.knew[4 * lane] : &sm.vnew[4 * lane]) = h;
-        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&h.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
-        const float x[4] = {a.x, a.y, b.x, b.y};
-        kv4_store_lane(kv4_block(p.cache, it.seq, it.kvh, it.pos >> 6), it.pos & 63, fold_v, lane, x);
-        if (p.is_swa && it.pos < p.cache.first_tokens)
-            kv4_store_lane(kv4_first_block(p.cache, it.seq, it.kvh), it.pos, fold_v, lane, x);
-    }
-    __syncthreads();
-    if (it.fold) {
-        const uint2 h = *reinterpret_cast<const uint2 *>(&sm.knew[4 * lane]);
+    for (int i = 0; i < kHeads; i++) s_new[i] = -INFINITY;
+    if (ends) {
+        const uint2 h = *reinterpret_cast<const uint2 *>(&sm.knew[d0]);
         const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&h.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const float s = warp_sum(q[i].x * a.x + q[i].y * a.y + q[i].z * b.x + q[i].w * b.y);
-            if (lane == 0) sm.s_new[warp * 2 + i] = s;
+        for (int i = 0; i < kHeads; i++) {
+            const uint2 w = *reinterpret_cast<const uint2 *>(&sm.q[warp * kHeads + i][d0]);
+            const float2 c = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)), d = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
+            s_new[i] = warp_sum(c.x * a.x + c.y * a.y + d.x * b.x + d.y * b.y);
         }
     }
 
     // ---- operands of Q: group c's 32 dims are the words t4 of its four 16-byte chunks, dims 32 c + 8 t4 + nibble
-    const int g = lane >> 2, t4 = lane & 3;
     uint32_t bq[kKv4Groups][4], qs_hi, qs_lo;
     {
         const __half2 up = __float2half2_rn(4.f), down = __float2half2_rn(0.25f);
@@ -162,16 +400,17 @@ __device__ __forceinline__ void decode_item(const Dec4Params &p, const DecItem &
 #pragma unroll
         for (int c = 0; c < kKv4Groups; c++) {
             const uint4 w = *reinterpret_cast<const uint4 *>(&sm.q[g][32 * c + 8 * t4]);
-            const uint32_t pair[4] = {__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632),   // nibbles 0 4, 1 5
-                                      __byte_perm(w.y, w.w, 0x5410), __byte_perm(w.y, w.w, 0x7632)};  // nibbles 2 6, 3 7
             float sum = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const __half2 v = *reinterpret_cast<const __half2 *>(&pair[j]);
-                const __half2 r = __hmul2(v, (j & 1) ? down : up);
-                bq[c][j] = *reinterpret_cast<const uint32_t *>(&r);
-                const float2 f = __half22float2(v);
-                sum += f.x + f.y;
+            for (int j = 0; j < 2; j++) {
+                const uint32_t lo = j == 0 ? w.x : w.y, hi = j == 0 ? w.z : w.w;  // nibbles 2 j, 2 j + 1 and those four further on
+                const uint32_t e = __byte_perm(lo, hi, 0x5410), f = __byte_perm(lo, hi, 0x7632);
+                const __half2 r1 = __hmul2(*reinterpret_cast<const __half2 *>(&f), down);                 // of n1: 4 q1 / 16
+                const __half2 c0 = __hfma2(*reinterpret_cast<const __half2 *>(&e), up, __hneg2(r1));  // of n0: 4 (q0 - q1 / 16)
+                bq[c][2 * j] = *reinterpret_cast<const uint32_t *>(&c0);
+                bq[c][2 * j + 1] = *reinterpret_cast<const uint32_t *>(&r1);
+                const float2 fc = __half22float2(c0), fr = __half22float2(r1);
+                sum += 0.25f * (fc.x + fc.y) + 4.25f * (fr.x + fr.y);  // q0 + q1 as the operands have them
             }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -186,25 +425,30 @@ __device__ __forceinline__ void decode_item(const Dec4Params &p, const DecItem &
     }
 
     // Per lane: reference maximum (replicated over g) and partial sum of heads 2 t4 and 2 t4 + 1; outputs o[2c] = dims
-    // 32 c + 4 g and + 1, o[2c + 1] = dims + 2 and + 3, each for the two heads; om = the part of lo, group g & 3.
+    // 32 c + 4 g (n0) and + 1 (n0 + 16 n1), o[2c + 1] = dims + 2 and + 3, each for the two heads; om = the part of lo, group
+    // g & 3.
     // The reference lies 2 under the maximum (base 2), so that probabilities times d keep two more bits above half's
     // subnormal steps; d is at most 8736, so four times that still fits a half.
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY;
+    uint64_t l01 = 0;  // (two zeros)
     float o[2 * kKv4Groups][4], om[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 2 * kKv4Groups; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    bool late = false;
-    int waited = 0;
-    for (int t = warp, k = 0; t < n_tiles; t += kWarps, k++) {
-        const int stage = k % kStages;
-        waited = k + 1;
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * stage, uint32_t(k / kStages) & 1u))) {
+    // what comes next (asked for a piece ago): its rows are fetched while this piece is worked on
+    bool late = !__all_sync(0xffffffffu, wait_bar(smem_u32(&sm.next_bar), turn & 1u));
+    const int next = late ? -1 : next_index(smem_u32(&sm.next));
+    if (next >= 0) {
+        fetch_rows(next);
+        rope_table(next);
+    }
+    const int extra = rg.n_first > 0 ? 1 : 0;
+    for (int t = ta + warp; t < tb; t += kWarps) {
+        if (!__all_sync(0xffffffffu, wait_bar(k_bar, uint32_t(used) & 1u))) {
             late = true;
             break;
         }
-        const uint32_t tile = tiles + stage * kKv4BlockBytes;
-        const int r0 = 64 * (b0 + t - extra);
-        const int r_lo = t < extra ? 0 : max(it.j0 - r0, 0), r_hi = t < extra ? n_first : min(it.j1 - r0, 64);
+        const int r0 = 64 * ((rg.j0 >> 6) + t - extra);
+        const int r_lo = t < extra ? 0 : max(rg.j0 - r0, 0), r_hi = t < extra ? rg.n_first : min(pc.pos - r0, 64);
         const bool edge = r_lo > 0 || r_hi < 64;
 
         // S^T (64 keys x 8 heads)
@@ -212,51 +456,46 @@ __device__ __forceinline__ void decode_item(const Dec4Params &p, const DecItem &
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             uint32_t ra[4], rb[4], ga[4], gb[4];
-            const int row = 16 * i + (lane & 7), ch = (lane >> 3) ^ ((row >> 1) & 3);
-            ldmatrix_x4(ra, tile + kKv4KCodes + row * kKv4RowBytes + ch * 16);
-            ldmatrix_x4(rb, tile + kKv4KCodes + (row + 8) * kKv4RowBytes + ch * 16);  // ((row + 8) >> 1 & 3 is the same)
-            lds128(ga, tile + kKv4KGroups + (16 * i + g) * 16);
-            lds128(gb, tile + kKv4KGroups + (16 * i + g + 8) * 16);
-            const uint32_t oa = lds32(tile + kKv4KGroups + (16 * i + g) * 16 + 4 * t4);
-            const uint32_t ob = lds32(tile + kKv4KGroups + (16 * i + g + 8) * 16 + 4 * t4);
-            float lo[4] = {0.f, 0.f, 0.f, 0.f};
+            ldmatrix_x4(ra, k_at + i * 16 * kKv4RowBytes);
+            ldmatrix_x4(rb, k_at + (i * 16 + 8) * kKv4RowBytes);
+            lds128(ga, kg_at + i * 256);
+            lds128(gb, kg_at + i * 256 + 128);
+            float lo[4];
             {
+                const uint32_t oa = lds32(kg_at + i * 256 + 4 * t4), ob = lds32(kg_at + i * 256 + 128 + 4 * t4);
                 const uint32_t a[4] = {oa, ob, oa, ob};
-                mma_16816(lo, a, qs_hi, qs_lo);
+                mma_16816_new(lo, a, qs_hi, qs_lo);
             }
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < kKv4Groups; c++) {
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                uint32_t x = ra[c], y = rb[c];
-                const uint32_t a0[4] = {x & kNib0, y & kNib0, x & kNib1, y & kNib1};
-                mma_16816(acc, a0, bq[c][0], bq[c][1]);
-                x >>= 8;
-                y >>= 8;
-                const uint32_t a1[4] = {x & kNib0, y & kNib0, x & kNib1, y & kNib1};
+                float acc[4];
+                const Codes x = split_codes(ra[c]), y = split_codes(rb[c]);
+                const uint32_t a0[4] = {x.n0, y.n0, x.n01, y.n01}, a1[4] = {x.n2, y.n2, x.n23, y.n23};
+                mma_16816_new(acc, a0, bq[c][0], bq[c][1]);
                 mma_16816(acc, a1, bq[c][2], bq[c][3]);
                 const float da = low_half(ga[c]), db = low_half(gb[c]);
-                sum[0] = fmaf(da, acc[0], sum[0]);
-                sum[1] = fmaf(da, acc[1], sum[1]);
-                sum[2] = fmaf(db, acc[2], sum[2]);
-                sum[3] = fmaf(db, acc[3], sum[3]);
+                s[i][0] = c == 0 ? da * acc[0] : fmaf(da, acc[0], s[i][0]);
+                s[i][1] = c == 0 ? da * acc[1] : fmaf(da, acc[1], s[i][1]);
+                s[i][2] = c == 0 ? db * acc[2] : fmaf(db, acc[2], s[i][2]);
+                s[i][3] = c == 0 ? db * acc[3] : fmaf(db, acc[3], s[i][3]);
             }
+            fma2(s[i][0], s[i][1], two22, lo[0], lo[1]);
+            fma2(s[i][2], s[i][3], two22, lo[2], lo[3]);
+        }
+        if (edge) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) s[i][j] = fmaf(sum[j], 4194304.f, lo[j]);
-            if (edge) {
+            for (int i = 0; i < 4; i++) {
                 const int ka = 16 * i + g, kb = ka + 8;
                 if (ka < r_lo || ka >= r_hi) s[i][0] = s[i][1] = -INFINITY;
                 if (kb < r_lo || kb >= r_hi) s[i][2] = s[i][3] = -INFINITY;
             }
         }
+        __syncwarp();  // the whole warp is done with the K part
+        if (lane == 0 && t + kWarps < tb) load_part(t + kWarps, 0);
 
         // running maximum (each block has a key that the query sees, so it gets finite), probabilities
-        float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            mx0 = fmaxf(mx0, fmaxf(s[i][0], s[i][2]));
-            mx1 = fmaxf(mx1, fmaxf(s[i][1], s[i][3]));
-        }
+        float mx0 = max3(fmaxf(s[0][0], s[0][2]), max3(s[1][0], s[1][2], s[2][0]), max3(s[2][2], s[3][0], s[3][2]));
+        float mx1 = max3(fmaxf(s[0][1], s[0][3]), max3(s[1][1], s[1][3], s[2][1]), max3(s[2][3], s[3][1], s[3][3]));
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
             mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
@@ -267,8 +506,7 @@ __device__ __forceinline__ void decode_item(const Dec4Params &p, const DecItem &
         if (__any_sync(0xffffffffu, mx0 > m0 || mx1 > m1)) {
             const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
             const float c0 = fast_exp2(m0 - n0), c1 = fast_exp2(m1 - n1);
-            l0 *= c0;
-            l1 *= c1;
+            l01 = mul2(l01, pack2(c0, c1));
 #pragma unroll
             for (int i = 0; i < 2 * kKv4Groups; i++) {
                 o[i][0] *= c0; o[i][1] *= c1; o[i][2] *= c0; o[i][3] *= c1;
@@ -278,19 +516,31 @@ __device__ __forceinline__ void decode_item(const Dec4Params &p, const DecItem &
             m0 = n0;
             m1 = n1;
         }
+        const uint64_t m01 = pack2(m0, m1);
+        uint32_t pb[4][2];  // P^T as the B operand: keys 2 t4, 2 t4 + 1 (and + 8) of the 16, head g
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float p0 = fast_exp2(s[i][0] - m0), p1 = fast_exp2(s[i][1] - m1);
-            const float p2 = fast_exp2(s[i][2] - m0), p3 = fast_exp2(s[i][3] - m1);
-            l0 += p0 + p2;
-            l1 += p1 + p3;
-            // P^T as the B operand: keys 2 t4, 2 t4 + 1 (and + 8) of the 16, head g
-            const uint32_t pb0 = movmatrix_trans(pack_half2(p0, p1)), pb1 = movmatrix_trans(pack_half2(p2, p3));
+            sub2(s[i][0], s[i][1], m01);
+            sub2(s[i][2], s[i][3], m01);
+            const float p0 = fast_exp2(s[i][0]), p1 = fast_exp2(s[i][1]), p2 = fast_exp2(s[i][2]), p3 = fast_exp2(s[i][3]);
+            add2(l01, p0, p1);
+            add2(l01, p2, p3);
+            pb[i][0] = movmatrix_trans(pack_half2(p0, p1));
+            pb[i][1] = movmatrix_trans(pack_half2(p2, p3));
+        }
+        if (!__all_sync(0xffffffffu, wait_bar(v_bar, uint32_t(used) & 1u))) {
+            late = true;
+            break;
+        }
+        used++;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t pb0 = pb[i][0], pb1 = pb[i][1];
             uint32_t da[4], db[4];
-            const uint32_t pair = tile + kKv4VGroups + (8 * i + t4) * 32;  // rows 16 i + 2 t4 and the next; + 8: 128 bytes on
-            lds128(da, pair);
-            lds128(db, pair + 128);
-            uint32_t la = lds32(pair + 16 + 4 * (g & 3)), lb = lds32(pair + 128 + 16 + 4 * (g & 3));
+            // d and lo of rows 16 i + 2 t4 and the next, and of those 8 rows on
+            lds128(da, vg_at + i * 256);
+            lds128(db, vg_at + i * 256 + 128);
+            uint32_t la = lds32(vg_at + i * 256 + 16 + 4 * (g & 3)), lb = lds32(vg_at + i * 256 + 144 + 4 * (g & 3));
             if (edge) {  // rows that the query does not see may hold anything: their d and lo count 0
                 const int ka = 16 * i + 2 * t4;
                 auto seen = [&](int r) {
@@ -312,174 +562,166 @@ __device__ __forceinline__ void decode_item(const Dec4Params &p, const DecItem &
 #pragma unroll
             for (int hf = 0; hf < 2; hf++) {  // two chunks (groups) of the 16 rows: rows 0-7 and 8-15 of each
                 uint32_t w[4];
-                const int j = lane >> 3, row = 16 * i + (j & 1) * 8 + (lane & 7), ch = (2 * hf + (j >> 1)) ^ ((row >> 1) & 3);
-                ldmatrix_x4_trans(w, tile + kKv4VCodes + row * kKv4RowBytes + ch * 16);
+                ldmatrix_x4_trans(w, (v_at ^ (hf * 32)) + i * 16 * kKv4RowBytes);
 #pragma unroll
                 for (int q2 = 0; q2 < 2; q2++) {
                     const int c = 2 * hf + q2;
                     const uint32_t b0v = mul_half2(pb0, da[c]), b1v = mul_half2(pb1, db[c]);
-                    uint32_t x = w[2 * q2], y = w[2 * q2 + 1];
-                    const uint32_t a0[4] = {x & kNib0, x & kNib1, y & kNib0, y & kNib1};
+                    const Codes x = split_codes(w[2 * q2]), y = split_codes(w[2 * q2 + 1]);
+                    const uint32_t a0[4] = {x.n0, x.n01, y.n0, y.n01}, a1[4] = {x.n2, x.n23, y.n2, y.n23};
                     mma_16816(o[2 * c], a0, b0v, b1v);
-                    x >>= 8;
-                    y >>= 8;
-                    const uint32_t a1[4] = {x & kNib0, x & kNib1, y & kNib0, y & kNib1};
                     mma_16816(o[2 * c + 1], a1, b0v, b1v);
                 }
             }
         }
-        __syncwarp();  // the whole warp is done with the stage
-        if (lane == 0 && t + kStages * kWarps < n_tiles) {
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // order the reads above before the next copy
-            load_tile(t + kStages * kWarps, stage);
-        }
+        __syncwarp();  // the whole warp is done with the V part
+        if (lane == 0 && t + kWarps < tb) load_part(t + kWarps, 1);
     }
-    if (late) {  // a copy never came: wait (bounded) for the others in flight before the CTA's memory goes back
-        for (int k = waited; warp + k * kWarps < n_tiles && k < waited - 1 + kStages; k++)
-            mbar_wait_bounded(bars + 8 * (k % kStages), uint32_t(k / kStages) & 1u);
+    const int row = p.tok0 + pc.tok;
+    const bool with_new = ends, more = next >= 0;
+    const int split = pc.split, n_split = pc.n_split, kv_head = kvh, rec0 = pc.part0 * kNHeadKv + kvh;  // this KV head's records: every fourth
+    if (more) {
+        get_piece(next);
+        if (lane == 0 && ta + warp < tb && !late) load_part(ta + warp, 0);
     }
-    if (__syncthreads_or(late)) {  // (and every warp is done with its tiles: they become the merge buffer)
+    if (__syncthreads_or(late)) {  // (and every warp is through with its V part: they become the merge buffer)
         if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 4);
+        cp_async_wait<0>();
+        if (lane == 0)
+            for (int i = 0; i < 4; i++) wait_bar(i & 1 ? v_bar : k_bar, uint32_t(i >> 1) & 1u);
+        if (tid == 0)
+            for (uint32_t i = 0; i < 2; i++) wait_bar(smem_u32(&sm.next_bar), i);
         return;
     }
+    if (more) {
+        if (tid == 0) ask_next(smem_u32(&sm.next), smem_u32(&sm.next_bar));
+        flip ^= 1;
+        finish_rows();
+    }
+    float l0, l1;
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(l0), "=f"(l1) : "l"(l01));
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) {
         l0 += __shfl_xor_sync(0xffffffffu, l0, off);
         l1 += __shfl_xor_sync(0xffffffffu, l1, off);
     }
-    float *obuf = reinterpret_cast<float *>(&sm.tile[0][0][0]);  // [warp][head][kORow]
     if (g == 0) {
         sm.red_m[warp][2 * t4] = m0; sm.red_m[warp][2 * t4 + 1] = m1;
         sm.red_l[warp][2 * t4] = l0; sm.red_l[warp][2 * t4 + 1] = l1;
     }
 #pragma unroll
     for (int c = 0; c < kKv4Groups; c++) {
-        constexpr float k0 = 16777216.f, k1 = 1048576.f;  // 2^24 and, for the second nibbles, 2^20
+        constexpr float k0 = 16777216.f, k1 = 1048576.f;  // 2^24, and 2^20 for the differences
         const float lo0 = __shfl_sync(0xffffffffu, om[0], 4 * c + t4), lo1 = __shfl_sync(0xffffffffu, om[1], 4 * c + t4);
-        float *row0 = obuf + (warp * kGqa + 2 * t4) * kORow + 32 * c + 4 * g;
         const float *e = o[2 * c], *f = o[2 * c + 1];
-        *reinterpret_cast<float4 *>(row0) = make_float4(fmaf(e[0], k0, lo0), fmaf(e[2], k1, lo0), fmaf(f[0], k0, lo0), fmaf(f[2], k1, lo0));
-        *reinterpret_cast<float4 *>(row0 + kORow) =
-            make_float4(fmaf(e[1], k0, lo1), fmaf(e[3], k1, lo1), fmaf(f[1], k0, lo1), fmaf(f[3], k1, lo1));
+        *reinterpret_cast<float4 *>(&sm.o[warp][2 * t4][32 * c + 4 * g]) =
+            make_float4(fmaf(e[0], k0, lo0), fmaf(e[2] - e[0], k1, lo0), fmaf(f[0], k0, lo0), fmaf(f[2] - f[0], k1, lo0));
+        *reinterpret_cast<float4 *>(&sm.o[warp][2 * t4 + 1][32 * c + 4 * g]) =
+            make_float4(fmaf(e[1], k0, lo1), fmaf(e[3] - e[1], k1, lo1), fmaf(f[1], k0, lo1), fmaf(f[3] - f[1], k1, lo1));
     }
     __syncthreads();
 
-    // ---- merge with the new token; a thread owns 8 dims of one head from here on
-    const bool direct = it.n_split == 1;
-    {
-        const float s_new = it.fold ? sm.s_new[mh] : -INFINITY;
-        float M = s_new;
+    // ---- merge of the warps and the new token: a lane owns four dims of each of the warp's heads
+    const int old = more ? flip ^ 1 : flip;
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) M = fmaxf(M, sm.red_m[w][mh]);
-        const float cn = it.fold ? fast_exp2(s_new - M) : 0.f;
-        float L = cn, A[8];
+    for (int i = 0; i < kHeads; i++) {
+        const int h = warp * kHeads + i, head = kv_head * kGqa + h;
+        float M = s_new[i];
 #pragma unroll
-        for (int j = 0; j < 8; j++) A[j] = 0.f;
+        for (int w = 0; w < kWarps; w++) M = fmaxf(M, sm.red_m[w][h]);
+        float L = with_new ? fast_exp2(s_new[i] - M) : 0.f, A[4] = {0.f, 0.f, 0.f, 0.f};
+        if (with_new) {
+            const uint2 hv = *reinterpret_cast<const uint2 *>(&sm.vnew[old][d0]);
+            const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&hv.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&hv.y));
+            A[0] = L * a.x; A[1] = L * a.y; A[2] = L * b.x; A[3] = L * b.y;
+        }
 #pragma unroll
         for (int w = 0; w < kWarps; w++) {
-            const float lw = sm.red_l[w][mh];
-            const float c = lw == 0.f ? 0.f : fast_exp2(sm.red_m[w][mh] - M);  // (a warp without a block: m = -inf, l = 0)
-            const float4 x = *reinterpret_cast<const float4 *>(obuf + (w * kGqa + mh) * kORow + md);
-            const float4 y = *reinterpret_cast<const float4 *>(obuf + (w * kGqa + mh) * kORow + md + 4);
+            const float lw = sm.red_l[w][h];
+            const float c = lw == 0.f ? 0.f : fast_exp2(sm.red_m[w][h] - M);  // (a warp without a tile: m = -inf, l = 0)
+            const float4 x = *reinterpret_cast<const float4 *>(&sm.o[w][h][d0]);
             L += lw * c;
             A[0] += x.x * c; A[1] += x.y * c; A[2] += x.z * c; A[3] += x.w * c;
-            A[4] += y.x * c; A[5] += y.y * c; A[6] += y.z * c; A[7] += y.w * c;
         }
-        if (it.fold) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) A[j] = fmaf(cn, __half2float(sm.vnew[md + j]), A[j]);
-        }
-        if (direct) {
-            const float sink2 = sink * kLog2e;
+        if (n_split == 1) {
+            const float sink2 = sm.sinks[head] * kLog2e;
             const float Mf = fmaxf(M, sink2), cf = fast_exp2(M - Mf);
             const float inv = cf / (L * cf + fast_exp2(sink2 - Mf));
-#pragma unroll
-            for (int j = 0; j < 8; j++) A[j] *= inv;
-            store_out8(p.out, p.out_dtype, size_t(it.tok) * kQDim + head * kHeadDim + md, A);
-            return;
+            store_out4(p.out, p.out_dtype, size_t(row) * kQDim + head * kHeadDim + d0, A[0] * inv, A[1] * inv, A[2] * inv, A[3] * inv);
+        } else {  // this piece's record: acc, m (base 2), l
+            float *rec = p.scratch + (size_t(rec0 + split * kNHeadKv) * kGqa + h) * kRecStride;
+            *reinterpret_cast<float4 *>(rec + d0) = make_float4(A[0], A[1], A[2], A[3]);
+            if (lane == 0) *reinterpret_cast<float2 *>(rec + kHeadDim) = make_float2(M, L);
         }
-        float *rec = p.scratch + ((size_t(it.part0) + it.split) * kGqa + mh) * kRecStride;
-        *reinterpret_cast<float4 *>(rec + md) = make_float4(A[0], A[1], A[2], A[3]);
-        *reinterpret_cast<float4 *>(rec + md + 4) = make_float4(A[4], A[5], A[6], A[7]);
-        if (md == 0) { rec[kHeadDim] = M * kLn2; rec[kHeadDim + 1] = L; }
     }
+    __syncthreads();  // the merge buffer is free, the next piece's rows are there
 
-    // ---- split-K merge by the last CTA of the group, in two levels (the half-precision kernel has the reasons)
-    const int sub = it.split / kMergeFan, n_sub = (it.n_split + kMergeFan - 1) / kMergeFan;
-    const int sub_size = min(kMergeFan, it.n_split - sub * kMergeFan);
-    __syncthreads();
-    if (tid == 0) {
-        const bool last = ticket_acq_rel(&p.tickets[it.sub0 + sub]) == sub_size - 1;
-        if (last) p.tickets[it.sub0 + sub] = 0;
-        sm.is_last = last;
+    // ---- split-K: the last piece of a run of records to arrive merges the run.  The record stores are ordered before thread
+    // 0's ticket by the barrier, and the ticket is an acquire-release atomic at device scope, cumulative over them; the
+    // readers go past L1.  The ticket's answer is looked at after the next piece: no piece waits for the round trip.
+    if (waiting && sm.done[(turn & 1) ^ 1].last) merge_run((turn & 1) ^ 1);
+    waiting = n_split > 1;
+    if (waiting && tid == 0) {
+        const int fan = dec4_fan(n_split), sub = split / fan;
+        int *ticket = &p.tickets[rec0 + sub * kNHeadKv];
+        const bool last = ticket_acq_rel(ticket) == min(fan, n_split - sub * fan) - 1;
+        if (last) *ticket = 0;  // ready for the next launch; nothing in this one waits for it
+        sm.done[turn & 1] = {rec0, split, n_split, kv_head, row, last};
     }
-    __syncthreads();
-    if (!sm.is_last) return;
-    const float *src = p.scratch + ((size_t(it.part0) + sub * kMergeFan) * kGqa + mh) * kRecStride;
-    int n_src = sub_size;
-    bool final_level = n_sub == 1;
-    Merged r;
-    for (;;) {
-        r = merge_records(src, n_src, md, final_level, sink);
-        if (final_level) break;
-        float *rec2 = p.scratch2 + ((size_t(it.sub0) + sub) * kGqa + mh) * kRecStride;
-        *reinterpret_cast<float4 *>(rec2 + md) = make_float4(r.a[0], r.a[1], r.a[2], r.a[3]);
-        *reinterpret_cast<float4 *>(rec2 + md + 4) = make_float4(r.a[4], r.a[5], r.a[6], r.a[7]);
-        if (md == 0) { rec2[kHeadDim] = r.M; rec2[kHeadDim + 1] = r.L; }
+    if (!more) {
         __syncthreads();
-        if (tid == 0) {
-            const bool last = ticket_acq_rel(&p.tickets2[it.group]) == n_sub - 1;
-            if (last) p.tickets2[it.group] = 0;
-            sm.is_last = last;
-        }
-        __syncthreads();
-        if (!sm.is_last) return;
-        src = p.scratch2 + (size_t(it.sub0) * kGqa + mh) * kRecStride;
-        n_src = n_sub;
-        final_level = true;
+        if (waiting && sm.done[turn & 1].last) merge_run(int(turn & 1));
+        break;
     }
-    const float inv = 1.0f / r.L;
-#pragma unroll
-    for (int j = 0; j < 8; j++) r.a[j] *= inv;
-    store_out8(p.out, p.out_dtype, size_t(it.tok) * kQDim + head * kHeadDim + md, r.a);
-}
-
-__global__ void __launch_bounds__(kThreads, 2) k_decode_kv4(const Dec4Params p) {
-    const DecItem it = p.items[blockIdx.x];
-    decode_item(p, it);
+    }  // pieces
 }
 
 template <int kCap>
-__global__ void __launch_bounds__(kThreads, 2)
-    k_decode_kv4_p(const __grid_constant__ Dec4Params p, const __grid_constant__ DecItemsParam<kCap> ip) {
-    const DecItem it = ip.items[blockIdx.x];
-    decode_item(p, it);
+struct Dec4List {
+    Dec4Piece pieces[kCap];
+};
+
+template <int kCap, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
+    k_decode_kv4(const __grid_constant__ Dec4Params p, const __grid_constant__ Dec4List<kCap> list) {
+    decode_pieces<kWarps>(p, list.pieces);
 }
 
-template <int kCap>
-cudaError_t launch_inline(const Dec4Params &p, const DecItem *host_items, int n_items, cudaStream_t stream) {
-    static thread_local DecItemsParam<kCap> ip;  // copied into the launch by the runtime before this returns
-    memcpy(ip.items, host_items, sizeof(DecItem) * size_t(n_items));
-    return launch_pdl(k_decode_kv4_p<kCap>, n_items, kThreads, sizeof(Dec4Smem), stream, p, ip);
+// The parameter block is copied at every launch, so the kernel comes in three capacities and a launch takes the smallest
+// that fits (the smallest one stays inside the classic 4 KiB parameter space).
+constexpr int kSmallPieces = 160, kMidPieces = 512;
+static_assert(sizeof(Dec4Params) + sizeof(Dec4List<kSmallPieces>) <= 4096, "small variant");
+static_assert(sizeof(Dec4Params) + sizeof(Dec4List<kDec4MaxPieces>) <= 32764, "largest variant fits the limit");
+
+template <int kCap, int kWarps>
+cudaError_t launch_list(const Dec4Params &p, const Dec4Piece *pieces, int n_pieces, cudaStream_t stream) {
+    static thread_local Dec4List<kCap> list;  // copied into the launch by the runtime before this returns
+    memcpy(list.pieces, pieces, sizeof(Dec4Piece) * size_t(n_pieces));
+    return launch_pdl(k_decode_kv4<kCap, kWarps>, n_pieces * kNHeadKv, kWarps * 32, sizeof(Dec4Smem<kWarps>), stream, p, list);
 }
+
+template <int kCap, int kWarps>
+cudaError_t setup_list() { return allow_smem(k_decode_kv4<kCap, kWarps>, sizeof(Dec4Smem<kWarps>)); }
 
 }  // namespace
 
 cudaError_t decode_kv4_setup() {
-    cudaError_t e = allow_smem(k_decode_kv4, sizeof(Dec4Smem));
-    if (e == cudaSuccess) e = allow_smem(k_decode_kv4_p<kCapSmall>, sizeof(Dec4Smem));
-    if (e == cudaSuccess) e = allow_smem(k_decode_kv4_p<kCapMid>, sizeof(Dec4Smem));
-    if (e == cudaSuccess) e = allow_smem(k_decode_kv4_p<kMaxParamItems>, sizeof(Dec4Smem));
+    cudaError_t e = setup_list<kSmallPieces, 8>();
+    if (e == cudaSuccess) e = setup_list<kMidPieces, 8>();
+    if (e == cudaSuccess) e = setup_list<kDec4MaxPieces, 8>();
+    if (e == cudaSuccess) e = setup_list<kMidPieces, 4>();
+    if (e == cudaSuccess) e = setup_list<kDec4MaxPieces, 4>();
     return e;
 }
 
-cudaError_t launch_decode_kv4(const Dec4Params &p, const DecItem *inline_items, int n_items, cudaStream_t stream) {
-    if (n_items <= 0) return cudaSuccess;
-    if (!inline_items) return launch_pdl(k_decode_kv4, n_items, kThreads, sizeof(Dec4Smem), stream, p);
-    if (n_items > kMaxParamItems) return cudaErrorInvalidValue;
-    if (n_items <= kCapSmall) return launch_inline<kCapSmall>(p, inline_items, n_items, stream);
-    if (n_items <= kCapMid) return launch_inline<kCapMid>(p, inline_items, n_items, stream);
-    return launch_inline<kMaxParamItems>(p, inline_items, n_items, stream);
+cudaError_t launch_decode_kv4(const Dec4Params &p, const Dec4Piece *pieces, int n_pieces, int n_warps, cudaStream_t stream) {
+    if (n_pieces <= 0) return cudaSuccess;
+    if (n_pieces > kDec4MaxPieces) return cudaErrorInvalidValue;
+    if (n_warps == 8 && n_pieces <= kSmallPieces) return launch_list<kSmallPieces, 8>(p, pieces, n_pieces, stream);
+    if (n_warps == 8 && n_pieces <= kMidPieces) return launch_list<kMidPieces, 8>(p, pieces, n_pieces, stream);
+    if (n_warps == 8) return launch_list<kDec4MaxPieces, 8>(p, pieces, n_pieces, stream);
+    if (n_pieces <= kMidPieces) return launch_list<kMidPieces, 4>(p, pieces, n_pieces, stream);
+    return launch_list<kDec4MaxPieces, 4>(p, pieces, n_pieces, stream);
 }
 
 }  // namespace flint

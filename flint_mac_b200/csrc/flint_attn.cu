@@ -257,6 +257,8 @@ struct flint_attn {
     std::vector<int> plan_victim;       // per layer: the way the next unknown batch replaces
     PlanScratch plan_scratch;
     std::vector<int32_t> batch_pos;
+    std::vector<int> kv4_tiles;
+    std::vector<Dec4Piece> kv4_pieces;
     std::vector<uint32_t> seen;  // per sequence: the number of the last decode batch it appeared in
     uint32_t batch_no = 0;
     // peer-memory exchange of partial records (KV-range sharding): one cudaMalloc block per rank, opened by the
@@ -408,6 +410,39 @@ struct flint_attn {
         size_t bytes = 0;
     };
 
+    // Decode over a 4-bit cache.
+    void decode_kv4(Layer &L, int n, const int32_t *seqs, const int32_t *p, const void *qkv, int qkv_dtype, void *out,
+                    int out_dtype, cudaStream_t st, const HostRows *rows) {
+        if (rows) {  // page-locked rows are read where they lie, as in decode_dev
+            const bool in_place = rows->mapped && n * kNHeadKv * 2 >= target_items;
+            if (!in_place) CK(cudaMemcpyAsync(rows->staging, rows->host, rows->bytes, cudaMemcpyHostToDevice, st));
+            qkv = in_place ? rows->mapped : rows->staging;
+        }
+        Dec4Params dp{};
+        dp.qkv = qkv;
+        dp.out = out;
+        dp.q_norm = L.q_norm; dp.k_norm = L.k_norm; dp.sinks = L.sinks; dp.inv_freq = inv_freq;
+        dp.cache = L.kv4;
+        dp.is_swa = L.is_swa; dp.has_rope = L.has_rope;
+        dp.qkv_dtype = qkv_dtype; dp.out_dtype = out_dtype;
+        dp.error_flag = dec_err;
+        time_mark(st);
+        kv4_tiles.resize(n);
+        for (int i = 0; i < n; i++) kv4_tiles[i] = dec4_range(p[i], L.is_swa, L.kv4.first_tokens).tiles;
+        for (int i0 = 0; i0 < n;) {
+            int n_records = 0, n_warps = 0;
+            const int m = plan_decode_kv4(n - i0, seqs + i0, p + i0, kv4_tiles.data() + i0, target_items, kv4_pieces, n_records, n_warps);
+            ensure_scratch(n_records * kNHeadKv, n_records * kNHeadKv, n_records * kNHeadKv);
+            dp.scratch = scratch; dp.scratch2 = scratch2;
+            dp.tickets = tickets; dp.tickets2 = tickets + n_records * kNHeadKv;
+            dp.tok0 = i0;
+            CK(launch_decode_kv4(dp, kv4_pieces.data(), int(kv4_pieces.size()), n_warps, st));
+            launches++;
+            i0 += m;
+        }
+        time_mark(st);
+    }
+
     // mode 0: out [n][4096]; mode 1: partial_out [n][32][130]; mode 2: records to every peer's gather buffer
     void decode_dev(int il, int n, const int32_t *seqs, const void *qkv, int qkv_dtype, void *out, int out_dtype,
                     float *partial_out, int mode, cudaStream_t st, uint32_t step = 0, const HostRows *rows = nullptr) {
@@ -438,6 +473,10 @@ struct flint_attn {
             if (want > free_pages.size())
                 throw std::runtime_error("KV page pool exhausted (" + std::to_string(kv_pages) + " pages of 64 keys)");
             for (int i = 0; i < n; i++) ensure_pages(seqs[i], p[i], st);
+        }
+        if (L.kv4.blocks) {
+            decode_kv4(L, n, seqs, p.data(), qkv, qkv_dtype, out, out_dtype, st, rows);
+            return;
         }
         PlanCache *hit = nullptr;
         for (int w = 0; w < kPlanWays && !hit; w++) {
@@ -479,25 +518,6 @@ struct flint_attn {
         }
         ensure_scratch(n_records, n_subs, n_groups);
         const bool inline_items = items.size() <= size_t(kMaxParamItems);
-        if (L.kv4.blocks) {
-            Dec4Params dp{};
-            dp.items = inline_items ? nullptr : upload_items(items, st);
-            dp.qkv = qkv;
-            dp.out = out;
-            dp.q_norm = L.q_norm; dp.k_norm = L.k_norm; dp.sinks = L.sinks; dp.inv_freq = inv_freq;
-            dp.cache = L.kv4;
-            dp.scratch = scratch; dp.scratch2 = scratch2;
-            dp.tickets = tickets; dp.tickets2 = tickets + n_subs;
-            dp.is_swa = L.is_swa; dp.has_rope = L.has_rope;
-            dp.qkv_dtype = qkv_dtype; dp.out_dtype = out_dtype;
-            dp.error_flag = dec_err;
-            time_mark(st);
-            CK(launch_decode_kv4(dp, inline_items ? items.data() : nullptr, int(items.size()), st));
-            time_mark(st);
-            launches++;
-            if (!inline_items) mark_ring_used(dp.items, st);
-            return;
-        }
         DecParams dp{};
         dp.items = inline_items ? nullptr : upload_items(items, st);
         dp.qkv = qkv;
@@ -594,7 +614,7 @@ flint_attn *flint_attn_open_kv(const flint_attn_config *cfg, const flint_attn_kv
         a->kv_format = kv_format;
         a->first_tokens = first_tokens;
         a->sm_count = prop.multiProcessorCount;
-        a->target_items = a->sm_count * 2;
+        a->target_items = a->sm_count * (kv_format == FLINT_ATTN_KV_INT4 ? kDec4CtasPerSm : 2);
         a->pos.assign(cfg->max_seqs, 0);
         if (cfg->kv_pages > 0) {
             a->kv_pages = cfg->kv_pages;
@@ -611,6 +631,7 @@ flint_attn *flint_attn_open_kv(const flint_attn_config *cfg, const flint_attn_kv
         CK(decode_kernel_setup());
         CK(prefill_kernel_setup());
         CK(decode_kv4_setup());
+        CK(kv_rows_setup());
         CK(cudaMalloc(&a->dec_err, sizeof(int)));
         CK(cudaMemset(a->dec_err, 0, sizeof(int)));
         float freq[kHeadDim / 2];
@@ -1358,6 +1379,33 @@ int32_t flint_attn_plan_decode(int32_t n, const int32_t *pos, int32_t is_swa, in
         memcpy(out + 8 * i, rec, sizeof(rec));
     }
     return int32_t(items.size());
+}
+
+int32_t flint_attn_plan_decode_int4(int32_t n, const int32_t *pos, int32_t is_swa, int32_t first_tokens,
+                                    int32_t target_items, int32_t *out, int32_t cap) {
+    try {
+        if (n <= 0 || first_tokens < 0 || !pos || !out) return -1;
+        std::vector<int> tiles(n);
+        std::vector<Dec4Piece> pieces;
+        for (int i = 0; i < n; i++) {
+            if (pos[i] < 0) return -1;
+            tiles[i] = dec4_range(pos[i], is_swa != 0, first_tokens).tiles;
+        }
+        int count = 0;
+        for (int i0 = 0, launch = 0; i0 < n; launch++) {
+            int n_records = 0, n_warps = 0;
+            const int m = plan_decode_kv4(n - i0, pos + i0, pos + i0, tiles.data() + i0, target_items, pieces, n_records, n_warps);
+            for (const Dec4Piece &p : pieces) {
+                if (count == cap) return -1;
+                const int32_t rec[8] = {i0 + p.tok, p.t0, p.t0 + p.n, p.split, p.n_split, p.part0, launch, n_records};
+                memcpy(out + 8 * count++, rec, sizeof(rec));
+            }
+            i0 += m;
+        }
+        return count;
+    } catch (const std::exception &) {
+        return -1;
+    }
 }
 
 int32_t flint_attn_set_target_items(flint_attn *a, int32_t target_items) {

@@ -1,4 +1,5 @@
 // Rows of K and V in and out of a layer's cache on the device (4-bit caches, and half-precision ones).
+#include "decode_common.cuh"
 #include "kv4.cuh"
 
 namespace flint {
@@ -43,6 +44,8 @@ __device__ __forceinline__ long long half_row(const KvRowsParams &p, int seq, in
 
 // One warp per (sequence, row, KV head): K's row, then V's.
 __global__ void __launch_bounds__(256) k_kv_store(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs, int n) {
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const int lane = threadIdx.x & 31;
     const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (w >= (long long)n * p.n_rows * kNHeadKv) return;
@@ -74,6 +77,8 @@ __global__ void __launch_bounds__(256) k_kv_store(const KvRowsParams p, const __
 }
 
 __global__ void __launch_bounds__(256) k_kv_load(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs, int n) {
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const int lane = threadIdx.x & 31;
     const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (w >= (long long)n * p.n_rows * kNHeadKv) return;
@@ -95,18 +100,24 @@ __global__ void __launch_bounds__(256) k_kv_load(const KvRowsParams p, const __g
 
 }  // namespace
 
+// The SM's memory is split as the decode kernel wants it: a kernel in between that wants another split makes the next one wait
+// for the SMs to be set up again.
+cudaError_t kv_rows_setup() {
+    cudaError_t e = cudaFuncSetAttribute(k_kv_store, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_kv_load, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    return e;
+}
+
 cudaError_t launch_kv_store(const KvRowsParams &p, const KvRowsSeqs &seqs, int n, cudaStream_t stream) {
     const long long warps = (long long)n * p.n_rows * kNHeadKv;
     if (warps <= 0) return cudaSuccess;
-    k_kv_store<<<unsigned((warps + 7) / 8), 256, 0, stream>>>(p, seqs, n);
-    return cudaGetLastError();
+    return launch_pdl(k_kv_store, int((warps + 7) / 8), 256, 0, stream, p, seqs, n);
 }
 
 cudaError_t launch_kv_load(const KvRowsParams &p, const KvRowsSeqs &seqs, int n, cudaStream_t stream) {
     const long long warps = (long long)n * p.n_rows * kNHeadKv;
     if (warps <= 0) return cudaSuccess;
-    k_kv_load<<<unsigned((warps + 7) / 8), 256, 0, stream>>>(p, seqs, n);
-    return cudaGetLastError();
+    return launch_pdl(k_kv_load, int((warps + 7) / 8), 256, 0, stream, p, seqs, n);
 }
 
 }  // namespace flint

@@ -18,6 +18,7 @@
 #pragma once
 
 #include "attn_common.h"
+#include "kv4_plan.h"
 
 namespace flint {
 
@@ -46,19 +47,19 @@ struct Kv4Cache {
 
 // One decode launch over 4-bit caches (the fields that DecParams has mean the same).
 struct Dec4Params {
-    const DecItem *items;
     const void *qkv;
     void *out;
     const float *q_norm, *k_norm, *sinks, *inv_freq;
     Kv4Cache cache;
-    float *scratch, *scratch2;
-    int *tickets, *tickets2;
+    float *scratch, *scratch2;  // split-K records of both merge levels, [n_records][4 KV heads][8][kRecStride]
+    int *tickets, *tickets2;    // arrival counters, [n_records][4]; zero between launches
+    int tok0;                   // row of qkv and out that the launch's token 0 has
     int is_swa, has_rope, qkv_dtype, out_dtype;
     int *error_flag;
 };
 cudaError_t decode_kv4_setup();
-// The work list travels in the kernel's parameters when `inline_items` is given (at most kMaxParamItems), else it is p.items.
-cudaError_t launch_decode_kv4(const Dec4Params &p, const DecItem *inline_items, int n_items, cudaStream_t stream);
+// The work list (kv4_plan.h; at most kDec4MaxPieces) travels in the kernel's parameters.
+cudaError_t launch_decode_kv4(const Dec4Params &p, const Dec4Piece *pieces, int n_pieces, int n_warps, cudaStream_t stream);
 
 // Rows of K and V between a cache and dense arrays [n][4][n_rows][128]: row r of sequence i is position pos0[i] + r.
 constexpr int kKvRowsSeqs = 128;  // sequences a launch names in its parameters
@@ -76,6 +77,7 @@ struct KvRowsParams {
     long long seq_stride = 0, head_stride = 0;  // elements of k and v
     void *k = nullptr, *v = nullptr;
 };
+cudaError_t kv_rows_setup();
 cudaError_t launch_kv_store(const KvRowsParams &p, const KvRowsSeqs &seqs, int n, cudaStream_t stream);
 cudaError_t launch_kv_load(const KvRowsParams &p, const KvRowsSeqs &seqs, int n, cudaStream_t stream);
 

@@ -267,6 +267,12 @@ int32_t flint_attn_pages_free(const flint_attn *a);
  * src/engine.mm:742-743, is tuned for 32 splits on an M5).  Returns the item count, or -1 if cap is too small. */
 int32_t flint_attn_plan_decode(int32_t n, const int32_t *pos, int32_t is_swa, int32_t kv_lo, int32_t kv_hi,
                                int32_t target_items, int32_t *items, int32_t cap);
+/* The same for decode over a 4-bit cache: one record of 8 int32 per piece of a token's visible keys, for each of the four
+ * KV heads alike = { token, tile0, tile1, split, n_split, first_record, launch, records_of_launch }.  Tiles are 64 keys,
+ * the first tokens' one in front where the token sees any; the pieces of a token tile all its tiles once.  Returns the
+ * piece count, or -1 if cap is too small. */
+int32_t flint_attn_plan_decode_int4(int32_t n, const int32_t *pos, int32_t is_swa, int32_t first_tokens,
+                                    int32_t target_items, int32_t *pieces, int32_t cap);
 /* Tuning knob: work items the planner aims for per launch (default: one wave of 2 CTAs on every SM). */
 int32_t flint_attn_set_target_items(flint_attn *a, int32_t target_items);
 /* Number of kernel launches this handle has enqueued so far. */

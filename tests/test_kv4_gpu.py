@@ -41,6 +41,38 @@ def test_statement_keeps_what_it_says():
     assert (err <= d * (0.5 + 15 * 2.0**-11)).all()
 
 
+@pytest.mark.parametrize("is_swa,first", [(False, 0), (True, 0), (True, 5), (True, 64)])
+@pytest.mark.parametrize("target", [1, 7, 100, 296])
+def test_plan_covers_every_tile_once(fa, is_swa, first, target):
+    """Whatever the batch: every tile of every token in one piece, the pieces of a launch longest first, their records and
+    counters apart from each other, and windows whole."""
+    rng = np.random.default_rng(target)
+    batches = [[0], [1], [64], [65], [131072], [0, 0, 0], [8192] * 64, [100] * 300, list(range(0, 2000, 7)), [131072, 0, 5, 5],
+               [int(x) for x in np.exp(rng.uniform(0, 11, 200))], [int(x) for x in rng.integers(0, 600, 2048)], [1 << 30, 3, 1 << 20]]
+    for pos in batches:
+        pcs = fa.plan_decode_int4(pos, is_swa, first, target)
+        assert (np.diff(pcs[:, 6]) >= 0).all() and np.bincount(pcs[:, 6]).max() <= 1300
+        for launch in set(pcs[:, 6]):
+            mine = pcs[pcs[:, 6] == launch]
+            assert (np.diff(mine[:, 2] - mine[:, 1]) <= 0).all()
+            cut = mine[mine[:, 4] > 1]
+            records = cut[:, 5] + cut[:, 3]
+            assert sorted(records) == list(range(len(cut))) and (mine[:, 7] == len(cut)).all()
+        assert set(pcs[:, 0]) == set(range(len(pos)))
+        for i, p in enumerate(pos):
+            j0 = max(p - 512, 0) if is_swa else 0
+            tiles = (1 if is_swa and min(first, j0) > 0 else 0) + (0 if p == j0 else (p - 1) // 64 - j0 // 64 + 1)
+            mine = pcs[pcs[:, 0] == i]
+            mine = mine[np.argsort(mine[:, 3])]
+            n = len(mine)
+            assert (mine[:, 3] == range(n)).all() and (mine[:, 4] == n).all() and len(set(mine[:, 6])) == 1
+            assert mine[0, 1] == 0 and mine[-1, 2] == tiles and (mine[1:, 1] == mine[:-1, 2]).all()
+            assert n == 1 or (mine[:, 2] > mine[:, 1]).all()
+            assert n == 1 or not is_swa
+    with pytest.raises(fa.FlintAttnError):
+        fa.plan_decode_int4([5, -1], is_swa, first, target)
+
+
 gpu = pytest.mark.gpu
 
 
