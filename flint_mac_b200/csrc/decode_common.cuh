@@ -181,14 +181,14 @@ constexpr int kCapSmall = 76, kCapMid = 304;  // 304: one wave of items on a 148
 // has finished (it waits inside, see decode_item), which hides launch latency between the short kernels of a decode
 // step.  FLINT_ATTN_NO_PDL=1 in the environment turns it off.
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_pdl(void (*kernel)(KArgs...), int n_items, int n_threads, size_t smem_bytes,
+inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, int n_threads, size_t smem_bytes,
                        cudaStream_t stream, const Args &...args) {
     static const bool off = [] {
         const char *v = getenv("FLINT_ATTN_NO_PDL");
         return v && v[0] == '1';
     }();
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(n_items));
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(unsigned(n_threads));
     cfg.dynamicSmemBytes = smem_bytes;
     cfg.stream = stream;

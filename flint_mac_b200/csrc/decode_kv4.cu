@@ -315,11 +315,9 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
     auto store_new = [&] {  // the new token's rows -> the cache (warps 0 and 1)
         if (!ends || warp >= 2) return;
         const uint2 h = *reinterpret_cast<const uint2 *>(warp == 0 ? &sm.knew[d0] : &sm.vnew[flip][d0]);
-        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&h.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
-        const float f[4] = {a.x, a.y, b.x, b.y};
-        kv4_store_lane(kv4_block(p.cache, pc.seq, kvh, pc.pos >> 6), pc.pos & 63, warp == 1, lane, f);
+        kv4_store_lane(kv4_block(p.cache, pc.seq, kvh, pc.pos >> 6), pc.pos & 63, warp == 1, lane, h);
         if (p.is_swa && pc.pos < p.cache.first_tokens)
-            kv4_store_lane(kv4_first_block(p.cache, pc.seq, kvh), pc.pos, warp == 1, lane, f);
+            kv4_store_lane(kv4_first_block(p.cache, pc.seq, kvh), pc.pos, warp == 1, lane, h);
     };
     // Split-K: merges the run of records that piece `w` was the last of to arrive, and if that was the group's last run, the
     // runs (the whole CTA calls this).

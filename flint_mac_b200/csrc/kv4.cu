@@ -1,4 +1,6 @@
 // Rows of K and V in and out of a layer's cache on the device (4-bit caches, and half-precision ones).
+#include <climits>
+
 #include "decode_common.cuh"
 #include "kv4.cuh"
 
@@ -42,82 +44,248 @@ __device__ __forceinline__ long long half_row(const KvRowsParams &p, int seq, in
     return (((long long)seq * kNHeadKv + kvh) * p.n_slots + slot) * kHeadDim;
 }
 
-// One warp per (sequence, row, KV head): K's row, then V's.
-__global__ void __launch_bounds__(256) k_kv_store(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs, int n) {
+// ---- half-precision caches: one warp per (sequence, row, KV head)
+__global__ void __launch_bounds__(256) k_half_store(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs, int n) {
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const int lane = threadIdx.x & 31;
     const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (w >= (long long)n * p.n_rows * kNHeadKv) return;
     const int kvh = int(w % kNHeadKv), r = int(w / kNHeadKv % p.n_rows), i = int(w / kNHeadKv / p.n_rows);
-    const int seq = seqs.seq[i], pos = seqs.pos0[i] + r;
     // positions r and r + 1024 of one call share a slot of a ring: only the last one of a slot is stored, whatever the order
     // in which the warps run
-    const bool to_ring = !p.is_swa || p.raw_slots || r + kSwaRing >= p.n_rows;
-    const bool raw_first = p.is_swa && p.raw_slots && pos >= kSwaRing;
-    const bool to_first = p.is_swa && !p.raw_slots && pos < p.cache.first_tokens;
+    if (p.is_swa && r + kSwaRing < p.n_rows) return;
     const size_t at = size_t(i) * p.seq_stride + size_t(kvh) * p.head_stride + size_t(r) * kHeadDim + 4 * lane;
-    if (!to_ring && !to_first) return;
+    const long long row = half_row(p, seqs.seq[i], kvh, seqs.pos0[i] + r);
+    row_store4(p.k_cache, kDtypeF16, size_t(row) + 4 * lane, row_load4(p.k, p.dtype, at));
+    row_store4(p.v_cache, kDtypeF16, size_t(row) + 4 * lane, row_load4(p.v, p.dtype, at));
+}
+
+__global__ void __launch_bounds__(256) k_half_load(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs, int n) {
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    const int lane = threadIdx.x & 31;
+    const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (w >= (long long)n * p.n_rows * kNHeadKv) return;
+    const int kvh = int(w % kNHeadKv), r = int(w / kNHeadKv % p.n_rows), i = int(w / kNHeadKv / p.n_rows);
+    const size_t at = size_t(i) * p.seq_stride + size_t(kvh) * p.head_stride + size_t(r) * kHeadDim + 4 * lane;
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    const long long row = half_row(p, seqs.seq[i], kvh, seqs.pos0[i] + r);
+    row_store4(p.k, p.dtype, at, row < 0 ? zero : row_load4(p.k_cache, kDtypeF16, size_t(row) + 4 * lane));
+    row_store4(p.v, p.dtype, at, row < 0 ? zero : row_load4(p.v_cache, kDtypeF16, size_t(row) + 4 * lane));
+}
+
+// ---- 4-bit caches: one CTA per (sequence, KV head, block of 64 positions), so that a block's codes are written or read by
+// one CTA.  Eight neighbouring values a lane (one 16-byte access in half precision, four bytes of codes): 16 lanes a row,
+// four lanes a group, two neighbouring rows a warp; a thread's loads are all in flight before the first is used.
+// Both are bound by memory: TIMES
+constexpr int kRowThreads = 256;
+constexpr int kRowSteps = kKv4BlockKeys * 16 / kRowThreads;  // rows of a lane in a block
+
+template <int kType>
+struct Eight;  // eight values of a row as they lie in memory
+template <>
+struct Eight<kDtypeF32> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const void *base, size_t elem) {
+        a = __ldcs(reinterpret_cast<const float4 *>(static_cast<const float *>(base) + elem));
+        b = __ldcs(reinterpret_cast<const float4 *>(static_cast<const float *>(base) + elem) + 1);
+    }
+    // the values, rounded to half
+    __device__ __forceinline__ uint4 get() const {
+        return make_uint4(pack_half2(a.x, a.y), pack_half2(a.z, a.w), pack_half2(b.x, b.y), pack_half2(b.z, b.w));
+    }
+    static __device__ __forceinline__ void store(void *base, size_t elem, const float (&x)[8]) {
+        float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(base) + elem);
+        __stcs(p, make_float4(x[0], x[1], x[2], x[3]));
+        __stcs(p + 1, make_float4(x[4], x[5], x[6], x[7]));
+    }
+};
+template <>
+struct Eight<kDtypeBf16> {
+    uint4 a;
+    __device__ __forceinline__ void load(const void *base, size_t elem) {
+        a = __ldcs(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + elem));
+    }
+    __device__ __forceinline__ uint4 get() const {
+        auto half2_of = [](uint32_t w) { return pack_half2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); };
+        return make_uint4(half2_of(a.x), half2_of(a.y), half2_of(a.z), half2_of(a.w));
+    }
+    static __device__ __forceinline__ void store(void *base, size_t elem, const float (&x)[8]) {
+        uint32_t w[4];
 #pragma unroll
-    for (int is_v = 0; is_v < 2; is_v++) {
-        const float4 f = row_load4(is_v ? p.v : p.k, p.dtype, at);
-        const uint2 h = make_uint2(pack_half2(f.x, f.y), pack_half2(f.z, f.w));
-        if (!p.cache.blocks) {
-            *reinterpret_cast<uint2 *>((is_v ? p.v_cache : p.k_cache) + half_row(p, seq, kvh, pos) + 4 * lane) = h;
-            continue;
+        for (int i = 0; i < 4; i++) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&b);
         }
-        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&h.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
-        const float x[4] = {a.x, a.y, b.x, b.y};
-        if (to_ring) {
-            unsigned char *block = raw_first ? kv4_first_block(p.cache, seq, kvh) : kv4_block(p.cache, seq, kvh, pos >> 6);
-            kv4_store_lane(block, pos & 63, is_v, lane, x);
-        }
-        if (to_first) kv4_store_lane(kv4_first_block(p.cache, seq, kvh), pos, is_v, lane, x);
+        __stcs(reinterpret_cast<uint4 *>(static_cast<uint16_t *>(base) + elem), make_uint4(w[0], w[1], w[2], w[3]));
+    }
+};
+template <>
+struct Eight<kDtypeF16> {
+    uint4 a;
+    __device__ __forceinline__ void load(const void *base, size_t elem) {
+        a = __ldcs(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + elem));
+    }
+    __device__ __forceinline__ uint4 get() const { return a; }
+    static __device__ __forceinline__ void store(void *base, size_t elem, const float (&x)[8]) {
+        __stcs(reinterpret_cast<uint4 *>(static_cast<uint16_t *>(base) + elem),
+               make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7])));
+    }
+};
+
+// The rows of a block that a call has: positions (slots, when p.raw_slots) p0 .. p0 + n_rows - 1.
+struct BlockRows {
+    int seq, kvh, first, block;  // first: position of the block's row 0
+    size_t base;                 // element of position 0's row in k and v
+    int p0, p1;
+    __device__ __forceinline__ BlockRows(const KvRowsParams &p, const KvRowsSeqs &seqs) {
+        const int i = blockIdx.z;
+        kvh = blockIdx.y % kNHeadKv;
+        seq = seqs.seq[i];
+        p0 = seqs.pos0[i];
+        p1 = p0 + p.n_rows;
+        block = (p0 >> 6) + int(blockIdx.x);
+        first = block * kKv4BlockKeys;
+        base = size_t(i) * p.seq_stride + size_t(kvh) * p.head_stride - size_t(p0) * kHeadDim;  // (wraps; added to p0 or more)
+    }
+    __device__ __forceinline__ bool has(int r) const { return first + r >= p0 && first + r < p1; }
+};
+// A block by position, or by slot (the first tokens' block follows the ring's).
+__device__ __forceinline__ unsigned char *block_of(const KvRowsParams &p, const BlockRows &b) {
+    if (!p.raw_slots || p.cache.block_table) return kv4_block(p.cache, b.seq, b.kvh, b.block);
+    return p.cache.blocks + ((size_t(b.seq) * kNHeadKv + b.kvh) * p.cache.blocks_per_seq + b.block) * kKv4BlockBytes;
+}
+
+// Storing is bound by instructions, so a lane has sixteen values here (half a group: one exchange between lanes, d and lo
+// worked out by two lanes instead of four), eight lanes a row, and K and V of a block are separate CTAs.
+constexpr int kStoreSteps = kKv4BlockKeys * 8 / kRowThreads;
+template <int kType>
+__global__ void __launch_bounds__(kRowThreads, 6) k_kv4_store(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs) {
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    const bool is_v = blockIdx.y >= kNHeadKv;
+    const BlockRows b(p, seqs);
+    if (b.first >= b.p1) return;
+    const int sub = threadIdx.x & 7, g = sub >> 1, r0 = threadIdx.x >> 3;  // rows r0, r0 + 32: a warp has rows 4 i .. 4 i + 3
+    const void *src = is_v ? p.v : p.k;
+    Eight<kType> x[kStoreSteps][2];
+#pragma unroll
+    for (int i = 0; i < kStoreSteps; i++) {
+        if (!b.has(r0 + 32 * i)) continue;
+        const size_t at = b.base + size_t(b.first + r0 + 32 * i) * kHeadDim + 16 * sub;
+        x[i][0].load(src, at);
+        x[i][1].load(src, at + 8);
+    }
+    unsigned char *block = block_of(p, b);
+    unsigned char *front = p.is_swa && !p.raw_slots && b.first < p.cache.first_tokens ? kv4_first_block(p.cache, b.seq, b.kvh) : nullptr;
+    // positions of one call that share a slot of a ring: only the last one of a slot is stored, whatever the order of CTAs
+    const int kept = p.is_swa && !p.raw_slots ? b.p1 - kSwaRing : INT_MIN;
+#pragma unroll
+    for (int i = 0; i < kStoreSteps; i++) {
+        const int r = r0 + 32 * i;
+        const bool in = b.has(r), pair = b.has(r & ~1) && b.has(r | 1);
+        if (!__any_sync(0xffffffffu, in)) continue;
+        uint32_t mine;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        const uint2 codes = kv4_quantise16(in ? x[i][0].get() : zero, in ? x[i][1].get() : zero, mine);
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 8);
+        auto put = [&](unsigned char *blk, bool both) {
+            *reinterpret_cast<uint2 *>(blk + (is_v ? kKv4VCodes : kKv4KCodes) + kv4_chunk(r, g) + (sub & 1) * 8) = codes;
+            if ((sub & 1) != 0) return;
+            if (is_v && both) {  // both rows of the pair: the even one's lanes write {d, d}, the odd one's {lo, lo}
+                const uint32_t w = (r & 1) ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
+                *reinterpret_cast<uint32_t *>(blk + kv4_v_group(r & ~1, g) + (r & 1) * 16) = w;
+            } else {
+                kv4_store_group(blk, r, g, is_v, mine);
+            }
+        };
+        if (in && b.first + r >= kept) put(block, pair && b.first + (r & ~1) >= kept);
+        if (in && front && b.first + r < p.cache.first_tokens) put(front, pair && b.first + (r | 1) < p.cache.first_tokens);
     }
 }
 
-__global__ void __launch_bounds__(256) k_kv_load(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs, int n) {
+template <int kType>
+__global__ void __launch_bounds__(kRowThreads) k_kv4_load(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs) {
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    const int lane = threadIdx.x & 31;
-    const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (w >= (long long)n * p.n_rows * kNHeadKv) return;
-    const int kvh = int(w % kNHeadKv), r = int(w / kNHeadKv % p.n_rows), i = int(w / kNHeadKv / p.n_rows);
-    const int seq = seqs.seq[i], pos = seqs.pos0[i] + r;
-    const bool first = p.is_swa && (p.raw_slots ? pos >= kSwaRing : pos < p.cache.first_tokens);
-    const size_t at = size_t(i) * p.seq_stride + size_t(kvh) * p.head_stride + size_t(r) * kHeadDim + 4 * lane;
-    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (p.cache.blocks) {
-        const unsigned char *block = first ? kv4_first_block(p.cache, seq, kvh) : kv4_block(p.cache, seq, kvh, pos >> 6);
-        row_store4(p.k, p.dtype, at, block ? kv4_load_lane(block, pos & 63, false, lane) : zero);
-        row_store4(p.v, p.dtype, at, block ? kv4_load_lane(block, pos & 63, true, lane) : zero);
-    } else {
-        const long long row = half_row(p, seq, kvh, pos);
-        row_store4(p.k, p.dtype, at, row < 0 ? zero : row_load4(p.k_cache, kDtypeF16, size_t(row) + 4 * lane));
-        row_store4(p.v, p.dtype, at, row < 0 ? zero : row_load4(p.v_cache, kDtypeF16, size_t(row) + 4 * lane));
+    const BlockRows b(p, seqs);
+    if (b.first >= b.p1) return;
+    const int sub = threadIdx.x & 15, r0 = threadIdx.x >> 4, g = sub >> 2;
+    const unsigned char *block = block_of(p, b);
+    const unsigned char *front = p.is_swa && !p.raw_slots && b.first < p.cache.first_tokens ? kv4_first_block(p.cache, b.seq, b.kvh) : nullptr;
+    uint32_t kc[kRowSteps], vc[kRowSteps], kg[kRowSteps];
+    uint16_t vd[kRowSteps], vl[kRowSteps];
+#pragma unroll
+    for (int i = 0; i < kRowSteps; i++) {
+        const int r = r0 + 16 * i;
+        kc[i] = vc[i] = kg[i] = 0;  // (rows on pages that the sequence does not hold read as zeros)
+        vd[i] = vl[i] = 0;
+        const unsigned char *blk = front && b.first + r < p.cache.first_tokens ? front : block;
+        if (!blk || !b.has(r)) continue;
+        kc[i] = __ldg(reinterpret_cast<const uint32_t *>(blk + kKv4KCodes + kv4_chunk(r, g) + (sub & 3) * 4));
+        kg[i] = __ldg(reinterpret_cast<const uint32_t *>(blk + kv4_k_group(r, g)));
+        vc[i] = __ldg(reinterpret_cast<const uint32_t *>(blk + kKv4VCodes + kv4_chunk(r, g) + (sub & 3) * 4));
+        vd[i] = __ldg(reinterpret_cast<const uint16_t *>(blk + kv4_v_group(r, g)));
+        vl[i] = __ldg(reinterpret_cast<const uint16_t *>(blk + kv4_v_group(r, g) + 16));
     }
+#pragma unroll
+    for (int i = 0; i < kRowSteps; i++) {
+        const int r = r0 + 16 * i;
+        if (!b.has(r)) continue;
+        const size_t at = b.base + size_t(b.first + r) * kHeadDim + 8 * sub;
+        float x[8];
+        const float2 dl = __half22float2(*reinterpret_cast<const __half2 *>(&kg[i]));
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = fmaf(float((kc[i] >> (4 * j)) & 15u), dl.x, dl.y);
+        Eight<kType>::store(p.k, at, x);
+        const float d = __half2float(__ushort_as_half(vd[i])), lo = __half2float(__ushort_as_half(vl[i]));
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = fmaf(float((vc[i] >> (4 * j)) & 15u), d, lo);
+        Eight<kType>::store(p.v, at, x);
+    }
+}
+
+dim3 block_grid(const KvRowsParams &p, int n, int parts) {  // a range that starts inside a block touches one more
+    return dim3(unsigned((p.n_rows + 2 * kKv4BlockKeys - 2) / kKv4BlockKeys), unsigned(kNHeadKv * parts), unsigned(n));
 }
 
 }  // namespace
 
 // The SM's memory is split as the decode kernel wants it: a kernel in between that wants another split makes the next one wait
 // for the SMs to be set up again.
+template <typename K>
+cudaError_t max_shared(K kernel) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+}
 cudaError_t kv_rows_setup() {
-    cudaError_t e = cudaFuncSetAttribute(k_kv_store, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_kv_load, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    cudaError_t e = max_shared(k_half_store);
+    if (e == cudaSuccess) e = max_shared(k_half_load);
+    if (e == cudaSuccess) e = max_shared(k_kv4_store<kDtypeF32>);
+    if (e == cudaSuccess) e = max_shared(k_kv4_store<kDtypeBf16>);
+    if (e == cudaSuccess) e = max_shared(k_kv4_store<kDtypeF16>);
+    if (e == cudaSuccess) e = max_shared(k_kv4_load<kDtypeF32>);
+    if (e == cudaSuccess) e = max_shared(k_kv4_load<kDtypeBf16>);
+    if (e == cudaSuccess) e = max_shared(k_kv4_load<kDtypeF16>);
     return e;
 }
 
 cudaError_t launch_kv_store(const KvRowsParams &p, const KvRowsSeqs &seqs, int n, cudaStream_t stream) {
-    const long long warps = (long long)n * p.n_rows * kNHeadKv;
-    if (warps <= 0) return cudaSuccess;
-    return launch_pdl(k_kv_store, int((warps + 7) / 8), 256, 0, stream, p, seqs, n);
+    if (n <= 0 || p.n_rows <= 0) return cudaSuccess;
+    if (!p.cache.blocks) return launch_pdl(k_half_store, dim3(unsigned(((long long)n * p.n_rows * kNHeadKv + 7) / 8)), 256, 0, stream, p, seqs, n);
+    const dim3 grid = block_grid(p, n, 2);
+    if (p.dtype == kDtypeF32) return launch_pdl(k_kv4_store<kDtypeF32>, grid, kRowThreads, 0, stream, p, seqs);
+    if (p.dtype == kDtypeBf16) return launch_pdl(k_kv4_store<kDtypeBf16>, grid, kRowThreads, 0, stream, p, seqs);
+    return launch_pdl(k_kv4_store<kDtypeF16>, grid, kRowThreads, 0, stream, p, seqs);
 }
 
 cudaError_t launch_kv_load(const KvRowsParams &p, const KvRowsSeqs &seqs, int n, cudaStream_t stream) {
-    const long long warps = (long long)n * p.n_rows * kNHeadKv;
-    if (warps <= 0) return cudaSuccess;
-    return launch_pdl(k_kv_load, int((warps + 7) / 8), 256, 0, stream, p, seqs, n);
+    if (n <= 0 || p.n_rows <= 0) return cudaSuccess;
+    if (!p.cache.blocks) return launch_pdl(k_half_load, dim3(unsigned(((long long)n * p.n_rows * kNHeadKv + 7) / 8)), 256, 0, stream, p, seqs, n);
+    const dim3 grid = block_grid(p, n, 1);
+    if (p.dtype == kDtypeF32) return launch_pdl(k_kv4_load<kDtypeF32>, grid, kRowThreads, 0, stream, p, seqs);
+    if (p.dtype == kDtypeBf16) return launch_pdl(k_kv4_load<kDtypeBf16>, grid, kRowThreads, 0, stream, p, seqs);
+    return launch_pdl(k_kv4_load<kDtypeF16>, grid, kRowThreads, 0, stream, p, seqs);
 }
 
 }  // namespace flint

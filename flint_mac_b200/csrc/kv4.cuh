@@ -24,63 +24,123 @@ __device__ __forceinline__ int kv4_chunk(int row, int ch) { return row * kKv4Row
 __device__ __forceinline__ int kv4_k_group(int row, int g) { return kKv4KGroups + row * 16 + g * 4; }
 __device__ __forceinline__ int kv4_v_group(int row, int g) { return kKv4VGroups + (row >> 1) * 32 + g * 4 + (row & 1) * 2; }
 
-// Quantises one group held by eight neighbouring lanes, four values a lane (in order; already values of type half).
-// Returns the lane's four codes, first one lowest; `dl` gets {d, lo}.  Whole warps call this.
-__device__ __forceinline__ uint32_t kv4_quantise4(const float (&x)[4], __half2 &dl) {
-    float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-    const bool fine = fabsf(x[0]) <= 65504.f && fabsf(x[1]) <= 65504.f && fabsf(x[2]) <= 65504.f && fabsf(x[3]) <= 65504.f;
+// d and lo of a group, packed {d, lo}, and 1 / d, from its least and largest value (halves; NaN if a value was one).  A group
+// that holds an infinity or a NaN gets d = NaN.  The quotient by 15, like those by d below, is the product with the
+// reciprocal and one correction step, which rounds it as a division does (Markstein 1990).
+struct Kv4Scale {
+    uint32_t dl;
+    float d, lo, inv;
+};
+__device__ __forceinline__ Kv4Scale kv4_scale(__half least, __half largest) {
+    Kv4Scale s;
+    s.lo = __half2float(least);
+    const float hi = __half2float(largest);
+    if (!(fabsf(s.lo) <= 65504.f && fabsf(hi) <= 65504.f)) {
+        s.dl = 0x00007fffu;
+        s.d = s.inv = s.lo = 0.f;
+        return s;
+    }
+    constexpr float k15 = 1.0f / 15.0f;
+    const float range = hi - s.lo;
+    float q = range * k15;
+    q = fmaf(fmaf(-q, 15.f, range), k15, q);
+    const __half2 dl = __halves2half2(__float2half_rn(q), least);
+    s.dl = *reinterpret_cast<const uint32_t *>(&dl);
+    s.d = __low2float(dl);
+    s.inv = s.d > 0.f ? __frcp_rn(s.d) : 0.f;
+    return s;
+}
+// Two floats at a time
+__device__ __forceinline__ uint64_t kv4_pack(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t kv4_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t kv4_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t kv4_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// Codes of four values, in the low 16 bits, first one lowest.  Adding 1.5 * 2^23 rounds a quotient to the nearest whole
+// number, ties to even, and leaves that in the low bits of the sum, whose next bits are zeros.  (d = 0: the codes are 0.)
+__device__ __forceinline__ uint32_t kv4_codes4(float2 x01, float2 x23, const Kv4Scale &s) {
+    const uint64_t lo2 = kv4_pack(-s.lo, -s.lo), inv2 = kv4_pack(s.inv, s.inv), nd2 = kv4_pack(-s.d, -s.d), magic = kv4_pack(12582912.f, 12582912.f);
+    const uint64_t a = kv4_add(kv4_pack(x01.x, x01.y), lo2), b = kv4_add(kv4_pack(x23.x, x23.y), lo2);
+    uint64_t q = kv4_mul(a, inv2), r = kv4_mul(b, inv2);
+    q = kv4_fma(kv4_fma(q, nd2, a), inv2, q);
+    r = kv4_fma(kv4_fma(r, nd2, b), inv2, r);
+    if (s.d < 6.103515625e-5f) {  // a subnormal d may lie well below (max - lo) / 15: limit to 15 (else 15.01 is the most)
+        float q0, q1, r0, r1;
+        asm("mov.b64 {%0, %1}, %2;\n" : "=f"(q0), "=f"(q1) : "l"(q));
+        asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r0), "=f"(r1) : "l"(r));
+        q = kv4_pack(fminf(q0, 15.f), fminf(q1, 15.f));
+        r = kv4_pack(fminf(r0, 15.f), fminf(r1, 15.f));
+    }
+    q = kv4_add(q, magic);
+    r = kv4_add(r, magic);
+    return (uint32_t(q) + (uint32_t(q >> 32) << 4) + (uint32_t(r) << 8) + (uint32_t(r >> 32) << 12)) & 0xffffu;
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2 *>(&w); }
+__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<const uint32_t *>(&h); }
+
+// Quantises a group held by eight neighbouring lanes, four half-precision values a lane, in order.  Returns the lane's four
+// codes; `dl` gets {d, lo}.  Whole warps call this.
+__device__ __forceinline__ uint32_t kv4_quantise4(uint2 h, uint32_t &dl) {
+    __half2 lo = __hmin2_nan(as_half2(h.x), as_half2(h.y)), hi = __hmax2_nan(as_half2(h.x), as_half2(h.y));
 #pragma unroll
     for (int off = 1; off < 8; off <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+        lo = __hmin2_nan(lo, as_half2(__shfl_xor_sync(0xffffffffu, as_u32(lo), off)));
+        hi = __hmax2_nan(hi, as_half2(__shfl_xor_sync(0xffffffffu, as_u32(hi), off)));
     }
-    const uint32_t group = 0xffu << (threadIdx.x & 24);
-    if ((__ballot_sync(0xffffffffu, fine) & group) != group) {
-        dl = __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0));
-        return 0;
-    }
-    const __half dh = __float2half_rn((hi - lo) / 15.0f);
-    const float d = __half2float(dh);
-    dl = __halves2half2(dh, __float2half_rn(lo));  // (exact: lo is one of the halves)
-    uint32_t codes = 0;
-    if (d > 0.f) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) codes |= uint32_t(fminf(rintf((x[i] - lo) / d), 15.f)) << (4 * i);
-    }
-    return codes;
+    const Kv4Scale s = kv4_scale(__hmin_nan(__low2half(lo), __high2half(lo)), __hmax_nan(__low2half(hi), __high2half(hi)));
+    dl = s.dl;
+    const float2 a = __half22float2(as_half2(h.x)), b = __half22float2(as_half2(h.y));
+    return s.inv == 0.f ? 0u : kv4_codes4(a, b, s);
+}
+// The same for two neighbouring lanes with sixteen values each.
+__device__ __forceinline__ uint2 kv4_quantise16(uint4 h, uint4 k, uint32_t &dl) {
+    auto least = [](uint4 w) { return __hmin2_nan(__hmin2_nan(as_half2(w.x), as_half2(w.y)), __hmin2_nan(as_half2(w.z), as_half2(w.w))); };
+    auto largest = [](uint4 w) { return __hmax2_nan(__hmax2_nan(as_half2(w.x), as_half2(w.y)), __hmax2_nan(as_half2(w.z), as_half2(w.w))); };
+    __half2 lo = __hmin2_nan(least(h), least(k)), hi = __hmax2_nan(largest(h), largest(k));
+    lo = __hmin2_nan(lo, as_half2(__shfl_xor_sync(0xffffffffu, as_u32(lo), 1)));
+    hi = __hmax2_nan(hi, as_half2(__shfl_xor_sync(0xffffffffu, as_u32(hi), 1)));
+    const Kv4Scale s = kv4_scale(__hmin_nan(__low2half(lo), __high2half(lo)), __hmax_nan(__low2half(hi), __high2half(hi)));
+    dl = s.dl;
+    if (s.inv == 0.f) return make_uint2(0, 0);
+    auto eight = [&](uint4 w) {
+        return kv4_codes4(__half22float2(as_half2(w.x)), __half22float2(as_half2(w.y)), s) |
+               kv4_codes4(__half22float2(as_half2(w.z)), __half22float2(as_half2(w.w)), s) << 16;
+    };
+    return make_uint2(eight(h), eight(k));
 }
 
-// Writes a lane's share (dims 4 * lane .. + 3) of a quantised K or V row.  Whole warps call this.
-__device__ __forceinline__ void kv4_store_lane(unsigned char *block, int row, bool is_v, int lane, const float (&x)[4]) {
-    __half2 dl;
-    const uint32_t codes = kv4_quantise4(x, dl);
+// Writes {d, lo} of a group of one row.
+__device__ __forceinline__ void kv4_store_group(unsigned char *block, int row, int g, bool is_v, uint32_t dl) {
+    if (is_v) {
+        *reinterpret_cast<uint16_t *>(block + kv4_v_group(row, g)) = uint16_t(dl);
+        *reinterpret_cast<uint16_t *>(block + kv4_v_group(row, g) + 16) = uint16_t(dl >> 16);
+    } else {
+        *reinterpret_cast<uint32_t *>(block + kv4_k_group(row, g)) = dl;
+    }
+}
+
+// Writes a lane's share (dims 4 * lane .. + 3) of a K or V row, quantised.  Whole warps call this.
+__device__ __forceinline__ void kv4_store_lane(unsigned char *block, int row, bool is_v, int lane, uint2 h) {
+    uint32_t dl;
+    const uint32_t codes = kv4_quantise4(h, dl);
     const int g = lane >> 3;
     *reinterpret_cast<uint16_t *>(block + (is_v ? kKv4VCodes : kKv4KCodes) + kv4_chunk(row, g) + (lane & 7) * 2) = uint16_t(codes);
-    if ((lane & 7) == 0) {
-        if (is_v) {
-            *reinterpret_cast<__half *>(block + kv4_v_group(row, g)) = __low2half(dl);
-            *reinterpret_cast<__half *>(block + kv4_v_group(row, g) + 16) = __high2half(dl);
-        } else {
-            *reinterpret_cast<__half2 *>(block + kv4_k_group(row, g)) = dl;
-        }
-    }
-}
-
-// A lane's share (dims 4 * lane .. + 3) of a row, as values.
-__device__ __forceinline__ float4 kv4_load_lane(const unsigned char *block, int row, bool is_v, int lane) {
-    const int g = lane >> 3;
-    const uint32_t c = *reinterpret_cast<const uint16_t *>(block + (is_v ? kKv4VCodes : kKv4KCodes) + kv4_chunk(row, g) + (lane & 7) * 2);
-    float d, lo;
-    if (is_v) {
-        d = __half2float(*reinterpret_cast<const __half *>(block + kv4_v_group(row, g)));
-        lo = __half2float(*reinterpret_cast<const __half *>(block + kv4_v_group(row, g) + 16));
-    } else {
-        const float2 dl = __half22float2(*reinterpret_cast<const __half2 *>(block + kv4_k_group(row, g)));
-        d = dl.x;
-        lo = dl.y;
-    }
-    return make_float4(fmaf(float(c & 15), d, lo), fmaf(float((c >> 4) & 15), d, lo), fmaf(float((c >> 8) & 15), d, lo),
-                       fmaf(float(c >> 12), d, lo));
+    if ((lane & 7) == 0) kv4_store_group(block, row, g, is_v, dl);
 }
 
 }  // namespace flint

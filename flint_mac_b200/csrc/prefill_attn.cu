@@ -228,21 +228,12 @@ __device__ __forceinline__ void store_row_kv4(const PrologueArgs &a, const float
     unsigned char *block = kv4_block(a.kv4, a.seq, kvh, pos >> 6);
 #pragma unroll
     for (int hi = 0; hi < 2; hi++) {
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = __half2float(__float2half_rn(x[4 * hi + j]));
-        __half2 dl;
-        const uint32_t codes = kv4_quantise4(v, dl);
+        uint32_t dl;
+        const uint32_t codes = kv4_quantise4(make_uint2(pack_half2(x[4 * hi], x[4 * hi + 1]), pack_half2(x[4 * hi + 2], x[4 * hi + 3])), dl);
         const int g = (sub >> 3) + 2 * hi;
         auto put = [&](unsigned char *blk, int row) {
             *reinterpret_cast<uint16_t *>(blk + (is_v ? kKv4VCodes : kKv4KCodes) + kv4_chunk(row, g) + (sub & 7) * 2) = uint16_t(codes);
-            if ((sub & 7) != 0) return;
-            if (is_v) {
-                *reinterpret_cast<__half *>(blk + kv4_v_group(row, g)) = __low2half(dl);
-                *reinterpret_cast<__half *>(blk + kv4_v_group(row, g) + 16) = __high2half(dl);
-            } else {
-                *reinterpret_cast<__half2 *>(blk + kv4_k_group(row, g)) = dl;
-            }
+            if ((sub & 7) == 0) kv4_store_group(blk, row, g, is_v, dl);
         };
         if (to_cache) put(block, pos & 63);
         if (to_first) put(kv4_first_block(a.kv4, a.seq, kvh), pos);
