@@ -46,8 +46,8 @@ __device__ __forceinline__ long long half_row(const KvRowsParams &p, int seq, in
 
 // ---- half-precision caches: one warp per (sequence, row, KV head)
 __global__ void __launch_bounds__(256) k_half_store(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs, int n) {
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // (after the wait: see the prefill prologue)
     const int lane = threadIdx.x & 31;
     const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (w >= (long long)n * p.n_rows * kNHeadKv) return;
@@ -62,8 +62,8 @@ __global__ void __launch_bounds__(256) k_half_store(const KvRowsParams p, const 
 }
 
 __global__ void __launch_bounds__(256) k_half_load(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs, int n) {
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // (after the wait: see the prefill prologue)
     const int lane = threadIdx.x & 31;
     const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (w >= (long long)n * p.n_rows * kNHeadKv) return;
@@ -162,8 +162,8 @@ __device__ __forceinline__ unsigned char *block_of(const KvRowsParams &p, const 
 constexpr int kStoreSteps = kKv4BlockKeys * 8 / kRowThreads;
 template <int kType>
 __global__ void __launch_bounds__(kRowThreads, 6) k_kv4_store(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs) {
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // (after the wait: see the prefill prologue)
     const bool is_v = blockIdx.y >= kNHeadKv;
     const BlockRows b(p, seqs);
     if (b.first >= b.p1) return;
@@ -207,8 +207,8 @@ __global__ void __launch_bounds__(kRowThreads, 6) k_kv4_store(const KvRowsParams
 
 template <int kType>
 __global__ void __launch_bounds__(kRowThreads) k_kv4_load(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs) {
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // (after the wait: see the prefill prologue)
     const BlockRows b(p, seqs);
     if (b.first >= b.p1) return;
     const int sub = threadIdx.x & 15, r0 = threadIdx.x >> 4, g = sub >> 2;

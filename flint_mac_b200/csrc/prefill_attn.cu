@@ -25,6 +25,7 @@
 #include <utility>
 #include <vector>
 
+#include "decode_common.cuh"
 #include "kv4.cuh"
 #include "ptx.cuh"
 #include "tc5.cuh"
@@ -33,7 +34,6 @@ namespace flint {
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kQPos = 16;              // query positions per 128-row Q tile (x 8 heads of the GQA group)
 constexpr int kBM = kQPos * kGqa;      // 128 query rows per Q tile
 constexpr int kQTiles = 2;             // Q tiles per CTA: they share every K/V tile and take turns on the tensor core
@@ -87,8 +87,9 @@ struct PfArgs {
     int kr_lo, kr_hi, with_sink, cp_partial;
     // Sliding-window layer with first tokens that stay visible: rows [0, first_rows) of the K/V staging hold positions
     // [0, first_tokens), the window's rows follow.
-    int first_tokens, first_rows;
+    int first_tokens, first_rows;  // (first_rows: 64)
 };
+static_assert(kMaxFirstTokens == 64, "half a key tile");
 
 // What a query sees, beyond the causal limit; the attention kernel is compiled for each.
 enum { kFull = 0, kWindow = 1, kWindowFirst = 2 };
@@ -277,8 +278,8 @@ __device__ __forceinline__ void prologue_rows(const PrologueArgs &a) {
     // On a ring layer tokens t and t + 1024 of one launch share a slot: only the last token that maps to a slot
     // stores there, so the ring's final contents do not depend on the order in which the CTAs run.
     const bool to_cache = mine && (!a.is_swa || t + kSwaRing >= a.n_tok);
-    if (kKv4 && a.first_rows > 0 && t == 0) {  // the product takes the first tokens' rows 16 at a time: those past them count as 0
-        const int from = a.kv4.first_tokens, to = (from + 15) & ~15;
+    if (kKv4 && a.first_rows > 0 && t == 0) {  // the products take 64 rows of first tokens: those past the last one count as 0
+        const int from = a.kv4.first_tokens, to = kMaxFirstTokens;
         for (int i = threadIdx.x; i < (to - from) * kNHeadKv * (kHeadDim / 8); i += 128) {
             const int c = i % (kHeadDim / 8), r = from + i / (kHeadDim / 8) / kNHeadKv, kvh = i / (kHeadDim / 8) % kNHeadKv;
             const size_t off = (size_t(kvh) * a.st_rows + r) * kHeadDim + 8 * c;
@@ -359,7 +360,12 @@ __global__ void __launch_bounds__(128, kBf16 ? 8 : 5) k_prefill_prologue(const P
     // the attention kernel of this prefill may be scheduled as soon as SMs come free: it waits for this grid's
     // completion (griddepcontrol.wait) before it reads anything written here
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    // With a 4-bit cache the kernel in front brings earlier tokens into the staging, and this one may have been scheduled
+    // while that still runs (which began only when everything before it had ended).  On a ring layer it reads the slots that
+    // are written here; on a full layer the two touch different rows, so they run side by side, and this one ends last.
+    if (kKv4 && a.is_swa) asm volatile("griddepcontrol.wait;\n" ::: "memory");
     prologue_rows<kBf16, kKv4>(a);
+    if (kKv4 && !a.is_swa) asm volatile("griddepcontrol.wait;\n" ::: "memory");
 }
 
 // ------------------------------------------------------------------------------------------------- attention
@@ -401,7 +407,7 @@ enum {
 // key range is split, one range of its key tiles.
 struct Unit {
     int t0, kvh, q_first, q_last, klo, n_keys, n_tiles, split;
-    int first;  // 1: tile 0 holds the first tokens, the window's tiles follow
+    int first;  // 1: the first 64 keys of tile 0 are the first tokens' rows, the window follows; klo and n_keys count them in
 };
 // Units are handed out longest first: late query blocks (full 544-key bands) before the first 16 blocks of the
 // prompt, whose bands are shorter, so that the CTAs that get one unit more than the others get short ones.
@@ -420,6 +426,11 @@ __host__ __device__ inline Unit unit_geom_of(int u, int n_tok, int p0, int is_sw
     const int lo_swa = g.q_first - kHist > key_row0 ? g.q_first - kHist : key_row0;
     g.klo = is_swa ? lo_swa : (kr_lo > 0 ? kr_lo : 0);
     g.n_keys = (is_swa || g.q_last < kr_hi ? g.q_last + 1 : kr_hi) - g.klo;  // <= 0: the unit has no key on this device
+    // A query at q sees the first tokens below q - 512 through rows of their own, those from there on through its window.
+    // The window's 544 keys leave three quarters of the fifth tile empty: 64 rows more are no tile more.
+    g.first = first_tokens > 0 && g.q_last > kHist ? 1 : 0;
+    g.klo -= g.first * kMaxFirstTokens;
+    g.n_keys += g.first * kMaxFirstTokens;
     g.n_tiles = (g.n_keys + kBN - 1) / kBN;
     if (n_ksplit > 1) {  // the host guarantees at least 4 tiles per range; the last range takes the remainder
         const int per = g.n_tiles / n_ksplit;
@@ -429,9 +440,6 @@ __host__ __device__ inline Unit unit_geom_of(int u, int n_tok, int p0, int is_sw
         g.n_keys = left < (kt_b - kt_a) * kBN ? left : (kt_b - kt_a) * kBN;
         g.n_tiles = kt_b - kt_a;
     }
-    // a query at q sees the first tokens below q - 512 through the extra tile, those from there on through its window
-    g.first = first_tokens > 0 && g.q_last > kHist ? 1 : 0;
-    g.n_tiles += g.first;
     return g;
 }
 template <int kKind>
@@ -534,9 +542,17 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
                 g++;
                 if (use >= 1 && !wait_bar(bar(kBarSlotEmpty + slot), (use - 1) & 1)) return false;
                 const uint32_t dst = base + kOffKV + slot * kTileBytes, full = bar(kBarSlotFull + slot);
-                int row = un.klo + kt * kBN - a.key_row0;
-                if (kKind == kWindowFirst) row = kt < un.first ? 0 : row + a.first_rows - un.first * kBN;
+                const int row = un.klo + kt * kBN - a.key_row0;
                 tc5::mbar_expect_tx(full, kTileBytes);
+                if (kKind == kWindowFirst) {  // two 64-row boxes: the first one of a unit may be the first tokens' rows
+                    for (int rh = 0; rh < 2; rh++) {
+                        const int y = un.first && kt == 0 && rh == 0 ? 0 : row + rh * 64 + a.first_rows;
+                        const uint32_t d = dst + rh * (kTileBytes / 4);
+                        tc5::tma_load_3d(d, map, full, 0, y, un.kvh);
+                        tc5::tma_load_3d(d + kTileBytes / 2, map, full, 64, y, un.kvh);
+                    }
+                    return true;
+                }
                 if (a.block_table) {
                     // a 128-key tile is two pages; a page past the sequence's last one holds only keys that every
                     // query of the unit has masked, so any resident page stands in for it
@@ -599,13 +615,7 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
             Unit un;
         };
         // keys of a tile that any query of the unit can see, rounded up to the MMA's N granularity
-        auto tile_n = [&](const Cursor &c) {
-            if (kKind == kWindowFirst) {
-                if (c.kt < c.un.first) return (a.first_tokens + 15) & ~15;
-                return min(kBN, (c.un.n_keys - (c.kt - c.un.first) * kBN + 15) & ~15);
-            }
-            return min(kBN, (c.un.n_keys - c.kt * kBN + 15) & ~15);
-        };
+        auto tile_n = [&](const Cursor &c) { return min(kBN, (c.un.n_keys - c.kt * kBN + 15) & ~15); };
         auto advance = [&](Cursor &c) {  // returns false at the end of the stream
             if (c.kt + 1 < c.un.n_tiles) {
                 c.kt++;
@@ -699,23 +709,21 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
             ok = __all_sync(0xffffffffu, wait_bar(bar(kBarSReady + w), j & 1));  // warp-uniform for tcgen05.ld
             if (!ok) break;
             tc5::fence_after_sync();
-            const bool first_tile = kKind == kWindowFirst && kt < un.first;
-            const int kw = kKind == kWindowFirst ? kt - un.first : kt;  // tile of the window
-            const int kbase = first_tile ? 0 : klo + kw * kBN;
-            // columns the MMA wrote (same as the issuer)
-            const int n_cols = first_tile ? (a.first_tokens + 15) & ~15 : min(kBN, (n_keys - kw * kBN + 15) & ~15);
+            const bool first_tile = kKind == kWindowFirst && un.first && kt == 0;
+            const int kbase = klo + kt * kBN;
+            const int n_cols = min(kBN, (n_keys - kt * kBN + 15) & ~15);  // columns the MMA wrote (same as the issuer)
             const int n_chunks = (n_cols + 31) >> 5;
             // visible columns of this row form one range [c_lo, c_hi] (prefill.metal:212); on a key-range shard the
             // unit's keys also end with the shard (k_end), before the causal limit of later queries
             const int k_end = klo + n_keys - 1;
-            // (in the tile of the first tokens: those in front of the row's window, which may be none)
-            const int n_front = min(a.first_tokens, qpos - kHist);
-            const int c_hi = first_tile ? (n_front > 0 ? n_front - 1 : 1 << 20) : min(qpos, k_end) - kbase;
-            const int c_lo = first_tile ? (n_front > 0 ? 0 : 1 << 20) : kSwa ? qpos - kHist - kbase : -(1 << 30);
+            const int c_hi = min(qpos, k_end) - kbase;
+            const int c_lo = kKind == kWindowFirst ? max(qpos - kHist, klo + un.first * kMaxFirstTokens) - kbase
+                                                   : kSwa ? qpos - kHist - kbase : -(1 << 30);
+            const int n_front = min(a.first_tokens, qpos - kHist);  // of the first tokens' rows: those in front of the row's window
             // Per 32-column chunk, for the whole Q tile: 0 = every row sees every key (no per-element mask),
             // 1 = mixed, 2 = no row sees any key.  Only the two ends of the band are mixed.
             auto chunk_kind = [&](int ch) {
-                if (first_tile) return 1;
+                if (first_tile && ch < kMaxFirstTokens / 32) return 1;
                 const int key_lo = kbase + ch * 32, key_hi = key_lo + 31;
                 if (key_lo > qt_last || key_lo > k_end || (kSwa && key_hi < qt_first - kHist)) return 2;
                 if (key_hi <= qt_first && key_hi <= k_end && (!kSwa || key_lo >= qt_last - kHist)) return 0;
@@ -732,11 +740,15 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
             tc5::mbar_arrive(bar(kBarSFree + w));  // S is in registers: the next scores may overwrite it
             // Band-edge tiles (the first and the last of a unit): invisible scores become -inf, per 32-column chunk and
             // only in chunks that some row of the Q tile sees partly; interior tiles skip all of it on uniform branches.
-            if (chunk_kind(0) != 0 || chunk_kind(n_chunks - 1) != 0) {
+            if (chunk_kind(0) != 0 || chunk_kind(n_chunks - 1) != 0) {  // (the tile with the first tokens' rows is one of them)
                 const uint32_t span = uint32_t(c_hi - c_lo);
 #pragma unroll
                 for (int ch = 0; ch < kBN / 32; ch++) {
-                    if (ch < n_chunks && chunk_kind(ch) != 0) {
+                    if (kKind == kWindowFirst && first_tile && ch < kMaxFirstTokens / 32) {
+#pragma unroll
+                        for (int c = 0; c < 32; c++)
+                            if (ch * 32 + c >= n_front) sr[ch * 32 + c] = 0xff800000u;
+                    } else if (ch < n_chunks && chunk_kind(ch) != 0) {
 #pragma unroll
                         for (int c = 0; c < 32; c++)  // visible iff c_lo <= col <= c_hi
                             if (uint32_t(ch * 32 + c - c_lo) > span) sr[ch * 32 + c] = 0xff800000u;
@@ -1173,7 +1185,12 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
             (*n_launches)++;
         }
         const bool bf16 = pa.qkv_dtype == kDtypeBf16;
-        if (kv4 && bf16) k_prefill_prologue<true, true><<<unsigned(T), 128, 0, stream>>>(pa);
+        if (kv4 && p.p0 > 0) {
+            if (cudaError_t le = bf16 ? launch_pdl(k_prefill_prologue<true, true>, dim3(unsigned(T)), 128, 0, stream, pa)
+                                      : launch_pdl(k_prefill_prologue<false, true>, dim3(unsigned(T)), 128, 0, stream, pa);
+                le != cudaSuccess)
+                return le;
+        } else if (kv4 && bf16) k_prefill_prologue<true, true><<<unsigned(T), 128, 0, stream>>>(pa);
         else if (kv4) k_prefill_prologue<false, true><<<unsigned(T), 128, 0, stream>>>(pa);
         else if (bf16) k_prefill_prologue<true, false><<<unsigned(T), 128, 0, stream>>>(pa);
         else k_prefill_prologue<false, false><<<unsigned(T), 128, 0, stream>>>(pa);
@@ -1199,8 +1216,9 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
         if ((e = make_map(&tm_k, kb, 64, p.n_pages * kNHeadKv, 64, 1)) != cudaSuccess) return e;
         if ((e = make_map(&tm_v, vb, 64, p.n_pages * kNHeadKv, 64, 1)) != cudaSuccess) return e;
     } else {
-        if ((e = make_map(&tm_k, kb, kv_rows, kNHeadKv, kBN, 1)) != cudaSuccess) return e;
-        if ((e = make_map(&tm_v, vb, kv_rows, kNHeadKv, kBN, 1)) != cudaSuccess) return e;
+        const int box = first_tokens > 0 ? kMaxFirstTokens : kBN;
+        if ((e = make_map(&tm_k, kb, kv_rows, kNHeadKv, box, 1)) != cudaSuccess) return e;
+        if ((e = make_map(&tm_v, vb, kv_rows, kNHeadKv, box, 1)) != cudaSuccess) return e;
     }
 
     PfArgs a{};
