@@ -50,10 +50,6 @@ struct __align__(128) Dec4Smem {
     alignas(16) __half vnew[2][kHeadDim];  // (the present piece's is read while the next one's is written)
     alignas(16) float rope_cos[kHeadDim / 2], rope_sin[kHeadDim / 2];
     alignas(16) float q_norm[kHeadDim], k_norm[kHeadDim], sinks[kNHead];
-    struct {  // a piece whose record is written: where it belongs, and whether it was the last of its run to arrive
-        int rec0, split, n_split, kvh, row, last;
-    } done[2];
-    int last2;
 };
 static_assert(sizeof(Dec4Smem<4>) * 4 <= 223 * 1024 && sizeof(Dec4Smem<8>) * 2 <= 225 * 1024, "CTAs of an SM");
 
@@ -132,13 +128,13 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
 }
 
 // Folds n partial records of one head into (M, L, a): the lane's four dims d0 .. d0 + 3.  Record i lies at rec(i).
-// Ten records a trip, their loads in flight together.
+// kDec4MergeTrip records a trip, their loads in flight together.
 struct Merged4 {
     float M, L, a[4];
 };
 template <typename Rec>
 __device__ __forceinline__ Merged4 merge_records4(Rec rec, int n, int d0) {
-    constexpr int kTrip = 10;
+    constexpr int kTrip = kDec4MergeTrip;
     Merged4 r;
     r.M = -INFINITY;
     r.L = r.a[0] = r.a[1] = r.a[2] = r.a[3] = 0.f;
@@ -215,10 +211,14 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
     constexpr int kThreads = kWarps * 32, kHeads = kGqa / kWarps;  // kHeads: query heads of the group that a warp looks after
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t4 = lane & 3, d0 = 4 * lane;
+    // Which warps do what beside: the last two have the new token's k and v (their tiles come last, if they have any), two
+    // others the rotation table.
+    const int nw = warp - (kWarps - 2), rope_at = tid - (kWarps / 2 - 2) * 32;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const bool rope = p.has_rope != 0;
     float freq = 0.f;
-    if (rope && tid < kHeadDim / 2) freq = p.inv_freq[tid];
+    const bool rope_warp = rope && rope_at >= 0 && rope_at < kHeadDim / 2;
+    if (rope_warp) freq = p.inv_freq[rope_at];
     // the layer's constants: read from shared memory at every piece (a load past a busy memory system takes microseconds)
     for (int i = tid; i < kHeadDim; i += kThreads) {
         sm.q_norm[i] = p.q_norm[i];
@@ -265,7 +265,7 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
         mbar_expect_tx(bar, kHalf);
         bulk_load(is_v ? v_tile : k_tile, block + is_v * kHalf, kHalf, bar);
     };
-    // Raw rows: its heads of the group by each warp, the new k and v by warps 0 and 1 too.  A warp reads what it fetched.
+    // Raw rows: its heads of the group by each warp, the new k and v by the last two warps too.  A warp reads what it fetched.
     auto fetch_rows = [&](int index) {
         const Dec4Piece &w = pieces[index >> 2];
         const int head0 = (index & 3) * kGqa, tok = p.tok0 + w.tok;
@@ -278,15 +278,15 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
         };
 #pragma unroll
         for (int i = 0; i < kHeads; i++) fetch((head0 + warp * kHeads + i) * kHeadDim, warp * kHeads + i);
-        if (w.split == w.n_split - 1 && warp < 2) fetch(kQDim + warp * kKvDim + (index & 3) * kHeadDim, kGqa + warp);
+        if (w.split == w.n_split - 1 && nw >= 0) fetch(kQDim + nw * kKvDim + (index & 3) * kHeadDim, kGqa + nw);
         cp_async_commit();
     };
     auto rope_table = [&](int index) {
-        if (!rope || tid >= kHeadDim / 2) return;
+        if (!rope_warp) return;
         float sn, cs;
         sincos_reduced(float(pieces[index >> 2].pos) * freq, &sn, &cs);
-        sm.rope_cos[tid] = cs;
-        sm.rope_sin[tid] = sn;
+        sm.rope_cos[rope_at] = cs;
+        sm.rope_sin[rope_at] = sn;
     };
     int flip = 0;
     auto finish_rows = [&] {  // raw rows (and the rotation table, visible already) -> sm.q, the new token's rows, the cache
@@ -305,57 +305,65 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
             x.x *= qscale; x.y *= qscale; x.z *= qscale; x.w *= qscale;
             store_half4(&sm.q[h][d0], x);
         }
-        if (ends && warp < 2) {
-            float4 x = load_row4(&sm.raw[kGqa + warp][0], p.qkv_dtype, 0, lane);
-            if (warp == 0) x = norm_rope(x, reinterpret_cast<const float4 *>(sm.k_norm)[lane], cs, sn, lane, rope);
+        if (ends && nw >= 0) {
+            float4 x = load_row4(&sm.raw[kGqa + nw][0], p.qkv_dtype, 0, lane);
+            if (nw == 0) x = norm_rope(x, reinterpret_cast<const float4 *>(sm.k_norm)[lane], cs, sn, lane, rope);
             const uint2 h = make_uint2(pack_half2(x.x, x.y), pack_half2(x.z, x.w));
-            *reinterpret_cast<uint2 *>(warp == 0 ? &sm.knew[d0] : &sm.vnew[flip][d0]) = h;
+            *reinterpret_cast<uint2 *>(nw == 0 ? &sm.knew[d0] : &sm.vnew[flip][d0]) = h;
         }
     };
-    auto store_new = [&] {  // the new token's rows -> the cache (warps 0 and 1)
-        if (!ends || warp >= 2) return;
-        const uint2 h = *reinterpret_cast<const uint2 *>(warp == 0 ? &sm.knew[d0] : &sm.vnew[flip][d0]);
-        kv4_store_lane(kv4_block(p.cache, pc.seq, kvh, pc.pos >> 6), pc.pos & 63, warp == 1, lane, h);
+    auto store_new = [&] {  // the new token's rows -> the cache
+        if (!ends || nw < 0) return;
+        const uint2 h = *reinterpret_cast<const uint2 *>(nw == 0 ? &sm.knew[d0] : &sm.vnew[flip][d0]);
+        kv4_store_lane(kv4_block(p.cache, pc.seq, kvh, pc.pos >> 6), pc.pos & 63, nw == 1, lane, h);
         if (p.is_swa && pc.pos < p.cache.first_tokens)
-            kv4_store_lane(kv4_first_block(p.cache, pc.seq, kvh), pc.pos, warp == 1, lane, h);
+            kv4_store_lane(kv4_first_block(p.cache, pc.seq, kvh), pc.pos, nw == 1, lane, h);
     };
-    // Split-K: merges the run of records that piece `w` was the last of to arrive, and if that was the group's last run, the
-    // runs (the whole CTA calls this).
-    auto merge_run = [&](int w) {
-        const auto &f = sm.done[w];
-        const int rec0 = f.rec0, fan = dec4_fan(f.n_split), sub = f.split / fan, n_sub = (f.n_split + fan - 1) / fan;
-        auto record = [&](float *base, int i, int h) { return base + (size_t(rec0 + i * kNHeadKv) * kGqa + h) * kRecStride; };
-        const int h0 = warp * kHeads, n = min(fan, f.n_split - sub * fan);
-        auto finish = [&](const Merged4 &r, int h) {
-            const int head = f.kvh * kGqa + h;
+    // Split-K, per query head: a warp that has written its record of a head counts it; the one that finds itself the last of
+    // its run of records merges the run, and if that was the last run of the head, the runs.  (The record's stores are ordered
+    // before lane 0's ticket by the warp's barrier; the ticket is an acquire-release atomic at device scope, cumulative over
+    // them; the readers go past L1.)  The first ticket's answer is looked at after the next piece, if there is one: no piece
+    // waits for the round trip.
+    struct Out {
+        int rec0, split, n_split, kvh, row;
+    } out = {};
+    int arrived[kHeads];
+    auto count_record = [&] {
+        const int fan = dec4_fan(out.n_split);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kHeads; i++)
+            if (lane == 0) arrived[i] = ticket_acq_rel(&p.tickets[(out.rec0 + out.split / fan * kNHeadKv) * kGqa + warp * kHeads + i]);
+    };
+    auto merge_runs = [&] {
+        const int fan = dec4_fan(out.n_split), sub = out.split / fan, n_sub = (out.n_split + fan - 1) / fan;
+        const int n = min(fan, out.n_split - sub * fan);
+#pragma unroll
+        for (int i = 0; i < kHeads; i++) {
+            const int h = warp * kHeads + i, head = out.kvh * kGqa + h;
+            auto record = [&](float *base, int k) { return base + (size_t(out.rec0 + k * kNHeadKv) * kGqa + h) * kRecStride; };
+            if (__shfl_sync(0xffffffffu, arrived[i], 0) != n - 1) continue;
+            if (lane == 0) p.tickets[(out.rec0 + sub * kNHeadKv) * kGqa + h] = 0;  // ready for the next launch
+            Merged4 r = merge_records4([&](int k) { return record(p.scratch, sub * fan + k); }, n, d0);
+            if (n_sub > 1) {
+                float *rec = record(p.scratch2, sub);
+                *reinterpret_cast<float4 *>(rec + d0) = make_float4(r.a[0], r.a[1], r.a[2], r.a[3]);
+                if (lane == 0) *reinterpret_cast<float2 *>(rec + kHeadDim) = make_float2(r.M, r.L);
+                __syncwarp();
+                int last = 0;
+                int *ticket = &p.tickets2[out.rec0 * kGqa + h];
+                if (lane == 0) {
+                    last = ticket_acq_rel(ticket) == n_sub - 1;
+                    if (last) *ticket = 0;
+                }
+                if (!__shfl_sync(0xffffffffu, last, 0)) continue;
+                r = merge_records4([&](int k) { return record(p.scratch2, k); }, n_sub, d0);
+            }
             const float sink2 = sm.sinks[head] * kLog2e;
             const float Mf = fmaxf(r.M, sink2), cf = fast_exp2(r.M - Mf);
             const float inv = cf / (r.L * cf + fast_exp2(sink2 - Mf));
-            store_out4(p.out, p.out_dtype, size_t(f.row) * kQDim + head * kHeadDim + d0, r.a[0] * inv, r.a[1] * inv, r.a[2] * inv, r.a[3] * inv);
-        };
-#pragma unroll 1
-        for (int h = h0; h < h0 + kHeads; h++) {
-            const Merged4 r = merge_records4([&](int i) { return record(p.scratch, sub * fan + i, h); }, n, d0);
-            if (n_sub == 1) {
-                finish(r, h);
-                continue;
-            }
-            float *rec = record(p.scratch2, sub, h);
-            *reinterpret_cast<float4 *>(rec + d0) = make_float4(r.a[0], r.a[1], r.a[2], r.a[3]);
-            if (lane == 0) *reinterpret_cast<float2 *>(rec + kHeadDim) = make_float2(r.M, r.L);
+            store_out4(p.out, p.out_dtype, size_t(out.row) * kQDim + head * kHeadDim + d0, r.a[0] * inv, r.a[1] * inv, r.a[2] * inv, r.a[3] * inv);
         }
-        if (n_sub == 1) return;
-        __syncthreads();
-        if (tid == 0) {
-            const bool last = ticket_acq_rel(&p.tickets2[rec0]) == n_sub - 1;
-            if (last) p.tickets2[rec0] = 0;
-            sm.last2 = last;
-        }
-        __syncthreads();
-        if (!sm.last2) return;
-#pragma unroll 1
-        for (int h = h0; h < h0 + kHeads; h++)
-            finish(merge_records4([&](int i) { return record(p.scratch2, i, h); }, n_sub, d0), h);
     };
 
     get_piece(int(blockIdx.x));
@@ -364,7 +372,7 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     fetch_rows(int(blockIdx.x));
     if (lane == 0 && ta + warp < tb) load_part(ta + warp, 0);
-    if (tid == 0) ask_next(smem_u32(&sm.next), smem_u32(&sm.next_bar));
+    if (p.several_rounds && tid == 0) ask_next(smem_u32(&sm.next), smem_u32(&sm.next_bar));
     rope_table(int(blockIdx.x));
     __syncthreads();
     finish_rows();
@@ -433,8 +441,8 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
 #pragma unroll
     for (int i = 0; i < 2 * kKv4Groups; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     // what comes next (asked for a piece ago): its rows are fetched while this piece is worked on
-    bool late = !__all_sync(0xffffffffu, wait_bar(smem_u32(&sm.next_bar), turn & 1u));
-    const int next = late ? -1 : next_index(smem_u32(&sm.next));
+    bool late = p.several_rounds && !__all_sync(0xffffffffu, wait_bar(smem_u32(&sm.next_bar), turn & 1u));
+    const int next = !p.several_rounds || late ? -1 : next_index(smem_u32(&sm.next));
     if (next >= 0) {
         fetch_rows(next);
         rope_table(next);
@@ -587,7 +595,7 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
         cp_async_wait<0>();
         if (lane == 0)
             for (int i = 0; i < 4; i++) wait_bar(i & 1 ? v_bar : k_bar, uint32_t(i >> 1) & 1u);
-        if (tid == 0)
+        if (p.several_rounds && tid == 0)
             for (uint32_t i = 0; i < 2; i++) wait_bar(smem_u32(&sm.next_bar), i);
         return;
     }
@@ -652,26 +660,16 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
             if (lane == 0) *reinterpret_cast<float2 *>(rec + kHeadDim) = make_float2(M, L);
         }
     }
-    __syncthreads();  // the merge buffer is free, the next piece's rows are there
-
-    // ---- split-K: the last piece of a run of records to arrive merges the run.  The record stores are ordered before thread
-    // 0's ticket by the barrier, and the ticket is an acquire-release atomic at device scope, cumulative over them; the
-    // readers go past L1.  The ticket's answer is looked at after the next piece: no piece waits for the round trip.
-    if (waiting && sm.done[(turn & 1) ^ 1].last) merge_run((turn & 1) ^ 1);
+    if (waiting) merge_runs();
     waiting = n_split > 1;
-    if (waiting && tid == 0) {
-        const int fan = dec4_fan(n_split), sub = split / fan;
-        int *ticket = &p.tickets[rec0 + sub * kNHeadKv];
-        const bool last = ticket_acq_rel(ticket) == min(fan, n_split - sub * fan) - 1;
-        if (last) *ticket = 0;  // ready for the next launch; nothing in this one waits for it
-        sm.done[turn & 1] = {rec0, split, n_split, kv_head, row, last};
+    if (waiting) {
+        out = {rec0, split, n_split, kv_head, row};
+        count_record();
     }
-    if (!more) {
-        __syncthreads();
-        if (waiting && sm.done[turn & 1].last) merge_run(int(turn & 1));
-        break;
-    }
+    if (!more) break;
+    __syncthreads();  // the merge buffer is free, the next piece's rows are there
     }  // pieces
+    if (waiting) merge_runs();
 }
 
 template <int kCap>

@@ -40,11 +40,12 @@ __host__ __device__ inline Dec4Range dec4_range(int pos, int is_swa, int first_t
     return r;
 }
 
-// Splits folded by one CTA in the first merge level: all of them while one trip to memory holds their records, else two
+// Splits folded by one warp in the first merge level: all of them while one trip to memory holds their records, else two
 // levels of about equal size.
+constexpr int kDec4MergeTrip = 10;  // records whose loads are in flight together
 __host__ __device__ inline int dec4_fan(int n_split) {
-    if (n_split <= 10) return n_split;
-    int f = 10;
+    if (n_split <= kDec4MergeTrip) return n_split;
+    int f = kDec4MergeTrip;
     while (f * f < n_split) f++;
     return f;
 }
