@@ -413,6 +413,9 @@ struct flint_attn {
     // Decode over a 4-bit cache.
     void decode_kv4(Layer &L, int n, const int32_t *seqs, const int32_t *p, const void *qkv, int qkv_dtype, void *out,
                     int out_dtype, cudaStream_t st, const HostRows *rows) {
+        if (!rows && (!qkv || !out)) throw std::runtime_error("null pointer");
+        if (!rows && ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(out)) & 15))
+            throw std::runtime_error("q/k/v and output rows must start on a 16-byte boundary");
         if (rows) {  // page-locked rows are read where they lie, as in decode_dev
             const bool in_place = rows->mapped && n * kNHeadKv * 2 >= target_items;
             if (!in_place) CK(cudaMemcpyAsync(rows->staging, rows->host, rows->bytes, cudaMemcpyHostToDevice, st));

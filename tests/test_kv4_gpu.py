@@ -239,6 +239,11 @@ def test_rows_refused(fa):
         w = _weights(torch, 1)
         h.set_layer(0, *(t.numpy() for t in w))
         big = torch.zeros(1, 5120, device="cuda")
+        for rows, out in ((0, big), (big, 0), (big.data_ptr() + 8, big), (big, big.data_ptr() + 2)):
+            with pytest.raises(fa.FlintAttnError, match="null|16-byte"):
+                h.decode_dev(0, [0], rows, fa.F32, out, fa.F32)
+        with pytest.raises(fa.FlintAttnError, match="dtype"):
+            h.decode_dev(0, [0], big, fa.F16, big, fa.F32)
         with pytest.raises(fa.FlintAttnError, match="4-bit"):
             h.decode_partial_dev(0, [0], big, fa.F32, big)
         with pytest.raises(fa.FlintAttnError, match="4-bit"):
@@ -314,7 +319,7 @@ def test_decode(fa, in_type, out_type, is_swa, rope, paged, first):
 
 
 @gpu
-@pytest.mark.parametrize("n,pos,target", [(1, 9000, 0), (2, 40000, 0), (64, 700, 0), (70, 513, 7), (1, 70000, 2000), (200, 90, 0)])
+@pytest.mark.parametrize("n,pos,target", [(700, 130, 0), (1, 1040, 0), (30, 1700, 0), (1, 9000, 0), (2, 40000, 0), (64, 700, 0), (70, 513, 7), (1, 70000, 2000), (200, 90, 0)])
 def test_decode_splits(fa, n, pos, target):
     """Long ranges cut into many items and merged in two levels, batches that fill the GPU, work lists that are uploaded."""
     import torch
@@ -515,7 +520,7 @@ def test_host_buffers_blocks_and_other_streams(fa, fo):
     kinds = [(True, True), (False, False)]
     sw = fo.stack_weights(3, 2, 256, 128, kinds)
     outs = []
-    for how in ("host", "dev"):
+    for how in ("host", "pinned", "dev"):
         with fa.Attn([True, False], [True, False], n, 200, kv_format=fa.KV_INT4, first_tokens=4) as h:
             for il in range(2):
                 h.set_layer(il, sw["q_norm"][il], sw["k_norm"][il], sw["sinks"][il])
@@ -525,7 +530,7 @@ def test_host_buffers_blocks_and_other_streams(fa, fo):
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
             for il in range(2):
-                if how == "host":
+                if how != "dev":
                     rows = qkv.cpu()
                     h.prefill(il, 0, T, rows[:T].contiguous(), fa.F32, out, fa.F32)
                 else:
@@ -535,8 +540,11 @@ def test_host_buffers_blocks_and_other_streams(fa, fo):
                     out.copy_(d)
             h.advance([0], T)
             for il in range(2):
-                if how == "host":
-                    h.decode(il, [0], qkv[T:].cpu(), fa.F32, row, fa.F32)
+                if how != "dev":
+                    rows = qkv[T:].cpu()
+                    if how == "pinned":
+                        rows, row = rows.pin_memory(), row.pin_memory()
+                    h.decode(il, [0], rows, fa.F32, row, fa.F32)
                 else:
                     d = torch.empty(1, 4096, device="cuda")
                     h.decode_dev(il, [0], qkv[T:].contiguous(), fa.F32, d, fa.F32, side.cuda_stream)
@@ -551,8 +559,8 @@ def test_host_buffers_blocks_and_other_streams(fa, fo):
                 h.decode_block_dev(il, [1], y)
             h.check()
             outs.append([t.cpu().clone() for t in (out, row, x, y)])
-    for a, b in zip(*outs):
-        assert torch.isfinite(a).all() and torch.equal(a, b)
+    for a, b, c in zip(*outs):
+        assert torch.isfinite(a).all() and torch.equal(a, b) and torch.equal(a, c)
 
 
 @gpu
@@ -618,3 +626,66 @@ def test_positions_past_32_bits_of_bytes(fa):
         kb, vb = torch.empty(2, 1, 4, 3, 128, device="cuda")
         h.load_kv_dev(0, [n - 1], [n_ctx - 3], 3, kb, vb, fa.F32)
         assert torch.equal(kb, ref.kept(far_k).float()) and torch.equal(vb, ref.kept(far_v).float())
+
+
+@gpu
+def test_serving_loop_on_pages(fa):
+    """Requests that join, decode together and leave, on a pool too small for all of them at once: pages that held other
+    sequences (not-a-number rows among them) serve the next ones, and each request gets what it gets alone."""
+    import torch
+
+    from flint_mac_b200 import ContinuousBatcher
+
+    torch.manual_seed(5)
+    reqs = {i: (40 + 97 * i, 5 + i) for i in range(6)}  # prompt tokens, new tokens
+    rows = {i: _rand(torch, 100 + i, p + n, 5120) for i, (p, n) in reqs.items()}
+    alone = {}
+    for i, (p, n) in reqs.items():
+        h, _ = _open(fa, torch, False, True, 1, p + n)
+        with h:
+            out = torch.empty(p + n, 4096, device="cuda")
+            h.prefill_dev(0, 0, p, rows[i], fa.F32, out, fa.F32)
+            h.advance([0], p)
+            for t in range(p, p + n):
+                h.decode_dev(0, [0], rows[i][t:t + 1].contiguous(), fa.F32, out[t:t + 1], fa.F32)
+                h.advance([0])
+            h.check()
+            alone[i] = out
+    h, _ = _open(fa, torch, False, True, 3, 1024, kv_pages=18)
+    with h:
+        junk = torch.full((1, 4, 1024, 128), math.nan, device="cuda")
+        for s in range(3):  # every page has held something else
+            h.store_kv_dev(0, [s], [0], 6 * 64, junk[:, :, :6 * 64].contiguous(), junk[:, :, :6 * 64].contiguous(), fa.F32)
+        for s in range(3):
+            h.seq_release(s)
+        assert h.pages_free() == 18
+        b = ContinuousBatcher(max_seqs=3, kv_pages=18, n_ctx=1024)
+        for i, (p, n) in reqs.items():
+            b.submit(i, p, n)
+        got = {i: torch.empty_like(alone[i]) for i in reqs}
+        steps = 0
+        while not b.idle:
+            plan = b.next_step()
+            for r in plan.admit:
+                p = reqs[r.req_id][0]
+                h.prefill_dev(0, r.slot, p, rows[r.req_id], fa.F32, got[r.req_id], fa.F32)
+                h.advance([r.slot], p)
+            if plan.decode:
+                slots = [r.slot for r in plan.decode]
+                at = [h.pos(s) for s in slots]
+                x = torch.stack([rows[r.req_id][t] for r, t in zip(plan.decode, at)])
+                o = torch.empty(len(slots), 4096, device="cuda")
+                h.decode_dev(0, slots, x, fa.F32, o, fa.F32)
+                h.advance(slots)
+                for r, t, y in zip(plan.decode, at, o):
+                    got[r.req_id][t] = y
+            for r in b.complete(plan):
+                h.seq_release(r.slot)
+            steps += 1
+            assert steps < 200
+        h.check()
+        assert h.pages_free() == 18
+    for i in reqs:
+        # the same values, split and summed in another order: 32-bit sums and the probabilities' half rounding
+        err = float((got[i] - alone[i]).norm() / alone[i].norm())
+        assert err <= 1e-3, (i, err)
