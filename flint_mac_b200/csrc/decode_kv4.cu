@@ -51,7 +51,7 @@ struct __align__(128) Dec4Smem {
     alignas(16) float rope_cos[kHeadDim / 2], rope_sin[kHeadDim / 2];
     alignas(16) float q_norm[kHeadDim], k_norm[kHeadDim], sinks[kNHead];
 };
-static_assert(sizeof(Dec4Smem<4>) * 4 <= 223 * 1024 && sizeof(Dec4Smem<8>) * 2 <= 225 * 1024, "CTAs of an SM");
+static_assert(sizeof(Dec4Smem<16>) <= 225 * 1024 && sizeof(Dec4Smem<4>) * 4 <= 223 * 1024 && sizeof(Dec4Smem<8>) * 2 <= 225 * 1024, "CTAs of an SM");
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst),
@@ -208,11 +208,13 @@ template <int kWarps>
 __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Piece *pieces) {
     extern __shared__ __align__(128) unsigned char smem_raw[];
     Dec4Smem<kWarps> &sm = *reinterpret_cast<Dec4Smem<kWarps> *>(smem_raw);
-    constexpr int kThreads = kWarps * 32, kHeads = kGqa / kWarps;  // kHeads: query heads of the group that a warp looks after
+    constexpr int kThreads = kWarps * 32;
+    constexpr int kHeads = kWarps < kGqa ? kGqa / kWarps : 1;  // query heads of the group that a warp looks after, if it does:
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, t4 = lane & 3, d0 = 4 * lane;
     // Which warps do what beside: the last two have the new token's k and v (their tiles come last, if they have any), two
     // others the rotation table.
+    const bool has_heads = kWarps <= kGqa || warp < kGqa;
     const int nw = warp - (kWarps - 2), rope_at = tid - (kWarps / 2 - 2) * 32;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const bool rope = p.has_rope != 0;
@@ -277,7 +279,8 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
             else cp_async8(dst, row + (at + d0) * es);
         };
 #pragma unroll
-        for (int i = 0; i < kHeads; i++) fetch((head0 + warp * kHeads + i) * kHeadDim, warp * kHeads + i);
+        for (int i = 0; i < kHeads; i++)
+            if (has_heads) fetch((head0 + warp * kHeads + i) * kHeadDim, warp * kHeads + i);
         if (w.split == w.n_split - 1 && nw >= 0) fetch(kQDim + nw * kKvDim + (index & 3) * kHeadDim, kGqa + nw);
         cp_async_commit();
     };
@@ -300,6 +303,7 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
         const float qscale = rsqrtf(float(kHeadDim)) * kLog2e;  // softmax runs in base 2
 #pragma unroll
         for (int i = 0; i < kHeads; i++) {
+            if (!has_heads) break;
             const int h = warp * kHeads + i;
             float4 x = norm_rope(load_row4(&sm.raw[h][0], p.qkv_dtype, 0, lane), reinterpret_cast<const float4 *>(sm.q_norm)[lane], cs, sn, lane, rope);
             x.x *= qscale; x.y *= qscale; x.z *= qscale; x.w *= qscale;
@@ -387,7 +391,7 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
     float s_new[kHeads];  // the new token's score with the warp's heads
 #pragma unroll
     for (int i = 0; i < kHeads; i++) s_new[i] = -INFINITY;
-    if (ends) {
+    if (ends && has_heads) {
         const uint2 h = *reinterpret_cast<const uint2 *>(&sm.knew[d0]);
         const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&h.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
 #pragma unroll
@@ -631,6 +635,7 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
     const int old = more ? flip ^ 1 : flip;
 #pragma unroll
     for (int i = 0; i < kHeads; i++) {
+        if (!has_heads) break;
         const int h = warp * kHeads + i, head = kv_head * kGqa + h;
         float M = s_new[i];
 #pragma unroll
@@ -661,7 +666,7 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
         }
     }
     if (waiting) merge_runs();
-    waiting = n_split > 1;
+    waiting = n_split > 1 && has_heads;
     if (waiting) {
         out = {rec0, split, n_split, kv_head, row};
         count_record();
@@ -702,7 +707,8 @@ cudaError_t setup_list() { return allow_smem(k_decode_kv4<kCap, kWarps>, sizeof(
 }  // namespace
 
 cudaError_t decode_kv4_setup() {
-    cudaError_t e = setup_list<kSmallPieces, 8>();
+    cudaError_t e = setup_list<kSmallPieces, 16>();
+    if (e == cudaSuccess) e = setup_list<kSmallPieces, 8>();
     if (e == cudaSuccess) e = setup_list<kMidPieces, 8>();
     if (e == cudaSuccess) e = setup_list<kDec4MaxPieces, 8>();
     if (e == cudaSuccess) e = setup_list<kMidPieces, 4>();
@@ -713,7 +719,8 @@ cudaError_t decode_kv4_setup() {
 cudaError_t launch_decode_kv4(const Dec4Params &p, const Dec4Piece *pieces, int n_pieces, int n_warps, cudaStream_t stream) {
     if (n_pieces <= 0) return cudaSuccess;
     if (n_pieces > kDec4MaxPieces) return cudaErrorInvalidValue;
-    if (n_warps == 8 && n_pieces <= kSmallPieces) return launch_list<kSmallPieces, 8>(p, pieces, n_pieces, stream);
+    if (n_warps == 16 && n_pieces <= kSmallPieces) return launch_list<kSmallPieces, 16>(p, pieces, n_pieces, stream);
+    if (n_warps >= 8 && n_pieces <= kSmallPieces) return launch_list<kSmallPieces, 8>(p, pieces, n_pieces, stream);
     if (n_warps == 8 && n_pieces <= kMidPieces) return launch_list<kMidPieces, 8>(p, pieces, n_pieces, stream);
     if (n_warps == 8) return launch_list<kDec4MaxPieces, 8>(p, pieces, n_pieces, stream);
     if (n_pieces <= kMidPieces) return launch_list<kMidPieces, 4>(p, pieces, n_pieces, stream);

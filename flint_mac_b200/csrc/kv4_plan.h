@@ -14,7 +14,7 @@
 
 namespace flint {
 
-constexpr int kDec4CtasPerSm = 2;     // CTAs of eight warps that an SM holds at a time (of four: four)
+constexpr int kDec4CtasPerSm = 2;     // CTAs of eight warps that an SM holds at a time (of four: four, of sixteen: one)
 constexpr int kDec4MaxPieces = 1300;  // of one launch (the list travels in the kernel's parameters)
 
 // Tiles [t0, t0 + n) of a token, part `split` of n_split, for each of the four KV heads.
@@ -57,9 +57,10 @@ __host__ __device__ inline int dec4_fan(int n_split) {
 // While every token's four groups fit the slots the launch is one round: the tokens are cut so that the longest piece is as
 // short as the slots allow.  A piece costs some 5 us beside its tiles (rows, norm and rotation, the merges), so nothing is
 // cut below kLeast tiles, and a window never.  Larger batches go in several rounds, cut only where a token is longer than a
-// slot's share.  Eight warps a piece: 64 x 8192 keys take 68 us (four warps: 73), one 131072-key sequence 28 (33); a round
-// of many short pieces is over sooner with four, whose CTAs overlap each other's beginnings and ends (256 windows: 33
-// against 40 us).
+// slot's share.  Eight warps a piece: 64 x 8192 keys take 68 us (four warps: 73), one 131072-key sequence 28 (33); many
+// short pieces are over sooner with four, whose CTAs overlap each other's beginnings and ends (256 windows: 33 against
+// 40 us), and pieces that leave half of the GPU idle with sixteen, if they have tiles for them (32 windows: 7.5 against
+// 10.2 us).
 inline int plan_decode_kv4(int n, const int32_t *seqs, const int32_t *pos, const int *tiles, int slots,
                            std::vector<Dec4Piece> &pieces, int &n_records, int &n_warps) {
     constexpr int kLeast = 16;
@@ -93,7 +94,7 @@ inline int plan_decode_kv4(int n, const int32_t *seqs, const int32_t *pos, const
         if (n_split > 1) n_records += n_split;
     }
     std::stable_sort(pieces.begin(), pieces.end(), [](const Dec4Piece &a, const Dec4Piece &b) { return a.n > b.n; });
-    n_warps = !one_round && largest <= kLeast ? 4 : 8;
+    n_warps = !one_round && largest <= kLeast ? 4 : int(pieces.size()) * kNHeadKv * 2 <= slots && largest > 8 ? 16 : 8;
     return n;
 }
 
