@@ -225,6 +225,17 @@ class Attn:
         if r != 0:
             raise FlintAttnError(err.value.decode(errors="replace"))
 
+    def _bound(self, name, *args):
+        """(function, arguments as C objects, error buffer) for a call that is made again and again: nothing is converted
+        when it is made, which is two of its four microseconds."""
+        fn = self._lib[name]  # a function object of its own, without argument types
+        fn.restype = C.c_int32
+        types = SYMBOLS[name][1]
+        given = (self._h,) + args + (self._err, ERR_LEN)
+        assert len(given) == len(types)
+        simple = (C.c_int32, C.c_void_p)
+        return fn, tuple(t(x) if t in simple and not isinstance(x, C._SimpleCData) else x for t, x in zip(types, given)), self._err
+
     # ---- state
     def pos(self, seq: int) -> int:
         return int(self._lib.flint_attn_pos(self._h, seq))
@@ -283,10 +294,13 @@ class Attn:
     def prepared_decode_dev(self, layer, seqs, qkv_dtype, out_dev, out_dtype, stream: int = 0):
         """For a caller that decodes the same batch every step (a serving loop): every argument except the address
         of the step's q|k|v rows is converted once.  Returns f(qkv_address) that enqueues flint_attn_decode_dev."""
-        fn, h, n, arr, outp, err = self._lib.flint_attn_decode_dev, self._h, len(seqs), _i32(seqs), _ptr(out_dev), self._err
+        rows = C.c_void_p(0)
+        fn, args, err = self._bound("flint_attn_decode_dev", layer, len(seqs), _i32(seqs), rows, qkv_dtype, _ptr(out_dev),
+                                    out_dtype, stream)
 
         def call(qkv_address: int):
-            if fn(h, layer, n, arr, qkv_address, qkv_dtype, outp, out_dtype, stream, err, ERR_LEN) != 0:
+            rows.value = qkv_address
+            if fn(*args) != 0:
                 raise FlintAttnError(err.value.decode(errors="replace"))
 
         return call
@@ -391,11 +405,10 @@ class Attn:
         """f() that enqueues the call, with every argument converted once."""
         if len(seqs) != len(pos0):
             raise ValueError("one start position per sequence")
-        fn, h, err = getattr(self._lib, name), self._h, self._err
-        args = (layer, len(seqs), _i32(seqs), _i32(pos0), n_rows, _ptr(k_dev), _ptr(v_dev), dtype, stream)
+        fn, args, err = self._bound(name, layer, len(seqs), _i32(seqs), _i32(pos0), n_rows, _ptr(k_dev), _ptr(v_dev), dtype, stream)
 
         def call():
-            if fn(h, *args, err, ERR_LEN) != 0:
+            if fn(*args) != 0:
                 raise FlintAttnError(err.value.decode(errors="replace"))
 
         return call
