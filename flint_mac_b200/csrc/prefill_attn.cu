@@ -92,7 +92,18 @@ struct PfArgs {
 static_assert(kMaxFirstTokens == 64, "half a key tile");
 
 // What a query sees, beyond the causal limit; the attention kernel is compiled for each.
-enum { kFull = 0, kWindow = 1, kWindowFirst = 2 };
+enum { kFull = 0, kWindow = 1, kWindowFirst = 2, kFullCut = 3 };
+
+// kFullCut: a full layer whose units are cut at any key tile, so that every CTA has the same number of tiles.  Entry e: key
+// tiles [tile0, tile1) of unit `unit`, part `part` of it; CTA b has the entries start[b] .. start[b + 1] - 1.
+constexpr int kMaxCuts = 640, kMaxCutCtas = 160;
+struct PfCut {
+    uint16_t unit, part, tile0, tile1;
+};
+struct PfCuts {
+    PfCut e[kMaxCuts];
+    uint16_t start[kMaxCutCtas + 2];
+};
 
 // ------------------------------------------------------------------------------------------------- prologue
 // Packed two-float arithmetic (sm_100): a 64-bit register holds two floats.
@@ -443,7 +454,16 @@ __host__ __device__ inline Unit unit_geom_of(int u, int n_tok, int p0, int is_sw
     return g;
 }
 template <int kKind>
-__device__ __forceinline__ Unit unit_geom(const PfArgs &a, int u) {
+__device__ __forceinline__ Unit unit_geom(const PfArgs &a, const PfCuts *cuts, int u) {
+    if (kKind == kFullCut) {
+        const PfCut c = cuts->e[u];
+        Unit g = unit_geom_of(c.unit, a.n_tok, a.p0, 0, a.key_row0, 1, a.kr_lo, a.kr_hi);
+        g.klo += c.tile0 * kBN;
+        g.n_keys = min(g.n_keys - c.tile0 * kBN, (c.tile1 - c.tile0) * kBN);
+        g.n_tiles = c.tile1 - c.tile0;
+        g.split = c.part;
+        return g;
+    }
     return unit_geom_of(u, a.n_tok, a.p0, a.is_swa, a.key_row0, a.n_ksplit, a.kr_lo, a.kr_hi,
                         kKind == kWindowFirst ? a.first_tokens : 0);
 }
@@ -452,7 +472,12 @@ __device__ __forceinline__ Unit unit_geom(const PfArgs &a, int u) {
 // CTA's list out longest first; the CTA copies its list into shared memory at start (entries past kSchedLocal stay
 // in global memory).  Without a table (at most one unit per CTA, or FLINT_ATTN_PREFILL_SCHEDULE=roundrobin in the
 // environment) CTA b takes units b, b + grid, ...
-__device__ __forceinline__ int unit_at(const PfArgs &a, const int *local, int i) {
+template <int kKind>
+__device__ __forceinline__ int unit_at(const PfArgs &a, const PfCuts *cuts, const int *local, int i) {
+    if (kKind == kFullCut) {
+        const int u = cuts->start[blockIdx.x] + i;
+        return u < cuts->start[blockIdx.x + 1] ? u : -1;
+    }
     if (!a.sched) {
         const int u = int(blockIdx.x) + i * int(gridDim.x);
         return u < a.n_units ? u : -1;
@@ -472,12 +497,9 @@ __device__ __forceinline__ int unit_at(const PfArgs &a, const int *local, int i)
 // (compiled per layer kind and output type: the code of the other three combinations would only take up
 // instruction cache, which the softmax warps are short of)
 template <int kKind, bool kOutF32>
-__global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_constant__ CUtensorMap tm_q,
-                                                                  const __grid_constant__ CUtensorMap tm_k,
-                                                                  const __grid_constant__ CUtensorMap tm_v,
-                                                                  const __grid_constant__ CUtensorMap tm_o,
-                                                                  const PfArgs a) {
-    constexpr bool kSwa = kKind != kFull;
+__device__ __forceinline__ void prefill_attn(const CUtensorMap &tm_q, const CUtensorMap &tm_k, const CUtensorMap &tm_v,
+                                             const CUtensorMap &tm_o, const PfArgs &a, const PfCuts *cuts) {
+    constexpr bool kSwa = kKind == kWindow || kKind == kWindowFirst;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t base = smem_u32(smem_raw);
     unsigned char *gen = smem_raw;
@@ -579,9 +601,9 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
                 return true;
             };
             for (int i = 0; ok; i++) {
-                const int u = unit_at(a, sched_local, i);
+                const int u = unit_at<kKind>(a, cuts, sched_local, i);
                 if (u < 0) break;
-                const Unit un = unit_geom<kKind>(a, u);
+                const Unit un = unit_geom<kKind>(a, cuts, u);
                 // order of need: Q0, K(0), Q1, V(0), K(1), V(1), ...
                 ok = load_q(un, 0, i) && load_tile(&tm_k, un, 0) && load_q(un, 1, i);
                 for (int kt = 0; kt < un.n_tiles && ok; kt++) {
@@ -620,11 +642,11 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
             if (c.kt + 1 < c.un.n_tiles) {
                 c.kt++;
             } else {
-                const int u = unit_at(a, sched_local, c.i + 1);
+                const int u = unit_at<kKind>(a, cuts, sched_local, c.i + 1);
                 if (u < 0) return false;
                 c.i++;
                 c.kt = 0;
-                c.un = unit_geom<kKind>(a, u);
+                c.un = unit_geom<kKind>(a, cuts, u);
             }
             c.j++;
             return true;
@@ -664,8 +686,8 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
             tc5::mma_commit_w(bar(kBarSlotEmpty + slot), leader);
             return true;
         };
-        if (unit_at(a, sched_local, 0) >= 0) {
-            Cursor cur{0, 0, 0, unit_geom<kKind>(a, unit_at(a, sched_local, 0))};
+        if (unit_at<kKind>(a, cuts, sched_local, 0) >= 0) {
+            Cursor cur{0, 0, 0, unit_geom<kKind>(a, cuts, unit_at<kKind>(a, cuts, sched_local, 0))};
             ok = issue_qk(cur);
             while (ok) {
                 Cursor nxt = cur;
@@ -692,9 +714,9 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
         const uint32_t colS = lane_base + kColS + w * kBN, colO = lane_base + kColO + w * kHeadDim;
         int j = 0;  // tiles of the stream seen so far (phase of the S / P / P.V barriers)
         for (int i = 0; ok; i++) {
-        const int u = unit_at(a, sched_local, i);
+        const int u = unit_at<kKind>(a, cuts, sched_local, i);
         if (u < 0) break;
-        const Unit un = unit_geom<kKind>(a, u);
+        const Unit un = unit_geom<kKind>(a, cuts, u);
         const int kvh = un.kvh, t0 = un.t0, klo = un.klo, n_keys = un.n_keys, n_tiles = un.n_tiles;
         const int qt_first = un.q_first + w * kQPos;  // first / last position of this Q tile
         const int qt_last = min(qt_first + kQPos - 1, un.q_last);
@@ -943,6 +965,23 @@ __global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_c
     if (warp == 0) tc5::tmem_dealloc(tmem, kTmemCols);
 }
 
+template <int kKind, bool kOutF32>
+__global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn(const __grid_constant__ CUtensorMap tm_q,
+                                                                  const __grid_constant__ CUtensorMap tm_k,
+                                                                  const __grid_constant__ CUtensorMap tm_v,
+                                                                  const __grid_constant__ CUtensorMap tm_o,
+                                                                  const PfArgs a) {
+    prefill_attn<kKind, kOutF32>(tm_q, tm_k, tm_v, tm_o, a, nullptr);
+}
+__global__ void __launch_bounds__(kThreadsAttn, 1) k_prefill_attn_cut(const __grid_constant__ CUtensorMap tm_q,
+                                                                      const __grid_constant__ CUtensorMap tm_k,
+                                                                      const __grid_constant__ CUtensorMap tm_v,
+                                                                      const __grid_constant__ CUtensorMap tm_o,
+                                                                      const __grid_constant__ PfArgs a,
+                                                                      const __grid_constant__ PfCuts cuts) {
+    prefill_attn<kFullCut, true>(tm_q, tm_k, tm_v, tm_o, a, &cuts);
+}
+
 // Merge of the key-range partials of one chunk: out[t][head][:] = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M)
 // (the log-sum-exp merge of src/metal/fused.metal:332-350 applied to prefill rows; the sink is inside range 0's l).
 // One CTA per (token, 4 heads), thread = (head, 4 dims).
@@ -1055,6 +1094,58 @@ cudaError_t build_schedule(PrefillWorkspace &ws, const PfArgs &a, int n_units, i
     return cudaSuccess;
 }
 
+// Cuts the units' key tiles into `grid` stretches of equal length, no piece under four tiles (but whole units).  Returns
+// the number of parts that the most divided unit has, 0 if there would be more pieces than `cuts` holds.
+int plan_cuts(const PfArgs &a, int n_units, int grid, PfCuts &cuts, int &n_pieces) {
+    constexpr int kLeast = 4;
+    if (grid > kMaxCutCtas || n_units > 0xffff) return 0;
+    auto tiles_of = [&](int u) { return unit_geom_of(u, a.n_tok, a.p0, 0, a.key_row0, 1, a.kr_lo, a.kr_hi).n_tiles; };
+    long long total = 0;
+    for (int u = 0; u < n_units; u++) total += tiles_of(u);
+    int most = 0, cta = 0;
+    long long done = 0;  // tiles handed out
+    n_pieces = 0;
+    cuts.start[0] = 0;
+    for (int u = 0; u < n_units; u++) {
+        const int T = tiles_of(u);
+        if (T > 0xffff) return 0;
+        int at = 0, part = 0;
+        while (at < T) {
+            // to the end of the CTA's stretch; a rest that would be too short stays with its neighbour
+            long long take = total * (cta + 1) / grid - done;
+            if (cta == grid - 1 || take > T - at - kLeast) take = T - at;
+            if (take < kLeast && take < T - at) {  // (the stretch is as good as full)
+                cuts.start[++cta] = uint16_t(n_pieces);
+                continue;
+            }
+            if (n_pieces == kMaxCuts) return 0;
+            cuts.e[n_pieces++] = PfCut{uint16_t(u), uint16_t(part++), uint16_t(at), uint16_t(at + take)};
+            at += int(take);
+            done += take;
+            while (cta < grid - 1 && total * (cta + 1) / grid - done < 1) cuts.start[++cta] = uint16_t(n_pieces);
+        }
+        most = std::max(most, part);
+    }
+    while (cta < grid) cuts.start[++cta] = uint16_t(n_pieces);
+    return most;
+}
+
+// The load of the busiest CTA, in tiles, when whole units go to the least loaded CTA in turn (build_schedule).
+int whole_units_load(const PfArgs &a, int n_units, int grid) {
+    std::vector<int> load(grid, 0);
+    std::priority_queue<std::pair<int, int>, std::vector<std::pair<int, int>>, std::greater<std::pair<int, int>>> heap;
+    for (int b = 0; b < grid; b++) heap.push({0, b});
+    int most = 0;
+    for (int u = 0; u < n_units; u++) {
+        const auto [l, b] = heap.top();
+        heap.pop();
+        const int now = l + unit_geom_of(u, a.n_tok, a.p0, 0, a.key_row0, 1, a.kr_lo, a.kr_hi).n_tiles + 1;
+        most = std::max(most, now);
+        heap.push({now, b});
+    }
+    return most;
+}
+
 }  // namespace
 
 cudaError_t prefill_kernel_setup() {
@@ -1073,6 +1164,7 @@ cudaError_t prefill_kernel_setup() {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_prefill_attn<kWindow, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_prefill_attn<kWindow, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_prefill_attn<kWindowFirst, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_prefill_attn_cut, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_prefill_attn<kWindowFirst, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     return e;
 }
@@ -1118,6 +1210,26 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
         n_ksplit = std::max(1, std::min(g_sm_count / n_units_q, min_tiles / 4));
     }
     const int t_pad = (T + kCtaPos - 1) / kCtaPos * kCtaPos;
+    // A full layer with a 4-bit cache: units are cut so that all CTAs end together, where that gains more than the partials
+    // cost (a piece is 131 KB of fp32 rows written and read again, about 0.05 us; a key tile takes a CTA 2.2 us).
+    static thread_local PfCuts cuts;
+    int n_cut_pieces = 0;
+    bool cut = false;
+    if (kv4 && !p.is_swa && n_units_q > 0) {
+        PfArgs g{};
+        g.n_tok = T; g.p0 = p.p0; g.key_row0 = kr_lo; g.kr_lo = kr_lo; g.kr_hi = kr_hi;
+        const int parts = plan_cuts(g, n_units_q, g_sm_count, cuts, n_cut_pieces);
+        if (parts > 1) {
+            long long total = 0;
+            for (int u = 0; u < n_units_q; u++) total += unit_geom_of(u, T, p.p0, 0, kr_lo, 1, kr_lo, kr_hi).n_tiles;
+            const double even = double(total) / g_sm_count + 2.0;
+            const double whole = n_ksplit > 1 ? unit_geom_of(0, T, p.p0, 0, kr_lo, 1, kr_lo, kr_hi).n_tiles / double(n_ksplit) + 1.0
+                                              : double(whole_units_load(g, n_units_q, g_sm_count));
+            const double partials = 0.05 * (n_cut_pieces - (n_ksplit > 1 ? n_units_q * n_ksplit : 0)) + (n_ksplit > 1 ? 0.0 : 6.0);
+            cut = (whole - even) * 2.2 > partials;
+            if (cut) n_ksplit = parts;
+        }
+    }
     const size_t part_o_bytes = n_ksplit > 1 ? up(size_t(n_ksplit) * t_pad * kQDim * sizeof(float)) : 0;
     const size_t part_ml_bytes = n_ksplit > 1 ? up(size_t(n_ksplit) * t_pad * kNHead * sizeof(float2)) : 0;
     const size_t need = q_bytes + 2 * kv_bytes + part_o_bytes + part_ml_bytes + 1024;
@@ -1235,18 +1347,20 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
     a.cp_partial = cp ? 1 : 0;
     a.block_table = p.block_table; a.table_len = p.table_len;
     a.first_tokens = first_tokens; a.first_rows = first_rows;
-    const int n_units = n_units_q * n_ksplit;
-    const dim3 grid(n_units < g_sm_count ? n_units : g_sm_count);
+    const int n_units = cut ? n_cut_pieces : n_units_q * n_ksplit;
+    const dim3 grid(cut || n_units >= g_sm_count ? g_sm_count : n_units);
     a.n_units = n_units;
     static const bool round_robin = [] {
         const char *v = getenv("FLINT_ATTN_PREFILL_SCHEDULE");
         return v && strcmp(v, "roundrobin") == 0;
     }();
-    if (n_units > int(grid.x) && !round_robin) {
+    if (n_units > int(grid.x) && !round_robin && !cut) {
         if ((e = build_schedule(ws, a, n_units, int(grid.x), stream)) != cudaSuccess) return e;
         a.sched = ws.sched;
         a.n_rounds = ws.sched_rounds;
     }
+    // (parts that a unit does not have must read as empty)
+    if (cut && (e = cudaMemsetAsync(part_ml, 0, size_t(n_ksplit) * t_pad * kNHead * sizeof(float2), stream)) != cudaSuccess) return e;
     if ((e = launch_prologue()) != cudaSuccess) return e;
     if (p.ev_attn_begin && (e = cudaEventRecord(p.ev_attn_begin, stream)) != cudaSuccess) return e;
     {
@@ -1265,7 +1379,8 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
         cfg.attrs = &attr;
         cfg.numAttrs = no_pdl ? 0 : 1;
         const bool f32 = a.out_dtype == kDtypeF32;
-        if (first_tokens > 0) e = f32 ? cudaLaunchKernelEx(&cfg, k_prefill_attn<kWindowFirst, true>, tm_q, tm_k, tm_v, tm_o, a)
+        if (cut) e = cudaLaunchKernelEx(&cfg, k_prefill_attn_cut, tm_q, tm_k, tm_v, tm_o, a, cuts);
+        else if (first_tokens > 0) e = f32 ? cudaLaunchKernelEx(&cfg, k_prefill_attn<kWindowFirst, true>, tm_q, tm_k, tm_v, tm_o, a)
                                       : cudaLaunchKernelEx(&cfg, k_prefill_attn<kWindowFirst, false>, tm_q, tm_k, tm_v, tm_o, a);
         else if (a.is_swa) e = f32 ? cudaLaunchKernelEx(&cfg, k_prefill_attn<kWindow, true>, tm_q, tm_k, tm_v, tm_o, a)
                                    : cudaLaunchKernelEx(&cfg, k_prefill_attn<kWindow, false>, tm_q, tm_k, tm_v, tm_o, a);

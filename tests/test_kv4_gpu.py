@@ -420,7 +420,7 @@ def test_extreme_scales_of_values(fa):
 @gpu
 @pytest.mark.parametrize("in_type,out_type", [("float32", "float32"), ("bfloat16", "bfloat16")])
 @pytest.mark.parametrize("is_swa,first,paged", [(False, 0, False), (False, 0, True), (True, 0, False), (True, 1, False), (True, 20, False), (True, 64, False)])
-@pytest.mark.parametrize("past,tokens", [(0, 1), (0, 33), (0, 700), (63, 2), (510, 7), (700, 130), (1500, 512), (40, 600), (2000, 1)])
+@pytest.mark.parametrize("past,tokens", [(0, 1), (0, 33), (0, 700), (63, 2), (510, 7), (700, 130), (1500, 512), (40, 600), (2000, 1), (2000, 700), (2400, 512), (1900, 1100)])
 def test_prefill(fa, in_type, out_type, is_swa, first, paged, past, tokens):
     import torch
 
