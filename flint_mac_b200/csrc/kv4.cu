@@ -161,7 +161,7 @@ __device__ __forceinline__ unsigned char *block_of(const KvRowsParams &p, const 
 // worked out by two lanes instead of four), eight lanes a row, and K and V of a block are separate CTAs.
 constexpr int kStoreSteps = kKv4BlockKeys * 8 / kRowThreads;
 template <int kType>
-__global__ void __launch_bounds__(kRowThreads, 6) k_kv4_store(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs) {
+__global__ void __launch_bounds__(kRowThreads, kType == kDtypeF32 ? 4 : 6) k_kv4_store(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs) {
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // (after the wait: see the prefill prologue)
     const bool is_v = blockIdx.y >= kNHeadKv;
@@ -169,39 +169,53 @@ __global__ void __launch_bounds__(kRowThreads, 6) k_kv4_store(const KvRowsParams
     if (b.first >= b.p1) return;
     const int sub = threadIdx.x & 7, g = sub >> 1, r0 = threadIdx.x >> 3;  // rows r0, r0 + 32: a warp has rows 4 i .. 4 i + 3
     const void *src = is_v ? p.v : p.k;
-    Eight<kType> x[kStoreSteps][2];
-#pragma unroll
-    for (int i = 0; i < kStoreSteps; i++) {
-        if (!b.has(r0 + 32 * i)) continue;
-        const size_t at = b.base + size_t(b.first + r0 + 32 * i) * kHeadDim + 16 * sub;
-        x[i][0].load(src, at);
-        x[i][1].load(src, at + 8);
-    }
     unsigned char *block = block_of(p, b);
-    unsigned char *front = p.is_swa && !p.raw_slots && b.first < p.cache.first_tokens ? kv4_first_block(p.cache, b.seq, b.kvh) : nullptr;
     // positions of one call that share a slot of a ring: only the last one of a slot is stored, whatever the order of CTAs
     const int kept = p.is_swa && !p.raw_slots ? b.p1 - kSwaRing : INT_MIN;
+    const bool front = p.is_swa && !p.raw_slots && b.first < p.cache.first_tokens;
+    Eight<kType> x[kStoreSteps][2];
+    if (!front && b.first >= b.p0 && b.first + kKv4BlockKeys <= b.p1 && b.first >= kept) {  // a whole block: the usual one of a long call
+        const size_t at = b.base + size_t(b.first + r0) * kHeadDim + 16 * sub;
 #pragma unroll
-    for (int i = 0; i < kStoreSteps; i++) {
-        const int r = r0 + 32 * i;
-        const bool in = b.has(r), pair = b.has(r & ~1) && b.has(r | 1);
+        for (int i = 0; i < kStoreSteps; i++) {
+            x[i][0].load(src, at + i * 32 * kHeadDim);
+            x[i][1].load(src, at + i * 32 * kHeadDim + 8);
+        }
+        // (32 rows further on the chunk's swizzle and the place in the pair are the same)
+        unsigned char *codes_at = block + (is_v ? kKv4VCodes : kKv4KCodes) + kv4_chunk(r0, g) + (sub & 1) * 8;
+        unsigned char *group_at = block + (is_v ? kv4_v_group(r0 & ~1, g) + (r0 & 1) * 16 : kv4_k_group(r0, g));
+#pragma unroll
+        for (int i = 0; i < kStoreSteps; i++) {
+            uint32_t mine;
+            const uint2 codes = kv4_quantise16(x[i][0].get(), x[i][1].get(), mine);
+            *reinterpret_cast<uint2 *>(codes_at + i * 32 * kKv4RowBytes) = codes;
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 8);
+            if (is_v) mine = (r0 & 1) ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);  // {lo, lo} or {d, d} of the pair
+            if ((sub & 1) == 0) *reinterpret_cast<uint32_t *>(group_at + i * 32 * 16) = mine;
+        }
+        return;
+    }
+    unsigned char *first_block = front ? kv4_first_block(p.cache, b.seq, b.kvh) : nullptr;
+#pragma unroll 1
+    for (int r = r0; r < kKv4BlockKeys; r += 32) {
+        const bool in = b.has(r);
         if (!__any_sync(0xffffffffu, in)) continue;
-        uint32_t mine;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        const uint2 codes = kv4_quantise16(in ? x[i][0].get() : zero, in ? x[i][1].get() : zero, mine);
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 8);
-        auto put = [&](unsigned char *blk, bool both) {
+        uint4 h[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        if (in) {
+            const size_t at = b.base + size_t(b.first + r) * kHeadDim + 16 * sub;
+            x[0][0].load(src, at);
+            x[0][1].load(src, at + 8);
+            h[0] = x[0][0].get();
+            h[1] = x[0][1].get();
+        }
+        uint32_t dl;
+        const uint2 codes = kv4_quantise16(h[0], h[1], dl);
+        auto put = [&](unsigned char *blk) {
             *reinterpret_cast<uint2 *>(blk + (is_v ? kKv4VCodes : kKv4KCodes) + kv4_chunk(r, g) + (sub & 1) * 8) = codes;
-            if ((sub & 1) != 0) return;
-            if (is_v && both) {  // both rows of the pair: the even one's lanes write {d, d}, the odd one's {lo, lo}
-                const uint32_t w = (r & 1) ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
-                *reinterpret_cast<uint32_t *>(blk + kv4_v_group(r & ~1, g) + (r & 1) * 16) = w;
-            } else {
-                kv4_store_group(blk, r, g, is_v, mine);
-            }
+            if ((sub & 1) == 0) kv4_store_group(blk, r, g, is_v, dl);
         };
-        if (in && b.first + r >= kept) put(block, pair && b.first + (r & ~1) >= kept);
-        if (in && front && b.first + r < p.cache.first_tokens) put(front, pair && b.first + (r | 1) < p.cache.first_tokens);
+        if (in && b.first + r >= kept) put(block);
+        if (in && first_block && b.first + r < p.cache.first_tokens) put(first_block);
     }
 }
 

@@ -71,24 +71,37 @@ __device__ __forceinline__ uint64_t kv4_mul(uint64_t a, uint64_t b) {
     asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// Codes of four values, in the low 16 bits, first one lowest.  Adding 1.5 * 2^23 rounds a quotient to the nearest whole
-// number, ties to even, and leaves that in the low bits of the sum, whose next bits are zeros.  (d = 0: the codes are 0.)
-__device__ __forceinline__ uint32_t kv4_codes4(float2 x01, float2 x23, const Kv4Scale &s) {
+// Codes of N values (pairs of floats x, at most eight), first one lowest.  Adding 1.5 * 2^23 rounds a quotient to the nearest
+// whole number, ties to even, and leaves that in the low bits of the sum, whose next bits are zeros.
+template <int N, bool kLimit>
+__device__ __forceinline__ uint32_t kv4_codes(const float2 (&x)[N / 2], const Kv4Scale &s) {
     const uint64_t lo2 = kv4_pack(-s.lo, -s.lo), inv2 = kv4_pack(s.inv, s.inv), nd2 = kv4_pack(-s.d, -s.d), magic = kv4_pack(12582912.f, 12582912.f);
-    const uint64_t a = kv4_add(kv4_pack(x01.x, x01.y), lo2), b = kv4_add(kv4_pack(x23.x, x23.y), lo2);
-    uint64_t q = kv4_mul(a, inv2), r = kv4_mul(b, inv2);
-    q = kv4_fma(kv4_fma(q, nd2, a), inv2, q);
-    r = kv4_fma(kv4_fma(r, nd2, b), inv2, r);
-    if (s.d < 6.103515625e-5f) {  // a subnormal d may lie well below (max - lo) / 15: limit to 15 (else 15.01 is the most)
-        float q0, q1, r0, r1;
-        asm("mov.b64 {%0, %1}, %2;\n" : "=f"(q0), "=f"(q1) : "l"(q));
-        asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r0), "=f"(r1) : "l"(r));
-        q = kv4_pack(fminf(q0, 15.f), fminf(q1, 15.f));
-        r = kv4_pack(fminf(r0, 15.f), fminf(r1, 15.f));
+    uint32_t c[N / 4];
+#pragma unroll
+    for (int i = 0; i < N / 4; i++) {
+        uint64_t q[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const float2 v = x[2 * i + j];
+            const uint64_t a = kv4_add(kv4_pack(v.x, v.y), lo2), q0 = kv4_mul(a, inv2);
+            q[j] = kv4_fma(kv4_fma(q0, nd2, a), inv2, q0);
+            if (kLimit) {
+                float r0, r1;
+                asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r0), "=f"(r1) : "l"(q[j]));
+                q[j] = kv4_pack(fminf(r0, 15.f), fminf(r1, 15.f));
+            }
+            q[j] = kv4_add(q[j], magic);
+        }
+        c[i] = uint32_t(q[0]) + (uint32_t(q[0] >> 32) << 4) + (uint32_t(q[1]) << 8) + (uint32_t(q[1] >> 32) << 12);
     }
-    q = kv4_add(q, magic);
-    r = kv4_add(r, magic);
-    return (uint32_t(q) + (uint32_t(q >> 32) << 4) + (uint32_t(r) << 8) + (uint32_t(r >> 32) << 12)) & 0xffffu;
+    return N == 4 ? c[0] & 0xffffu : __byte_perm(c[0], c[N / 4 - 1], 0x5410);
+}
+// d = 0: the codes are 0.  A subnormal d may lie well below (max - lo) / 15, so its quotients are limited to 15 (else 15.01
+// is the most).
+template <int N>
+__device__ __forceinline__ uint32_t kv4_codes(const float2 (&x)[N / 2], const Kv4Scale &s) {
+    if (s.inv == 0.f) return 0;
+    return s.d < 6.103515625e-5f ? kv4_codes<N, true>(x, s) : kv4_codes<N, false>(x, s);
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2 *>(&w); }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<const uint32_t *>(&h); }
@@ -104,8 +117,8 @@ __device__ __forceinline__ uint32_t kv4_quantise4(uint2 h, uint32_t &dl) {
     }
     const Kv4Scale s = kv4_scale(__hmin_nan(__low2half(lo), __high2half(lo)), __hmax_nan(__low2half(hi), __high2half(hi)));
     dl = s.dl;
-    const float2 a = __half22float2(as_half2(h.x)), b = __half22float2(as_half2(h.y));
-    return s.inv == 0.f ? 0u : kv4_codes4(a, b, s);
+    const float2 x[2] = {__half22float2(as_half2(h.x)), __half22float2(as_half2(h.y))};
+    return kv4_codes<4>(x, s);
 }
 // The same for two neighbouring lanes with sixteen values each.
 __device__ __forceinline__ uint2 kv4_quantise16(uint4 h, uint4 k, uint32_t &dl) {
@@ -116,12 +129,11 @@ __device__ __forceinline__ uint2 kv4_quantise16(uint4 h, uint4 k, uint32_t &dl) 
     hi = __hmax2_nan(hi, as_half2(__shfl_xor_sync(0xffffffffu, as_u32(hi), 1)));
     const Kv4Scale s = kv4_scale(__hmin_nan(__low2half(lo), __high2half(lo)), __hmax_nan(__low2half(hi), __high2half(hi)));
     dl = s.dl;
+    const float2 x[4] = {__half22float2(as_half2(h.x)), __half22float2(as_half2(h.y)), __half22float2(as_half2(h.z)), __half22float2(as_half2(h.w))};
+    const float2 y[4] = {__half22float2(as_half2(k.x)), __half22float2(as_half2(k.y)), __half22float2(as_half2(k.z)), __half22float2(as_half2(k.w))};
     if (s.inv == 0.f) return make_uint2(0, 0);
-    auto eight = [&](uint4 w) {
-        return kv4_codes4(__half22float2(as_half2(w.x)), __half22float2(as_half2(w.y)), s) |
-               kv4_codes4(__half22float2(as_half2(w.z)), __half22float2(as_half2(w.w)), s) << 16;
-    };
-    return make_uint2(eight(h), eight(k));
+    if (s.d < 6.103515625e-5f) return make_uint2(kv4_codes<8, true>(x, s), kv4_codes<8, true>(y, s));
+    return make_uint2(kv4_codes<8, false>(x, s), kv4_codes<8, false>(y, s));
 }
 
 // Writes {d, lo} of a group of one row.
