@@ -960,6 +960,11 @@ static void prefill_impl(flint_attn *a, int layer, int seq, int n_tok, const voi
         pp.seq = seq;
         if (!L.is_swa) pp.stage_rows = a->n_ctx;
         if (L.paged) a->ensure_pages(seq, p0 + n_tok - 1, st);
+        if (n_tok == 1) {  // one token is a decode step, which reads the cache as it is (16000 keys behind: 13 instead of 43 us)
+            const int32_t one_seq = seq, one_pos = p0;
+            a->decode_kv4(L, 1, &one_seq, &one_pos, qkv, qkv_dtype, out, out_dtype, st, nullptr);
+            return;
+        }
     } else {
         pp.k_cache = L.k + (L.paged ? 0 : size_t(seq) * kNHeadKv * L.n_slots * kHeadDim);
         pp.v_cache = L.v + (L.paged ? 0 : size_t(seq) * kNHeadKv * L.n_slots * kHeadDim);
