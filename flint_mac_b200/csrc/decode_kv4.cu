@@ -446,8 +446,8 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
     // Per lane: reference maximum (replicated over g) and partial sum of heads 2 t4 and 2 t4 + 1; outputs o[2c] = dims
     // 32 c + 4 g (n0) and + 1 (n0 + 16 n1), o[2c + 1] = dims + 2 and + 3, each for the two heads; om = the part of lo, group
     // g & 3.
-    // The reference lies 2 under the maximum (base 2), so that probabilities times d keep two more bits above half's
-    // subnormal steps; d is at most 8736, so four times that still fits a half.
+    // The reference lies 1 under a maximum (base 2) and stays until one exceeds it by 2, so that few tiles have outputs to
+    // rescale.  Probabilities are then at most 4, and times d, which is at most 8736, they fit a half.
     float m0 = -INFINITY, m1 = -INFINITY;
     uint64_t l01 = 0;  // (two zeros)
     float o[2 * kKv4Groups][4], om[4] = {0.f, 0.f, 0.f, 0.f};
@@ -520,10 +520,8 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
             mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
             mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
         }
-        mx0 -= 2.f;
-        mx1 -= 2.f;
-        if (__any_sync(0xffffffffu, mx0 > m0 || mx1 > m1)) {
-            const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+        if (__any_sync(0xffffffffu, mx0 > m0 + 2.f || mx1 > m1 + 2.f)) {
+            const float n0 = mx0 > m0 + 2.f ? mx0 - 1.f : m0, n1 = mx1 > m1 + 2.f ? mx1 - 1.f : m1;
             const float c0 = fast_exp2(m0 - n0), c1 = fast_exp2(m1 - n1);
             l01 = mul2(l01, pack2(c0, c1));
 #pragma unroll
