@@ -83,7 +83,11 @@ struct DecParams {
     // swizzle; null: tiles are fetched with 16-byte cp.async (ring layers, caller-owned caches).
     const void *k_map, *v_map;
     int *error_flag;  // set when a bounded wait of the TMA variant runs out (null: not reported)
+    // Ring layers whose first tokens stay visible: positions below first_tokens are kept in [max_seqs][4][64][128] too.
+    __half *first_k, *first_v;
+    int first_tokens;
 };
+constexpr int kMaxFirstTokens = 64;             // positions a ring layer can keep beside its window
 constexpr int kPageKeys = 64;                   // keys per KV page = one decode tile
 
 struct CombineParams {

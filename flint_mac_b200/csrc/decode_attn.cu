@@ -96,7 +96,8 @@ __device__ __forceinline__ void publish_group(const DecParams &p, int tid) {
     }
 }
 
-template <int kStages, bool kTma>
+// kFirst: a ring layer whose first tokens stay visible; those in front of the window are one more tile, the first one.
+template <int kStages, bool kTma, bool kFirst = false>
 __device__ __forceinline__ void decode_item(const DecParams &p, const DecItem &it) {
     extern __shared__ __align__(128) unsigned char smem_raw[];
     // swizzled TMA tiles need 1024-byte alignment: the launch asks for 1 KiB more than the struct and rounds up here
@@ -107,7 +108,8 @@ __device__ __forceinline__ void decode_item(const DecParams &p, const DecItem &i
     const int g = lane >> 2, t4 = lane & 3;
     const int j0 = it.j0, j1 = it.j1;
     const int j_end = j1 + (it.fold ? 1 : 0);  // the new token sits right after the cached range of a fold item
-    const int n_tiles = (j_end - j0 + kTileKeys - 1) / kTileKeys;
+    const int n_first = kFirst ? min(p.first_tokens, j0) : 0, extra = n_first > 0 ? 1 : 0;
+    const int n_tiles = extra + (j_end - j0 + kTileKeys - 1) / kTileKeys;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     // layout of the merge steps at the end: 16 threads per head, 8 dims per thread; the head's sink is fetched now
     const int mh = tid >> 4, md = (tid & 15) * 8;
@@ -120,7 +122,8 @@ __device__ __forceinline__ void decode_item(const DecParams &p, const DecItem &i
 
     auto load_tile = [&](int t) {
         const int stage = t % kStages;
-        const int jt = j0 + t * kTileKeys;
+        const int jt = j0 + (t - extra) * kTileKeys;
+        const bool front = kFirst && t < extra;
         if (kTma) {
             // One thread asks for the whole tile: two 64-dim halves of K and of V, 32 KiB on one barrier.  Rows past
             // the item's range are real cache rows (later keys, or slots never written): they are masked below, and
@@ -147,13 +150,18 @@ __device__ __forceinline__ void decode_item(const DecParams &p, const DecItem &i
             kb = p.k_cache + off;
             vb = p.v_cache + off;
         }
+        if (front) {
+            const size_t off = (size_t(it.seq) * kNHeadKv + it.kvh) * kMaxFirstTokens * kHeadDim;
+            kb = p.first_k + off;
+            vb = p.first_v + off;
+        }
 #pragma unroll
         for (int i = 0; i < (kTileKeys * 16) / kThreads; i++) {
             const int c = tid + kThreads * i;
             const int row = c >> 4, ch = c & 15;
             const int j = jt + row;
-            const bool valid = j < j1;  // cached keys only; other rows are zero-filled
-            const int slot = !valid ? 0 : p.paged ? row : int(uint32_t(j) & p.slot_mask) - p.kv_lo;
+            const bool valid = front ? row < n_first : j < j1;  // cached keys only; other rows are zero-filled
+            const int slot = !valid ? 0 : p.paged || front ? row : int(uint32_t(j) & p.slot_mask) - p.kv_lo;
             const size_t off = size_t(slot) * kHeadDim + ch * 8;
             const uint32_t dst = stage * kTileBytes + tile_off<false>(row, ch);
             cp_async16(ks_addr + dst, kb + off, valid ? 16u : 0u);
@@ -232,6 +240,10 @@ __device__ __forceinline__ void decode_item(const DecParams &p, const DecItem &i
             } else {
                 const int slot = int(uint32_t(it.pos) & p.slot_mask) - p.kv_lo;
                 store_half4(const_cast<__half *>(fold_k ? kbase : vbase) + size_t(slot) * kHeadDim + 4 * lane, kv_new);
+                if (kFirst && it.pos < p.first_tokens) {
+                    const size_t off = ((size_t(it.seq) * kNHeadKv + it.kvh) * kMaxFirstTokens + it.pos) * kHeadDim;
+                    store_half4((fold_k ? p.first_k : p.first_v) + off + 4 * lane, kv_new);
+                }
             }
         }
     }
@@ -252,7 +264,7 @@ __device__ __forceinline__ void decode_item(const DecParams &p, const DecItem &i
 #pragma unroll
     for (int dm = 0; dm < 8; dm++) o[dm][0] = o[dm][1] = o[dm][2] = o[dm][3] = 0.f;
 
-    const int new_tile = it.fold ? (it.pos - j0) / kTileKeys : -1;
+    const int new_tile = it.fold ? (it.pos - j0) / kTileKeys + extra : -1;
     const int new_row = it.fold ? (it.pos - j0) % kTileKeys : -1;
 
     for (int t = 0; t < n_tiles; t++) {
@@ -272,8 +284,10 @@ __device__ __forceinline__ void decode_item(const DecParams &p, const DecItem &i
         if (!kTma) cp_async_commit();
 
         const int stage = t % kStages;
-        const int jw = j0 + t * kTileKeys + 16 * warp;  // first key of this warp's 16-row slice
-        if (jw >= j_end) continue;                       // warp-uniform
+        const bool front = kFirst && t < extra;
+        const int tile_end = front ? n_first : j_end;
+        const int jw = (front ? 0 : j0 + (t - extra) * kTileKeys) + 16 * warp;  // first key of this warp's 16-row slice
+        if (jw >= tile_end) continue;                    // warp-uniform
 
         if (t == new_tile && (new_row >> 4) == warp) {
             // the new token's row comes from registers/shared memory, never from the cache slot being written
@@ -297,8 +311,8 @@ __device__ __forceinline__ void decode_item(const DecParams &p, const DecItem &i
                 mma_16816(s, a, bq[k][0], bq[k][1]);
             }
         }
-        if (jw + g >= j_end) s[0] = s[1] = -INFINITY;
-        if (jw + g + 8 >= j_end) s[2] = s[3] = -INFINITY;
+        if (jw + g >= tile_end) s[0] = s[1] = -INFINITY;
+        if (jw + g + 8 >= tile_end) s[2] = s[3] = -INFINITY;
 
         float mx0 = fmaxf(s[0], s[2]), mx1 = fmaxf(s[1], s[3]);
 #pragma unroll
@@ -464,17 +478,17 @@ __device__ __forceinline__ void decode_item(const DecParams &p, const DecItem &i
     }
 }
 
-template <bool kTma>
+template <bool kTma, bool kFirst = false>
 __global__ void __launch_bounds__(kThreads, 2) k_decode_attn(const DecParams p) {
     const DecItem it = p.items[blockIdx.x];
-    decode_item<kStagesWave, kTma>(p, it);
+    decode_item<kStagesWave, kTma, kFirst>(p, it);
 }
 
-template <int kCap, int kStages, bool kTma>
+template <int kCap, int kStages, bool kTma, bool kFirst = false>
 __global__ void __launch_bounds__(kThreads, kStages == kStagesWave ? 2 : 1)
     k_decode_attn_p(const __grid_constant__ DecParams p, const __grid_constant__ DecItemsParam<kCap> ip) {
     const DecItem it = ip.items[blockIdx.x];
-    decode_item<kStages, kTma>(p, it);
+    decode_item<kStages, kTma, kFirst>(p, it);
 }
 
 template <int kStages>
@@ -489,6 +503,8 @@ template <int kCap, int kStages>
 cudaError_t launch_inline(const DecParams &p, const DecItem *host_items, int n_items, cudaStream_t stream) {
     static thread_local DecItemsParam<kCap> ip;  // copied into the launch by the runtime before this returns
     memcpy(ip.items, host_items, sizeof(DecItem) * size_t(n_items));
+    if (p.first_tokens > 0)
+        return launch_pdl(k_decode_attn_p<kCap, kStages, false, true>, n_items, kThreads, smem_bytes<kStages>(), stream, p, ip);
     if (p.k_map) return launch_pdl(k_decode_attn_p<kCap, kStages, true>, n_items, kThreads, smem_bytes<kStages>(), stream, p, ip);
     return launch_pdl(k_decode_attn_p<kCap, kStages, false>, n_items, kThreads, smem_bytes<kStages>(), stream, p, ip);
 }
@@ -551,11 +567,18 @@ cudaError_t decode_kernel_setup() {
     if (e == cudaSuccess) e = allow_smem(k_decode_attn_p<kMaxParamItems, kStagesWave, true>, wave);
     if (e == cudaSuccess) e = allow_smem(k_decode_attn_p<kCapSmall, kStagesDeep, true>, deep);
     if (e == cudaSuccess) e = allow_smem(k_decode_attn_p<kCapMid, kStagesDeep, true>, deep);
+    if (e == cudaSuccess) e = allow_smem(k_decode_attn<false, true>, wave);
+    if (e == cudaSuccess) e = allow_smem(k_decode_attn_p<kCapSmall, kStagesWave, false, true>, wave);
+    if (e == cudaSuccess) e = allow_smem(k_decode_attn_p<kCapMid, kStagesWave, false, true>, wave);
+    if (e == cudaSuccess) e = allow_smem(k_decode_attn_p<kMaxParamItems, kStagesWave, false, true>, wave);
+    if (e == cudaSuccess) e = allow_smem(k_decode_attn_p<kCapSmall, kStagesDeep, false, true>, deep);
+    if (e == cudaSuccess) e = allow_smem(k_decode_attn_p<kCapMid, kStagesDeep, false, true>, deep);
     return e;
 }
 
 cudaError_t launch_decode(const DecParams &p, int n_items, cudaStream_t stream) {
     if (n_items <= 0) return cudaSuccess;
+    if (p.first_tokens > 0) return launch_pdl(k_decode_attn<false, true>, n_items, kThreads, smem_bytes<kStagesWave>(), stream, p);
     if (p.k_map) return launch_pdl(k_decode_attn<true>, n_items, kThreads, smem_bytes<kStagesWave>(), stream, p);
     return launch_pdl(k_decode_attn<false>, n_items, kThreads, smem_bytes<kStagesWave>(), stream, p);
 }

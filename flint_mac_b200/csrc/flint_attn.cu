@@ -42,6 +42,8 @@ struct Layer {
     int kv_lo = 0, kv_hi = 0;  // positions a full layer holds on this device: [kv_lo, kv_hi)
     __half *k = nullptr, *v = nullptr;
     Kv4Cache kv4;  // the cache of a handle that keeps K/V in 4 bits (k and v are null then)
+    int first_tokens = 0;  // ring layers: positions below this one stay visible; a half-precision cache keeps their rows in
+    __half *first_k = nullptr, *first_v = nullptr;  // [max_seqs][4][64][128], a 4-bit one in one more block
     float *q_norm = nullptr, *k_norm = nullptr, *sinks = nullptr;  // device copies
     // projections either side of attention (optional): attn_norm [n_embd] fp32, W_qkv [5120][n_embd] bf16 (q rows,
     // then k rows, then v rows: the packed row of src/metal/fused.metal:211), W_o [n_embd][4096] bf16
@@ -277,7 +279,7 @@ struct flint_attn {
     ~flint_attn() {
         cudaSetDevice(device);
         for (auto &L : layers) {
-            cudaFree(L.k); cudaFree(L.v); cudaFree(L.kv4.blocks); cudaFree(L.q_norm); cudaFree(L.k_norm); cudaFree(L.sinks);
+            cudaFree(L.k); cudaFree(L.v); cudaFree(L.kv4.blocks); cudaFree(L.first_k); cudaFree(L.first_v); cudaFree(L.q_norm); cudaFree(L.k_norm); cudaFree(L.sinks);
             cudaFree(L.attn_norm); cudaFree(L.w_qkv); cudaFree(L.w_o); cudaFree(L.kv_maps);
         }
         cudaFree(dec_err);
@@ -398,6 +400,7 @@ struct flint_attn {
             const size_t nt = std::max<size_t>(size_t(n_subs + n_groups) * 2, 4096);
             CK(cudaMalloc(&tickets, nt * sizeof(int)));
             CK(cudaMemset(tickets, 0, nt * sizeof(int)));
+            CK(cudaDeviceSynchronize());  // (a launch on a non-blocking stream does not wait for the default stream)
             n_tickets = nt;
         }
     }
@@ -546,6 +549,7 @@ struct flint_attn {
         dp.k_map = L.kv_maps;
         dp.v_map = L.kv_maps ? L.kv_maps + 128 : nullptr;
         dp.error_flag = dec_err;
+        dp.first_k = L.first_k; dp.first_v = L.first_v; dp.first_tokens = L.first_tokens;
         if (mode == 2) {
             const size_t rec_bytes = size_t(xchg_n) * kNHead * kPartialDim * sizeof(float);
             const size_t buf_off = 256 + size_t(step & 1) * kv_ranks * rec_bytes + size_t(kv_rank) * rec_bytes;
@@ -592,8 +596,6 @@ flint_attn *flint_attn_open_kv(const flint_attn_config *cfg, const flint_attn_kv
         if (kv_format != FLINT_ATTN_KV_F16 && kv_format != FLINT_ATTN_KV_INT4) throw std::runtime_error("bad kv_format");
         if (first_tokens < 0 || first_tokens > kMaxFirstTokens)
             throw std::runtime_error("first_tokens must be 0 to " + std::to_string(kMaxFirstTokens));
-        if (first_tokens > 0 && kv_format != FLINT_ATTN_KV_INT4)
-            throw std::runtime_error("first tokens are kept by handles with a 4-bit cache only");
         if (kv_format == FLINT_ATTN_KV_INT4 && cfg->kv_ranks > 1)
             throw std::runtime_error("a 4-bit KV cache cannot be sharded by key range");
         if (cfg->n_layers <= 0 || !cfg->layer_is_swa || !cfg->layer_has_rope) throw std::runtime_error("bad layer table");
@@ -665,12 +667,19 @@ flint_attn *flint_attn_open_kv(const flint_attn_config *cfg, const flint_attn_kv
             CK(cudaMalloc(&L.q_norm, kHeadDim * sizeof(float)));
             CK(cudaMalloc(&L.k_norm, kHeadDim * sizeof(float)));
             CK(cudaMalloc(&L.sinks, kNHead * sizeof(float)));
+            L.first_tokens = L.is_swa ? first_tokens : 0;
+            if (L.first_tokens > 0 && kv_format == FLINT_ATTN_KV_F16) {
+                const size_t first_bytes = size_t(cfg->max_seqs) * kNHeadKv * kMaxFirstTokens * kHeadDim * sizeof(__half);
+                CK(cudaMalloc(&L.first_k, first_bytes));
+                CK(cudaMalloc(&L.first_v, first_bytes));
+                CK(cudaMemset(L.first_k, 0, first_bytes));
+                CK(cudaMemset(L.first_v, 0, first_bytes));
+            }
             if (kv_format == FLINT_ATTN_KV_INT4) {
-                L.kv4.first_tokens = L.is_swa ? first_tokens : 0;
+                L.kv4.first_tokens = L.first_tokens;
                 L.kv4.blocks_per_seq = L.is_swa ? kKv4RingBlocks + (first_tokens > 0 ? 1 : 0)
                                                 : (L.n_slots + kKv4BlockKeys - 1) / kKv4BlockKeys;
                 L.kv4.block_mask = L.is_swa ? uint32_t(kKv4RingBlocks - 1) : 0xFFFFFFFFu;
-                if (L.is_swa) L.n_slots += first_tokens;
                 if (L.paged) {
                     L.kv4.block_table = a->table_dev;
                     L.kv4.table_stride = a->pages_per_seq;
@@ -976,6 +985,11 @@ static void prefill_impl(flint_attn *a, int layer, int seq, int n_tok, const voi
         pp.table_len = a->pages_per_seq;
     }
     pp.n_slots = L.n_slots;
+    pp.first_tokens = L.first_tokens;
+    if (L.first_k) {
+        pp.first_k = L.first_k + size_t(seq) * kNHeadKv * kMaxFirstTokens * kHeadDim;
+        pp.first_v = L.first_v + size_t(seq) * kNHeadKv * kMaxFirstTokens * kHeadDim;
+    }
     pp.is_swa = L.is_swa; pp.has_rope = L.has_rope;
     pp.p0 = p0; pp.n_tok = n_tok;
     if (!L.is_swa) {
@@ -1180,7 +1194,7 @@ int32_t flint_attn_check(flint_attn *a, char *err, int32_t err_len) {
 
 int32_t flint_attn_n_slots(const flint_attn *a, int32_t layer) {
     if (layer < 0 || layer >= int(a->layers.size())) return -1;
-    return a->layers[layer].n_slots;
+    return a->layers[layer].n_slots + a->layers[layer].first_tokens;
 }
 
 // Rows of n sequences between a layer's cache and dense arrays [n][4][n_rows][128] on the device.
@@ -1213,7 +1227,9 @@ static void kv_rows(flint_attn *a, int layer, int n, const int32_t *seqs, const 
     }
     KvRowsParams kp{};
     kp.cache = L.kv4;
+    kp.cache.first_tokens = L.first_tokens;
     kp.k_cache = L.k; kp.v_cache = L.v;
+    kp.first_k = L.first_k; kp.first_v = L.first_v;
     if (L.paged) {
         kp.cache.block_table = a->table_dev;
         kp.cache.table_stride = a->pages_per_seq;
@@ -1273,7 +1289,7 @@ static void kv_copy(flint_attn *a, int layer, int seq, int slot0, int n, uint16_
     if (layer < 0 || layer >= int(a->layers.size())) throw std::runtime_error("layer index out of range");
     Layer &L = a->layers[layer];
     if (seq < 0 || seq >= a->max_seqs) throw std::runtime_error("sequence index out of range");
-    if (slot0 < 0 || n < 0 || slot0 + n > L.n_slots) throw std::runtime_error("slot range out of bounds");
+    if (slot0 < 0 || n < 0 || n > L.n_slots + L.first_tokens || slot0 > L.n_slots + L.first_tokens - n) throw std::runtime_error("slot range out of bounds");
     CK(cudaDeviceSynchronize());
     if (L.kv4.blocks) {
         kv4_copy(a, L, seq, slot0, n, k, v, to_host);
@@ -1307,16 +1323,24 @@ static void kv_copy(flint_attn *a, int layer, int seq, int slot0, int n, uint16_
         }
         return;
     }
+    // slots [slot0, slot0 + n) of the cache, and of the first tokens' rows behind it
+    const int n_cache = std::max(0, std::min(n, L.n_slots - slot0)), n_front = n - n_cache, front0 = std::max(0, slot0 - L.n_slots);
     for (int kvh = 0; kvh < kNHeadKv; kvh++) {
-        const size_t doff = ((size_t(seq) * kNHeadKv + kvh) * L.n_slots + slot0) * kHeadDim;
-        const size_t hoff = size_t(kvh) * n * kHeadDim, bytes = size_t(n) * kHeadDim * 2;
-        if (to_host) {
-            CK(cudaMemcpy(k + hoff, L.k + doff, bytes, cudaMemcpyDeviceToHost));
-            CK(cudaMemcpy(v + hoff, L.v + doff, bytes, cudaMemcpyDeviceToHost));
-        } else {
-            CK(cudaMemcpy(L.k + doff, k + hoff, bytes, cudaMemcpyHostToDevice));
-            CK(cudaMemcpy(L.v + doff, v + hoff, bytes, cudaMemcpyHostToDevice));
-        }
+        auto copy = [&](__half *dk, __half *dv, size_t doff, size_t hoff, int rows) {
+            const size_t bytes = size_t(rows) * kHeadDim * 2;
+            if (rows == 0) return;
+            if (to_host) {
+                CK(cudaMemcpy(k + hoff, dk + doff, bytes, cudaMemcpyDeviceToHost));
+                CK(cudaMemcpy(v + hoff, dv + doff, bytes, cudaMemcpyDeviceToHost));
+            } else {
+                CK(cudaMemcpy(dk + doff, k + hoff, bytes, cudaMemcpyHostToDevice));
+                CK(cudaMemcpy(dv + doff, v + hoff, bytes, cudaMemcpyHostToDevice));
+            }
+        };
+        const size_t hoff = size_t(kvh) * n * kHeadDim;
+        copy(L.k, L.v, ((size_t(seq) * kNHeadKv + kvh) * L.n_slots + slot0) * kHeadDim, hoff, n_cache);
+        copy(L.first_k, L.first_v, ((size_t(seq) * kNHeadKv + kvh) * kMaxFirstTokens + front0) * kHeadDim,
+             hoff + size_t(n_cache) * kHeadDim, n_front);
     }
 }
 

@@ -44,6 +44,11 @@ __device__ __forceinline__ long long half_row(const KvRowsParams &p, int seq, in
     return (((long long)seq * kNHeadKv + kvh) * p.n_slots + slot) * kHeadDim;
 }
 
+// Element offset of one of the first tokens' rows beside a half-precision ring.
+__device__ __forceinline__ size_t half_first_row(int seq, int kvh, int pos) {
+    return ((size_t(seq) * kNHeadKv + kvh) * kMaxFirstTokens + pos) * kHeadDim;
+}
+
 // ---- half-precision caches: one warp per (sequence, row, KV head)
 __global__ void __launch_bounds__(256) k_half_store(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs, int n) {
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
@@ -54,8 +59,13 @@ __global__ void __launch_bounds__(256) k_half_store(const KvRowsParams p, const 
     const int kvh = int(w % kNHeadKv), r = int(w / kNHeadKv % p.n_rows), i = int(w / kNHeadKv / p.n_rows);
     // positions r and r + 1024 of one call share a slot of a ring: only the last one of a slot is stored, whatever the order
     // in which the warps run
-    if (p.is_swa && r + kSwaRing < p.n_rows) return;
     const size_t at = size_t(i) * p.seq_stride + size_t(kvh) * p.head_stride + size_t(r) * kHeadDim + 4 * lane;
+    if (p.is_swa && seqs.pos0[i] + r < p.cache.first_tokens) {
+        const size_t to = half_first_row(seqs.seq[i], kvh, seqs.pos0[i] + r) + 4 * lane;
+        row_store4(p.first_k, kDtypeF16, to, row_load4(p.k, p.dtype, at));
+        row_store4(p.first_v, kDtypeF16, to, row_load4(p.v, p.dtype, at));
+    }
+    if (p.is_swa && r + kSwaRing < p.n_rows) return;
     const long long row = half_row(p, seqs.seq[i], kvh, seqs.pos0[i] + r);
     row_store4(p.k_cache, kDtypeF16, size_t(row) + 4 * lane, row_load4(p.k, p.dtype, at));
     row_store4(p.v_cache, kDtypeF16, size_t(row) + 4 * lane, row_load4(p.v, p.dtype, at));
@@ -70,6 +80,12 @@ __global__ void __launch_bounds__(256) k_half_load(const KvRowsParams p, const _
     const int kvh = int(w % kNHeadKv), r = int(w / kNHeadKv % p.n_rows), i = int(w / kNHeadKv / p.n_rows);
     const size_t at = size_t(i) * p.seq_stride + size_t(kvh) * p.head_stride + size_t(r) * kHeadDim + 4 * lane;
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.is_swa && seqs.pos0[i] + r < p.cache.first_tokens) {
+        const size_t from = half_first_row(seqs.seq[i], kvh, seqs.pos0[i] + r) + 4 * lane;
+        row_store4(p.k, p.dtype, at, row_load4(p.first_k, kDtypeF16, from));
+        row_store4(p.v, p.dtype, at, row_load4(p.first_v, kDtypeF16, from));
+        return;
+    }
     const long long row = half_row(p, seqs.seq[i], kvh, seqs.pos0[i] + r);
     row_store4(p.k, p.dtype, at, row < 0 ? zero : row_load4(p.k_cache, kDtypeF16, size_t(row) + 4 * lane));
     row_store4(p.v, p.dtype, at, row < 0 ? zero : row_load4(p.v_cache, kDtypeF16, size_t(row) + 4 * lane));

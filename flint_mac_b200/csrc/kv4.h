@@ -33,7 +33,7 @@ constexpr int kKv4VGroups = kKv4VCodes + kKv4BlockKeys * kKv4RowBytes;
 constexpr int kKv4BlockBytes = kKv4VGroups + kKv4BlockKeys * kKv4Groups * 4;
 static_assert(kKv4BlockBytes == 10240, "block layout");
 constexpr int kKv4RingBlocks = kSwaRing / kKv4BlockKeys;
-constexpr int kMaxFirstTokens = kKv4BlockKeys;
+static_assert(kMaxFirstTokens == kKv4BlockKeys, "one block keeps them");
 
 // Where a layer's blocks are.
 struct Kv4Cache {
@@ -70,6 +70,7 @@ struct KvRowsSeqs {
 struct KvRowsParams {
     Kv4Cache cache;             // 4-bit caches, or
     __half *k_cache = nullptr, *v_cache = nullptr;  // half-precision ones (cache.blocks is null then)
+    __half *first_k = nullptr, *first_v = nullptr;  // their first tokens' rows (cache.first_tokens > 0), [max_seqs][4][64][128]
     int n_slots = 0;
     int is_swa = 0;
     int raw_slots = 0;          // ring layers: pos0 counts slots (the first tokens' rows from kSwaRing on), not positions

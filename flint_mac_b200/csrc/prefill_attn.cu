@@ -149,8 +149,12 @@ struct PrologueArgs {
     int st_rows, st_new;
     Kv4Cache kv4;                // 4-bit cache (the other cache pointers are null), and the sequence's index into it
     int seq;
-    int first_rows;              // rows of the staging in front of the history that take positions [0, first_tokens)
+    int first_tokens;            // ring layers: positions below this one are kept beside the ring too, 4-bit or in
+    __half *first_k, *first_v;   // [4][64][128] of this sequence
+    int first_rows;              // rows of the staging in front of the history that take those positions
 };
+// What the prologue writes: half-precision caches, 4-bit ones, half-precision rings with first tokens beside them.
+enum { kHalfCache = 0, kKv4Cache = 1, kHalfFirst = 2 };
 
 // A lane's share of an input row of 128: dims 4*sub..4*sub+3 and the four 64 further on, the partners of the first
 // four under NEOX RoPE, so that the rotation needs no exchange between lanes.  Two 8-byte loads for bf16 rows, two
@@ -234,7 +238,7 @@ __device__ __forceinline__ void store_row_kv4(const PrologueArgs &a, const float
                                               int sub, bool to_cache) {
     __half *st = is_v ? a.v_st : a.k_st;
     pf_store_half44(st + (size_t(kvh) * a.st_rows + a.st_new + t) * kHeadDim + 4 * sub, x);
-    const bool to_first = a.is_swa && pos < a.kv4.first_tokens;
+    const bool to_first = pos < a.first_tokens;
     if (to_first && a.first_rows > 0) pf_store_half44(st + (size_t(kvh) * a.st_rows + pos) * kHeadDim + 4 * sub, x);
     if (!to_cache && !to_first) return;  // (the same for the whole token)
     unsigned char *block = kv4_block(a.kv4, a.seq, kvh, pos >> 6);
@@ -257,7 +261,7 @@ constexpr int kProRows = 10;  // input rows (heads) per warp: a token's 40 rows 
 // New-token pass: one CTA of four warps per token, each warp with ten of its 40 head rows, two rows per pass (one per
 // half-warp).  All loads of a warp go out before the first row is touched.  The token's 64 (cos, sin) pairs are
 // evaluated once, by the first warp, and shared through shared memory.
-template <bool kBf16, bool kKv4>
+template <bool kBf16, int kCache>
 __device__ __forceinline__ void prologue_rows(const PrologueArgs &a) {
     __shared__ float2 s_cs[kHeadDim / 2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -289,8 +293,8 @@ __device__ __forceinline__ void prologue_rows(const PrologueArgs &a) {
     // On a ring layer tokens t and t + 1024 of one launch share a slot: only the last token that maps to a slot
     // stores there, so the ring's final contents do not depend on the order in which the CTAs run.
     const bool to_cache = mine && (!a.is_swa || t + kSwaRing >= a.n_tok);
-    if (kKv4 && a.first_rows > 0 && t == 0) {  // the products take 64 rows of first tokens: those past the last one count as 0
-        const int from = a.kv4.first_tokens, to = kMaxFirstTokens;
+    if (kCache != kHalfCache && a.first_rows > 0 && t == 0) {  // the products take 64 rows of first tokens: those past the last one count as 0
+        const int from = a.first_tokens, to = kMaxFirstTokens;
         for (int i = threadIdx.x; i < (to - from) * kNHeadKv * (kHeadDim / 8); i += 128) {
             const int c = i % (kHeadDim / 8), r = from + i / (kHeadDim / 8) / kNHeadKv, kvh = i / (kHeadDim / 8) % kNHeadKv;
             const size_t off = (size_t(kvh) * a.st_rows + r) * kHeadDim + 8 * c;
@@ -333,7 +337,7 @@ __device__ __forceinline__ void prologue_rows(const PrologueArgs &a) {
                                               pack_f32x2(k1.z, k1.w)};
             pf_norm_rope8(x, wk, cs, sn, nsn, rope, 1.0f);
         }
-        if (kKv4) {
+        if (kCache == kKv4Cache) {
             store_row_kv4(a, x, pos, t, kvh, !is_k, sub, to_cache);
             continue;
         }
@@ -345,6 +349,10 @@ __device__ __forceinline__ void prologue_rows(const PrologueArgs &a) {
         if (a.k_st) {
             __half *st = is_k ? a.k_st : a.v_st;
             pf_store_half44(st + (size_t(kvh) * a.st_rows + a.st_new + t) * kHeadDim + 4 * sub, x);
+            if (kCache == kHalfFirst && pos < a.first_tokens) {
+                pf_store_half44((is_k ? a.first_k : a.first_v) + (size_t(kvh) * kMaxFirstTokens + pos) * kHeadDim + 4 * sub, x);
+                if (a.first_rows > 0) pf_store_half44(st + (size_t(kvh) * a.st_rows + pos) * kHeadDim + 4 * sub, x);
+            }
         }
     }
 }
@@ -360,13 +368,13 @@ __global__ void __launch_bounds__(256) k_prefill_history(const PrologueArgs a) {
     const int r = int(row / kNHeadKv), kvh = int(row % kNHeadKv);
     const int pos = a.p0 - a.n_hist + r, slot = pos & (kSwaRing - 1);
     const size_t src = (size_t(kvh) * a.n_slots + slot) * kHeadDim + 4 * lane;
-    const size_t dst = (size_t(kvh) * a.st_rows + r) * kHeadDim + 4 * lane;
+    const size_t dst = (size_t(kvh) * a.st_rows + a.first_rows + r) * kHeadDim + 4 * lane;
     *reinterpret_cast<uint2 *>(a.k_st + dst) = *reinterpret_cast<const uint2 *>(a.k_cache + src);
     *reinterpret_cast<uint2 *>(a.v_st + dst) = *reinterpret_cast<const uint2 *>(a.v_cache + src);
 }
 
 // (one kernel per input type: the bf16 one holds half the registers in flight and fits eight CTAs on an SM)
-template <bool kBf16, bool kKv4>
+template <bool kBf16, int kCache>
 __global__ void __launch_bounds__(128, kBf16 ? 8 : 5) k_prefill_prologue(const PrologueArgs a) {
     // the attention kernel of this prefill may be scheduled as soon as SMs come free: it waits for this grid's
     // completion (griddepcontrol.wait) before it reads anything written here
@@ -374,9 +382,9 @@ __global__ void __launch_bounds__(128, kBf16 ? 8 : 5) k_prefill_prologue(const P
     // With a 4-bit cache the kernel in front brings earlier tokens into the staging, and this one may have been scheduled
     // while that still runs (which began only when everything before it had ended).  On a ring layer it reads the slots that
     // are written here; on a full layer the two touch different rows, so they run side by side, and this one ends last.
-    if (kKv4 && a.is_swa) asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    prologue_rows<kBf16, kKv4>(a);
-    if (kKv4 && !a.is_swa) asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    if (kCache == kKv4Cache && a.is_swa) asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    prologue_rows<kBf16, kCache>(a);
+    if (kCache == kKv4Cache && !a.is_swa) asm volatile("griddepcontrol.wait;\n" ::: "memory");
 }
 
 // ------------------------------------------------------------------------------------------------- attention
@@ -1182,7 +1190,7 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
     const bool staged = p.is_swa || kv4;  // K/V rows come from linear staging, not from the cache itself
     const int n_hist = p.is_swa ? (p.p0 < kHist ? p.p0 : kHist) : kv4 ? p.p0 : 0;
     // (only queries past the first 512 + 1 have first tokens in front of their window)
-    const int first_tokens = p.is_swa && kv4 && p.p0 + T - 1 > kHist ? p.kv4.first_tokens : 0;
+    const int first_tokens = p.is_swa && p.p0 + T - 1 > kHist ? p.first_tokens : 0;
     const int first_rows = first_tokens > 0 ? kMaxFirstTokens : 0;
     const int st_new = first_rows + n_hist, st_rows = st_new + T;
     auto up = [](size_t x) { return (x + 1023) / 1024 * 1024; };
@@ -1263,34 +1271,38 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
     pa.kv_lo = p.is_swa ? 0 : p.kv_lo;
     pa.kv_hi = p.is_swa ? 0x7fffffff : p.kv_hi;
     pa.st_rows = st_rows; pa.st_new = st_new;
-    pa.kv4 = p.kv4; pa.seq = p.seq; pa.first_rows = first_rows;
+    pa.kv4 = p.kv4; pa.seq = p.seq;
+    pa.first_tokens = p.is_swa ? p.first_tokens : 0; pa.first_k = p.first_k; pa.first_v = p.first_v; pa.first_rows = first_rows;
     cudaError_t e;
     // The prologue is launched last, directly in front of the attention kernel, so that the two are neighbours on the
     // stream: the attention kernel is launched with programmatic stream serialisation and sets itself up (tensor
     // memory, barriers, work list) on SMs the prologue has already left.
     auto launch_prologue = [&]() -> cudaError_t {
-        if (kv4 && p.p0 > 0) {  // the values of earlier tokens, as the cache holds them
+        // rows of this sequence's cache to the staging, n positions from `from` on to its row `to`
+        auto bring = [&](int from, int n, int to) -> cudaError_t {
             KvRowsParams rows{};
             rows.cache = p.kv4;
+            rows.cache.first_tokens = p.is_swa ? p.first_tokens : 0;
+            rows.k_cache = p.k_cache; rows.v_cache = p.v_cache;  // (half precision: of this sequence already)
+            rows.first_k = p.first_k; rows.first_v = p.first_v;
+            rows.n_slots = p.n_slots;
             rows.is_swa = p.is_swa;
             rows.dtype = kDtypeF16;
             rows.head_stride = (long long)st_rows * kHeadDim;
+            rows.n_rows = n;
+            rows.k = k_st + size_t(to) * kHeadDim;
+            rows.v = v_st + size_t(to) * kHeadDim;
             KvRowsSeqs one{};
-            one.seq[0] = p.seq;
-            one.pos0[0] = p.p0 - n_hist;
-            rows.n_rows = n_hist;
-            rows.k = k_st + size_t(first_rows) * kHeadDim;
-            rows.v = v_st + size_t(first_rows) * kHeadDim;
+            one.seq[0] = kv4 ? p.seq : 0;
+            one.pos0[0] = from;
             if (cudaError_t le = launch_kv_load(rows, one, 1, stream); le != cudaSuccess) return le;
             (*n_launches)++;
-            if (first_tokens > 0) {
-                one.pos0[0] = 0;
-                rows.n_rows = std::min(first_tokens, p.p0);
-                rows.k = k_st;
-                rows.v = v_st;
-                if (cudaError_t le = launch_kv_load(rows, one, 1, stream); le != cudaSuccess) return le;
-                (*n_launches)++;
-            }
+            return cudaSuccess;
+        };
+        if (first_tokens > 0 && p.p0 > 0)
+            if (cudaError_t le = bring(0, std::min(first_tokens, p.p0), 0); le != cudaSuccess) return le;
+        if (kv4 && n_hist > 0) {  // the values of earlier tokens, as the cache holds them
+            if (cudaError_t le = bring(p.p0 - n_hist, n_hist, first_rows); le != cudaSuccess) return le;
         } else if (n_hist > 0) {
             k_prefill_history<<<unsigned((n_hist * kNHeadKv + 7) / 8), 256, 0, stream>>>(pa);
             if (cudaError_t le = cudaGetLastError(); le != cudaSuccess) return le;
@@ -1298,14 +1310,16 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
         }
         const bool bf16 = pa.qkv_dtype == kDtypeBf16;
         if (kv4 && p.p0 > 0) {
-            if (cudaError_t le = bf16 ? launch_pdl(k_prefill_prologue<true, true>, dim3(unsigned(T)), 128, 0, stream, pa)
-                                      : launch_pdl(k_prefill_prologue<false, true>, dim3(unsigned(T)), 128, 0, stream, pa);
+            if (cudaError_t le = bf16 ? launch_pdl(k_prefill_prologue<true, kKv4Cache>, dim3(unsigned(T)), 128, 0, stream, pa)
+                                      : launch_pdl(k_prefill_prologue<false, kKv4Cache>, dim3(unsigned(T)), 128, 0, stream, pa);
                 le != cudaSuccess)
                 return le;
-        } else if (kv4 && bf16) k_prefill_prologue<true, true><<<unsigned(T), 128, 0, stream>>>(pa);
-        else if (kv4) k_prefill_prologue<false, true><<<unsigned(T), 128, 0, stream>>>(pa);
-        else if (bf16) k_prefill_prologue<true, false><<<unsigned(T), 128, 0, stream>>>(pa);
-        else k_prefill_prologue<false, false><<<unsigned(T), 128, 0, stream>>>(pa);
+        } else if (kv4 && bf16) k_prefill_prologue<true, kKv4Cache><<<unsigned(T), 128, 0, stream>>>(pa);
+        else if (kv4) k_prefill_prologue<false, kKv4Cache><<<unsigned(T), 128, 0, stream>>>(pa);
+        else if (pa.first_tokens > 0 && bf16) k_prefill_prologue<true, kHalfFirst><<<unsigned(T), 128, 0, stream>>>(pa);
+        else if (pa.first_tokens > 0) k_prefill_prologue<false, kHalfFirst><<<unsigned(T), 128, 0, stream>>>(pa);
+        else if (bf16) k_prefill_prologue<true, kHalfCache><<<unsigned(T), 128, 0, stream>>>(pa);
+        else k_prefill_prologue<false, kHalfCache><<<unsigned(T), 128, 0, stream>>>(pa);
         if (cudaError_t le = cudaGetLastError(); le != cudaSuccess) return le;
         (*n_launches)++;
         return cudaSuccess;

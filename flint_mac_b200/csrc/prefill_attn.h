@@ -30,10 +30,13 @@ struct PrefillParams {
     float *partial_ml = nullptr;
     // Layer whose cache is held in 4 bits (k_cache, v_cache, block_table above are null then): the K/V rows that the
     // launch attends to are all staged in half precision, what the cache holds of earlier tokens as the values that it
-    // stands for, this call's own rows as they are; those are quantised into the cache on the way.  A sliding-window layer
-    // with kv4.first_tokens > 0 keeps those first tokens visible to every later query.
+    // stands for, this call's own rows as they are; those are quantised into the cache on the way.
     Kv4Cache kv4;
     int seq = 0;         // the sequence's index into kv4
+    // Sliding-window layer: positions below first_tokens stay visible to every later query.  A half-precision cache keeps
+    // their rows here, this sequence's [4][64][128] (a 4-bit one in a block of its own).
+    int first_tokens = 0;
+    __half *first_k = nullptr, *first_v = nullptr;
     int stage_rows = 0;  // rows of K/V staging to allocate for at least (a full layer's context length)
 };
 

@@ -65,7 +65,8 @@ flint_attn *flint_attn_open(const flint_attn_config *cfg, char *err, int32_t err
 void flint_attn_close(flint_attn *a);
 
 /* ---- K/V caches held in 4 bits, first tokens that stay visible ------------------------------------------
- * No counterpart in the reference, which caches K and V in half precision (src/engine.mm:509-511).  flint_attn_open_kv
+ * No counterpart in the reference, which caches K and V in half precision (src/engine.mm:509-511) and shows a
+ * sliding-window layer nothing but its window.  flint_attn_open_kv
  * is flint_attn_open with options (NULL: the defaults, all zero):
  *   kv_format     FLINT_ATTN_KV_INT4: every layer's cache in 4 bits, 80 bytes a row where half precision takes 256.
  *     A row is one token's 128 values of one KV head, K after norm and rotation, rounded to half as in a half-precision
@@ -76,7 +77,7 @@ void flint_attn_close(flint_attn *a);
  *     values that it stands for.  Not with kv_ranks > 1, and no partial records (decode_partial, prefill_partial, xchg).
  *     A prefill behind a cached context on a full layer brings that context into half-precision scratch of the handle
  *     (n_ctx rows, 2 KB each, once for all layers).
- *   first_tokens  0 to 64 (4-bit caches only): on sliding-window layers a query at position p sees, besides the last 513
+ *   first_tokens  0 to 64, with either format: on sliding-window layers a query at position p sees, besides the last 513
  *     positions, positions below first_tokens.  Each sequence keeps those rows outside the ring; n_slots is
  *     1024 + first_tokens there, slots from 1024 on being the first tokens' rows.
  * A 4-bit cache's device memory (flint_attn_kv_dev, which = 0; which = 1 is NULL) is in the library's own block format. */

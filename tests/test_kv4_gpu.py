@@ -1,4 +1,5 @@
-"""4-bit K/V caches through the C ABI: store, load, decode, decode with first tokens, prefill, against 64-bit statements."""
+"""4-bit K/V caches, and first tokens that stay visible beside rings of either format, through the C ABI: store, load, decode,
+prefill, against 64-bit statements."""
 import math
 
 import numpy as np
@@ -21,7 +22,7 @@ def fa():
     ({"kv_format": -1}, "kv_format"),
     ({"kv_format": 1, "first_tokens": 65}, "first_tokens"),
     ({"kv_format": 1, "first_tokens": -1}, "first_tokens"),
-    ({"first_tokens": 4}, "4-bit"),
+    ({"first_tokens": 65}, "first_tokens"),
     ({"kv_format": 1, "kv_ranks": 2}, "sharded"),
 ])
 def test_open_refuses(fa, kw, match):
@@ -81,12 +82,29 @@ def _weights(torch, seed):
     return (1 + 0.1 * torch.randn(128, generator=g), 1 + 0.1 * torch.randn(128, generator=g), torch.randn(32, generator=g))
 
 
-def _open(fa, torch, is_swa, rope, n, n_ctx, seed=3, n_layers=1, **kw):
-    h = fa.Attn([is_swa] * n_layers, [rope] * n_layers, n, n_ctx, kv_format=fa.KV_INT4, **kw)
+def _open(fa, torch, is_swa, rope, n, n_ctx, seed=3, n_layers=1, half=False, **kw):
+    h = fa.Attn([is_swa] * n_layers, [rope] * n_layers, n, n_ctx, kv_format=fa.KV_F16 if half else fa.KV_INT4, **kw)
     w = _weights(torch, seed)
     for il in range(n_layers):
         h.set_layer(il, *(x.numpy() for x in w))
     return h, tuple(x.cuda() for x in w)
+
+
+def _keep(half):
+    """What a cache of the format keeps of half-precision rows, in 64 bits."""
+    return (lambda x: x.double()) if half else ref.kept
+
+
+def _check_keys(got, half_rows, half, what):
+    if half:
+        # Norm and rotation in 32 bits: the scale is off by 2^-22 (a sum of 128 squares over seven levels) and four roundings
+        # of 2^-24, sine and cosine by 2^-23, the products and their sum by three of 2^-24: below 2^-20 of |a| + |b|, the two
+        # values that are turned into each other, which is at most 16 here.  A small result of large ones keeps that error,
+        # 2^-16; beyond it a value lands on the same half or its neighbour.
+        far = (got.double() - half_rows.double()).abs() > 2.0**-10 * half_rows.double().abs() + 2.0**-16
+        assert not bool(far.any()), f"{what}: {int(far.sum())} keys off"
+    else:
+        ref.assert_kept(got, half_rows, what)
 
 
 def _rand(torch, seed, *shape, dtype=None):
@@ -184,18 +202,19 @@ def test_groups_at_the_ends_of_the_range(fa):
 
 
 @gpu
+@pytest.mark.parametrize("half", [False, True])
 @pytest.mark.parametrize("first", [0, 5, 64])
-def test_ring_rows_by_position(fa, first):
+def test_ring_rows_by_position(fa, first, half):
     """A ring keeps the last row of each slot, and the first tokens' rows whatever comes after."""
     import torch
 
     x = _rand(torch, 9, 2, 4, 2500, 128, dtype=torch.float16)
-    with fa.Attn([True], [True], 2, 4000, kv_format=fa.KV_INT4, first_tokens=first) as h:
+    with fa.Attn([True], [True], 2, 4000, kv_format=fa.KV_F16 if half else fa.KV_INT4, first_tokens=first) as h:
         assert h.n_slots(0) == 1024 + first
         h.store_kv_dev(0, [1], [0], 2500, x[0], x[1], fa.F16)
         k, v = torch.empty(2, 4, 1024, 128, device="cuda")
         h.load_kv_dev(0, [1], [2500 - 1024], 1024, k, v, fa.F32)
-        want = ref.kept(x)
+        want = _keep(half)(x)
         assert torch.equal(k, want[0, :, -1024:].float()) and torch.equal(v, want[1, :, -1024:].float())
         if first:
             k, v = torch.empty(2, 4, first, 128, device="cuda")
@@ -260,14 +279,15 @@ def _history(torch, seed, n, rows):
     return k.to(torch.float16), (_rand(torch, seed + 1, n, 4, rows, 128) + 0.25).to(torch.float16)
 
 
-def _decode_want(torch, qkv, w, rope, is_swa, first, positions, k, v):
+def _decode_want(torch, qkv, w, rope, is_swa, first, positions, k, v, half=False):
+    kept = _keep(half)
     outs, rooms, k_new, v_new = [], [], [], []
     for i, p in enumerate(positions):
         at = torch.tensor([p], device="cuda")
         q, kn, vn = ref.split_rows(qkv[i:i + 1], w, at, rope)
         key_at = torch.arange(p + 1, device="cuda")
-        keys = torch.cat((ref.kept(k[i, :, :p]), kn.double().transpose(0, 1)), 1)
-        vals = torch.cat((ref.kept(v[i, :, :p]), vn.double().transpose(0, 1)), 1)
+        keys = torch.cat((kept(k[i, :, :p]), kn.double().transpose(0, 1)), 1)
+        vals = torch.cat((kept(v[i, :, :p]), vn.double().transpose(0, 1)), 1)
         o, r = ref.attend(q, keys, vals, ref.visible(at, key_at, is_swa, first), w[2])
         outs.append(o)
         rooms.append(r)
@@ -281,16 +301,17 @@ POSITIONS = [0, 1, 2, 63, 64, 65, 127, 128, 300, 511, 512, 513, 514, 575, 576, 6
 
 @gpu
 @pytest.mark.parametrize("in_type,out_type", [("float32", "float32"), ("bfloat16", "bfloat16"), ("float32", "bfloat16")])
-@pytest.mark.parametrize("is_swa,rope,paged,first", [
-    (False, False, False, 0), (False, True, True, 0), (True, True, False, 0), (True, True, False, 1), (True, True, False, 4),
-    (True, False, False, 33), (True, True, False, 64)])
-def test_decode(fa, in_type, out_type, is_swa, rope, paged, first):
+@pytest.mark.parametrize("is_swa,rope,paged,first,half", [
+    (False, False, False, 0, False), (False, True, True, 0, False), (True, True, False, 0, False), (True, True, False, 1, False),
+    (True, True, False, 4, False), (True, False, False, 33, False), (True, True, False, 64, False),
+    (True, True, False, 1, True), (True, False, False, 33, True), (True, True, False, 64, True)])
+def test_decode(fa, in_type, out_type, is_swa, rope, paged, first, half):
     import torch
 
     n, dt, ot = len(POSITIONS), getattr(torch, in_type), getattr(torch, out_type)
     k, v = _history(torch, 11, n, 2500)
     qkv = _rand(torch, 13, n, 5120, dtype=dt)
-    h, w = _open(fa, torch, is_swa, rope, n + 1, 2600, kv_pages=41 * n if paged else 0, first_tokens=first)
+    h, w = _open(fa, torch, is_swa, rope, n + 1, 2600, kv_pages=41 * n if paged else 0, first_tokens=first, half=half)
     with h:
         seqs = [(5 * i + 1) % (n + 1) for i in range(n)]
         assert len(set(seqs)) == n
@@ -301,7 +322,7 @@ def test_decode(fa, in_type, out_type, is_swa, rope, paged, first):
         out = torch.full((n + 1, 4096), 777.0, device="cuda", dtype=ot)
         h.decode_dev(0, seqs, qkv, _kind(fa, torch, dt), out, _kind(fa, torch, ot))
         h.check()
-        want, room, k_new, v_new = _decode_want(torch, qkv, w, rope, is_swa, first, POSITIONS, k, v)
+        want, room, k_new, v_new = _decode_want(torch, qkv, w, rope, is_swa, first, POSITIONS, k, v, half)
         ref.assert_near(out[:n], want, room, f"decode {is_swa} {paged} {first}")
         for i, p in enumerate(POSITIONS):  # each sequence by itself, the short ones above all
             ref_rel = float((out[i].double() - want[i].reshape(-1)).norm() / want[i].norm())
@@ -309,13 +330,13 @@ def test_decode(fa, in_type, out_type, is_swa, rope, paged, first):
         assert (out[n] == 777).all()  # rows behind the last sequence
         kb, vb = torch.empty(2, n, 4, 1, 128, device="cuda")
         h.load_kv_dev(0, seqs, POSITIONS, 1, kb, vb, fa.F32)
-        assert torch.equal(vb[:, :, 0], ref.kept(v_new).float())
-        ref.assert_kept(kb[:, :, 0], k_new, "stored keys")
+        assert torch.equal(vb[:, :, 0], _keep(half)(v_new).float())
+        _check_keys(kb[:, :, 0], k_new, half, "stored keys")
         if first:  # new tokens below `first` are among the first tokens' rows too
             for i, p in enumerate(POSITIONS):
                 if p < first:
                     _, v16 = h.read_kv(0, seqs[i], 1024 + p, 1)
-                    assert np.array_equal(v16[:, 0].view(np.float16), ref.kept(v_new[i]).float().to(torch.float16).cpu().numpy())
+                    assert np.array_equal(v16[:, 0].view(np.float16), _keep(half)(v_new[i]).float().to(torch.float16).cpu().numpy())
 
 
 @gpu
@@ -419,15 +440,18 @@ def test_extreme_scales_of_values(fa):
 # ------------------------------------------------------------------------------------------------ prefill
 @gpu
 @pytest.mark.parametrize("in_type,out_type", [("float32", "float32"), ("bfloat16", "bfloat16")])
-@pytest.mark.parametrize("is_swa,first,paged", [(False, 0, False), (False, 0, True), (True, 0, False), (True, 1, False), (True, 20, False), (True, 64, False)])
+@pytest.mark.parametrize("is_swa,first,paged,half", [
+    (False, 0, False, False), (False, 0, True, False), (True, 0, False, False), (True, 1, False, False), (True, 20, False, False),
+    (True, 64, False, False), (True, 3, False, True), (True, 64, False, True)])
 @pytest.mark.parametrize("past,tokens", [(0, 1), (0, 33), (0, 700), (63, 2), (510, 7), (700, 130), (1500, 512), (40, 600), (2000, 1), (2000, 700), (2400, 512), (1900, 1100)])
-def test_prefill(fa, in_type, out_type, is_swa, first, paged, past, tokens):
+def test_prefill(fa, in_type, out_type, is_swa, first, paged, half, past, tokens):
     import torch
 
     dt, ot = getattr(torch, in_type), getattr(torch, out_type)
     k, v = _history(torch, 33, 1, max(past, 1))
     qkv = _rand(torch, 35, tokens, 5120, dtype=dt)
-    h, w = _open(fa, torch, is_swa, True, 3, 3000, kv_pages=60 if paged else 0, first_tokens=first)
+    h, w = _open(fa, torch, is_swa, True, 3, 3000, kv_pages=60 if paged else 0, first_tokens=first, half=half)
+    kept = _keep(half)
     with h:
         if past:
             h.store_kv_dev(0, [1], [0], past, k, v, fa.F16)
@@ -437,32 +461,32 @@ def test_prefill(fa, in_type, out_type, is_swa, first, paged, past, tokens):
         h.check()
         at = torch.arange(past, past + tokens, device="cuda")
         q, kn, vn = ref.split_rows(qkv, w, at, True)
-        keys = torch.cat((ref.kept(k[0, :, :past]), kn.double().transpose(0, 1)), 1)
-        vals = torch.cat((ref.kept(v[0, :, :past]), vn.double().transpose(0, 1)), 1)
+        keys = torch.cat((kept(k[0, :, :past]), kn.double().transpose(0, 1)), 1)
+        vals = torch.cat((kept(v[0, :, :past]), vn.double().transpose(0, 1)), 1)
         want, room = ref.attend(q, keys, vals, ref.visible(at, torch.arange(past + tokens, device="cuda"), is_swa, first), w[2])
         ref.assert_near(out[:tokens], want, room, "prefill")
         assert (out[tokens] == 777).all()
         rows = min(tokens, 1024) if is_swa else tokens
         kb, vb = torch.empty(2, 4, rows, 128, device="cuda")
         h.load_kv_dev(0, [1], [past + tokens - rows], rows, kb, vb, fa.F32)
-        assert torch.equal(vb, ref.kept(vn[-rows:]).transpose(0, 1).float())
-        ref.assert_kept(kb, kn[-rows:].transpose(0, 1), "prefilled keys")
+        assert torch.equal(vb, kept(vn[-rows:]).transpose(0, 1).float())
+        _check_keys(kb, kn[-rows:].transpose(0, 1), half, "prefilled keys")
         for p in range(min(first, past + tokens)):
-            want_v = ref.kept(vn[p - past]) if p >= past else ref.kept(v[0, :, p])
+            want_v = kept(vn[p - past]) if p >= past else kept(v[0, :, p])
             _, v16 = h.read_kv(0, 1, 1024 + p, 1)
             assert np.array_equal(v16[:, 0].view(np.float16), want_v.float().to(torch.float16).cpu().numpy())
 
 
 # ------------------------------------------------------------------------------------------------ together
 @gpu
-@pytest.mark.parametrize("is_swa,first,paged", [(False, 0, True), (True, 4, False)])
-def test_a_conversation(fa, is_swa, first, paged):
+@pytest.mark.parametrize("is_swa,first,paged,half", [(False, 0, True, False), (True, 4, False, False), (True, 4, False, True)])
+def test_a_conversation(fa, is_swa, first, paged, half):
     """Prompt in two chunks, tokens one at a time beside another sequence, a rollback, and on: the cache that the calls
     left is what the next one sees, against the 64-bit statement run over the values that it holds."""
     import torch
 
     P1, P2, N = 590, 100, 40
-    h, w = _open(fa, torch, is_swa, True, 2, 1400, kv_pages=44 if paged else 0, first_tokens=first)
+    h, w = _open(fa, torch, is_swa, True, 2, 1400, kv_pages=44 if paged else 0, first_tokens=first, half=half)
     qkv = _rand(torch, 41, P1 + P2 + N, 5120)
     other = _rand(torch, 43, P1 + P2 + N, 5120)
     with h:
@@ -689,3 +713,29 @@ def test_serving_loop_on_pages(fa):
         # the same values, split and summed in another order: 32-bit sums and the probabilities' half rounding
         err = float((got[i] - alone[i]).norm() / alone[i].norm())
         assert err <= 1e-3, (i, err)
+
+
+@gpu
+def test_windows_of_many_sequences_on_half_precision_rings(fa):
+    """Work lists of every capacity of the half-precision kernel with first tokens, uploaded ones among them."""
+    import torch
+
+    first, n_ctx = 16, 1400
+    for n in (1, 12, 40, 120, 200):  # 4 n items
+        k, v = _history(torch, 81, n, 1100)
+        qkv = _rand(torch, 83, n, 5120)
+        positions = [1100 - (37 * i) % 700 for i in range(n)]
+        h, w = _open(fa, torch, True, True, n, n_ctx, half=True, first_tokens=first)
+        with h:
+            h.store_kv_dev(0, range(n), [0] * n, 1100, k, v, fa.F16)
+            for i, p in enumerate(positions):
+                h.set_pos(i, p)
+            # positions whose ring slots hold later rows are stored again, as a shorter sequence would have left them
+            for i, p in enumerate(positions):
+                h.store_kv_dev(0, [i], [0], p, k[i:i + 1, :, :p].contiguous(), v[i:i + 1, :, :p].contiguous(), fa.F16)
+            out = torch.empty(n, 4096, device="cuda")
+            h.decode_dev(0, range(n), qkv, fa.F32, out, fa.F32)
+            h.check()
+            some = list(range(0, n, max(1, n // 9)))
+            want, room, _, _ = _decode_want(torch, qkv[some], w, True, True, first, [positions[i] for i in some], k[some], v[some], True)
+            ref.assert_near(out[some], want, room, f"{n} windows")
