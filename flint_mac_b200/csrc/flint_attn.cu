@@ -1246,6 +1246,8 @@ static void kv_rows(flint_attn *a, int layer, int n, const int32_t *seqs, const 
         KvRowsSeqs ks;
         memcpy(ks.seq, seqs + i0, size_t(m) * sizeof(int32_t));
         memcpy(ks.pos0, pos0 + i0, size_t(m) * sizeof(int32_t));
+        if (L.paged)
+            for (int i = 0; i < m; i++) ks.held[i] = a->seq_blocks[seqs[i0 + i]];
         kp.k = static_cast<char *>(k) + size_t(i0 / kKvRowsSeqs) * step;
         kp.v = static_cast<char *>(v) + size_t(i0 / kKvRowsSeqs) * step;
         CK(store ? launch_kv_store(kp, ks, m, st) : launch_kv_load(kp, ks, m, st));
@@ -1271,6 +1273,7 @@ static void kv4_copy(flint_attn *a, Layer &L, int seq, int slot0, int n, uint16_
     KvRowsSeqs ks{};
     ks.seq[0] = seq;
     ks.pos0[0] = slot0;
+    if (L.paged) ks.held[0] = a->seq_blocks[seq];
     if (!to_host) {
         CK(cudaMemcpy(dk, k, bytes, cudaMemcpyHostToDevice));
         CK(cudaMemcpy(dv, v, bytes, cudaMemcpyHostToDevice));

@@ -35,8 +35,9 @@ __device__ __forceinline__ void row_store4(void *base, int dtype, size_t elem, f
 }
 
 // Element offset of a position's row in a half-precision cache; -1: no such row here.
-__device__ __forceinline__ long long half_row(const KvRowsParams &p, int seq, int kvh, int pos) {
+__device__ __forceinline__ long long half_row(const KvRowsParams &p, int seq, int kvh, int pos, int held) {
     if (p.cache.block_table) {
+        if ((pos >> 6) >= held) return -1;
         const int page = p.cache.block_table[size_t(seq) * p.cache.table_stride + (pos >> 6)];
         return page < 0 ? -1 : ((long long)(page * kNHeadKv + kvh) * kPageKeys + (pos & (kPageKeys - 1))) * kHeadDim;
     }
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(256) k_half_store(const KvRowsParams p, const 
         row_store4(p.first_v, kDtypeF16, to, row_load4(p.v, p.dtype, at));
     }
     if (p.is_swa && r + kSwaRing < p.n_rows) return;
-    const long long row = half_row(p, seqs.seq[i], kvh, seqs.pos0[i] + r);
+    const long long row = half_row(p, seqs.seq[i], kvh, seqs.pos0[i] + r, seqs.held[i]);
     row_store4(p.k_cache, kDtypeF16, size_t(row) + 4 * lane, row_load4(p.k, p.dtype, at));
     row_store4(p.v_cache, kDtypeF16, size_t(row) + 4 * lane, row_load4(p.v, p.dtype, at));
 }
@@ -86,7 +87,7 @@ __global__ void __launch_bounds__(256) k_half_load(const KvRowsParams p, const _
         row_store4(p.v, p.dtype, at, row_load4(p.first_v, kDtypeF16, from));
         return;
     }
-    const long long row = half_row(p, seqs.seq[i], kvh, seqs.pos0[i] + r);
+    const long long row = half_row(p, seqs.seq[i], kvh, seqs.pos0[i] + r, seqs.held[i]);
     row_store4(p.k, p.dtype, at, row < 0 ? zero : row_load4(p.k_cache, kDtypeF16, size_t(row) + 4 * lane));
     row_store4(p.v, p.dtype, at, row < 0 ? zero : row_load4(p.v_cache, kDtypeF16, size_t(row) + 4 * lane));
 }
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(kRowThreads) k_kv4_load(const KvRowsParams p, 
     const BlockRows b(p, seqs);
     if (b.first >= b.p1) return;
     const int sub = threadIdx.x & 15, r0 = threadIdx.x >> 4, g = sub >> 2;
-    const unsigned char *block = block_of(p, b);
+    const unsigned char *block = p.cache.block_table && b.block >= seqs.held[blockIdx.z] ? nullptr : block_of(p, b);
     const unsigned char *front = p.is_swa && !p.raw_slots && b.first < p.cache.first_tokens ? kv4_first_block(p.cache, b.seq, b.kvh) : nullptr;
     uint32_t kc[kRowSteps], vc[kRowSteps], kg[kRowSteps];
     uint16_t vd[kRowSteps], vl[kRowSteps];

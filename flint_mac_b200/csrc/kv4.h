@@ -66,6 +66,7 @@ cudaError_t launch_decode_kv4(const Dec4Params &p, const Dec4Piece *pieces, int 
 constexpr int kKvRowsSeqs = 128;  // sequences a launch names in its parameters
 struct KvRowsSeqs {
     int32_t seq[kKvRowsSeqs], pos0[kKvRowsSeqs];
+    int32_t held[kKvRowsSeqs];  // paged layers: pages of the sequence (the table's entries past them may be another's by now)
 };
 struct KvRowsParams {
     Kv4Cache cache;             // 4-bit caches, or

@@ -18,6 +18,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <climits>
 #include <cstdlib>
 #include <cstring>
 #include <functional>
@@ -1295,6 +1296,7 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
             KvRowsSeqs one{};
             one.seq[0] = kv4 ? p.seq : 0;
             one.pos0[0] = from;
+            one.held[0] = INT_MAX;  // (the call holds all its pages)
             if (cudaError_t le = launch_kv_load(rows, one, 1, stream); le != cudaSuccess) return le;
             (*n_launches)++;
             return cudaSuccess;

@@ -273,6 +273,29 @@ def test_rows_refused(fa):
         assert not k.any() and not v.any()
 
 
+@gpu
+@pytest.mark.parametrize("half", [False, True])
+def test_pages_given_back_read_as_zeros(fa, half):
+    """Pages a sequence gave back belong to another one: its positions there read as zeros, not as the other's rows."""
+    import torch
+
+    k, v = _history(torch, 91, 2, 640)
+    with fa.Attn([False], [False], 2, 1000, kv_format=fa.KV_F16 if half else fa.KV_INT4, kv_pages=12) as h:
+        h.store_kv_dev(0, [0], [0], 640, k[:1], v[:1], fa.F16)
+        h.seq_release(0)
+        h.store_kv_dev(0, [1], [0], 640, k[1:], v[1:], fa.F16)
+        kb, vb = torch.ones(2, 2, 4, 640, 128, device="cuda")
+        h.load_kv_dev(0, [0, 1], [0, 0], 640, kb, vb, fa.F32)
+        assert not kb[0].any() and not vb[0].any()
+        assert torch.equal(vb[1], _keep(half)(v[1]).float())
+        h.store_kv_dev(0, [0], [30], 70, k[:1, :, :70].contiguous(), v[:1, :, :70].contiguous(), fa.F16)
+        h.load_kv_dev(0, [0, 1], [30, 30], 600, kb2 := torch.ones(2, 4, 600, 128, device="cuda"), torch.empty(2, 4, 600, 128, device="cuda"), fa.F32)
+        assert torch.equal(kb2[0, :, :70], _keep(half)(k[0, :, :70]).float()) and not kb2[0, :, 98:].any()
+        assert torch.equal(kb2[1], kb[1, :, 30:630])
+        k16, v16 = h.read_kv(0, 0, 128, 300)
+        assert not k16.any() and not v16.any()
+
+
 # ------------------------------------------------------------------------------------------------ decode
 def _history(torch, seed, n, rows):
     k = _rand(torch, seed, n, 4, rows, 128) * (0.5 + torch.rand(4, 1, 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)))
