@@ -379,6 +379,30 @@ struct flint_attn {
             if (ring_dev[i] == dev) CK(cudaEventRecord(ring_ev[i], st));
     }
 
+    // Captured calls of handles with a 4-bit cache or first tokens: a graph must find the memory that its launches name.  So
+    // they take no pages (a replay would write the table again, as it is then), and a prefill, whose work list and scratch
+    // are made per call, is not captured.
+    static bool capturing(cudaStream_t st) {
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        CK(cudaStreamIsCapturing(st, &status));
+        return status != cudaStreamCaptureStatusNone;
+    }
+    static void refuse_captured_pages(size_t want, cudaStream_t st) {
+        if (want > 0 && capturing(st))
+            throw std::runtime_error("a captured call takes no KV pages: the sequence must hold them before (flint_attn_store_kv_dev or a decode)");
+    }
+
+    // Scratch and counters of a decode over 4-bit caches, for any batch: they stay where they are, whatever graphs name them
+    // (44 MB).
+    void reserve_kv4_scratch() {
+        scratch_recs = scratch2_recs = size_t(kDec4MaxPieces) * kNHeadKv;
+        n_tickets = 2 * scratch_recs * kGqa;
+        CK(cudaMalloc(&scratch, scratch_recs * kGqa * kRecStride * sizeof(float)));
+        CK(cudaMalloc(&scratch2, scratch2_recs * kGqa * kRecStride * sizeof(float)));
+        CK(cudaMalloc(&tickets, n_tickets * sizeof(int)));
+        CK(cudaMemset(tickets, 0, n_tickets * sizeof(int)));
+    }
+
     void ensure_scratch(int n_records, int n_subs, int n_groups) {
         auto grow = [&](float *&buf, size_t &have, size_t need, size_t floor_recs) {
             if (need <= have) return;
@@ -438,10 +462,8 @@ struct flint_attn {
         for (int i0 = 0; i0 < n;) {
             int n_records = 0, n_warps = 0;
             const int m = plan_decode_kv4(n - i0, seqs + i0, p + i0, kv4_tiles.data() + i0, target_items, kv4_pieces, n_records, n_warps);
-            const int n_recs = n_records * kNHeadKv, n_counts = n_recs * kGqa;
-            ensure_scratch(n_recs, n_recs, 2 * n_counts - n_recs);
             dp.scratch = scratch; dp.scratch2 = scratch2;
-            dp.tickets = tickets; dp.tickets2 = tickets + n_counts;
+            dp.tickets = tickets; dp.tickets2 = tickets + n_tickets / 2;
             // (a CTA of four warps takes half the room of one of eight)
             dp.several_rounds = int(kv4_pieces.size()) * kNHeadKv * n_warps > sm_count * kDec4CtasPerSm * 8;
             dp.tok0 = i0;
@@ -481,6 +503,7 @@ struct flint_attn {
             for (int i = 0; i < n; i++) want += size_t(std::max(0, p[i] / kPageKeys + 1 - seq_blocks[seqs[i]]));
             if (want > free_pages.size())
                 throw std::runtime_error("KV page pool exhausted (" + std::to_string(kv_pages) + " pages of 64 keys)");
+            if (L.kv4.blocks) refuse_captured_pages(want, st);
             for (int i = 0; i < n; i++) ensure_pages(seqs[i], p[i], st);
         }
         if (L.kv4.blocks) {
@@ -639,6 +662,7 @@ flint_attn *flint_attn_open_kv(const flint_attn_config *cfg, const flint_attn_kv
         CK(decode_kernel_setup());
         CK(prefill_kernel_setup());
         CK(decode_kv4_setup());
+        if (kv_format == FLINT_ATTN_KV_INT4) a->reserve_kv4_scratch();
         CK(kv_rows_setup());
         CK(cudaMalloc(&a->dec_err, sizeof(int)));
         CK(cudaMemset(a->dec_err, 0, sizeof(int)));
@@ -960,6 +984,10 @@ static void prefill_impl(flint_attn *a, int layer, int seq, int n_tok, const voi
         (!partial_o && out_dtype != kDtypeF32 && out_dtype != kDtypeBf16))
         throw std::runtime_error("bad dtype");
     if (reinterpret_cast<uintptr_t>(qkv) & 15) throw std::runtime_error("q/k/v rows must start on a 16-byte boundary");
+    const bool one_step = L.kv4.blocks && n_tok == 1;  // (a decode step, below)
+    if ((L.kv4.blocks || L.first_tokens > 0) && !one_step && a->capturing(st))
+        throw std::runtime_error("a prefill cannot be captured into a graph: its work list and scratch are made per call");
+    if (one_step && L.paged) a->refuse_captured_pages(size_t(std::max(0, p0 / kPageKeys + 1 - a->seq_blocks[seq])), st);
     PrefillParams pp{};
     pp.qkv = qkv; pp.out = out;
     pp.qkv_dtype = qkv_dtype; pp.out_dtype = out_dtype;
@@ -969,7 +997,7 @@ static void prefill_impl(flint_attn *a, int layer, int seq, int n_tok, const voi
         pp.seq = seq;
         if (!L.is_swa) pp.stage_rows = a->n_ctx;
         if (L.paged) a->ensure_pages(seq, p0 + n_tok - 1, st);
-        if (n_tok == 1) {  // one token is a decode step, which reads the cache as it is (16000 keys behind: 13 instead of 43 us)
+        if (one_step) {  // one token is a decode step, which reads the cache as it is (16000 keys behind: 13 instead of 43 us)
             const int32_t one_seq = seq, one_pos = p0;
             a->decode_kv4(L, 1, &one_seq, &one_pos, qkv, qkv_dtype, out, out_dtype, st, nullptr);
             return;
@@ -1178,6 +1206,8 @@ int32_t flint_attn_check(flint_attn *a, char *err, int32_t err_len) {
     CK(cudaMemcpy(&flag, a->dec_err, sizeof(int), cudaMemcpyDeviceToHost));
     if (flag) {
         CK(cudaMemset(a->dec_err, 0, sizeof(int)));
+        if (a->tickets) CK(cudaMemset(a->tickets, 0, a->n_tickets * sizeof(int)));  // (a launch that gave up left them counted)
+        CK(cudaDeviceSynchronize());
         throw std::runtime_error("decode kernel reported device error " + std::to_string(flag));
     }
     if (a->xchg) {
@@ -1223,6 +1253,7 @@ static void kv_rows(flint_attn *a, int layer, int n, const int32_t *seqs, const 
         for (int i = 0; i < n; i++) want += size_t(std::max(0, (pos0[i] + n_rows - 1) / kPageKeys + 1 - a->seq_blocks[seqs[i]]));
         if (want > a->free_pages.size())
             throw std::runtime_error("KV page pool exhausted (" + std::to_string(a->kv_pages) + " pages of 64 keys)");
+        a->refuse_captured_pages(want, st);
         for (int i = 0; i < n; i++) a->ensure_pages(seqs[i], pos0[i] + n_rows - 1, st);
     }
     KvRowsParams kp{};

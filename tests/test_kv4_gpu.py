@@ -652,6 +652,81 @@ def test_captured_and_replayed(fa):
 
 
 @gpu
+def test_a_graph_outlives_larger_calls(fa):
+    """Two graphs of one handle, replayed in turn and after larger batches of the handle, give what they gave."""
+    import torch
+
+    n, p = 300, 1500
+    k, v = _history(torch, 93, 1, p)
+    rows = _rand(torch, 95, n, 5120)
+    h, w = _open(fa, torch, False, True, n, 1600)
+    with h:
+        for s in range(n):
+            h.store_kv_dev(0, [s], [0], p, k, v, fa.F16)
+            h.set_pos(s, p)
+        outs = torch.empty(2, 2, 4096, device="cuda")
+        side = torch.cuda.Stream()
+        graphs = []
+        for i in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):  # (no call of the handle before the first capture)
+                h.decode_dev(0, [0, 1][: i + 1], rows, fa.F32, outs[i], fa.F32, torch.cuda.current_stream().cuda_stream)
+            graphs.append(g)
+        big = torch.empty(n, 4096, device="cuda")
+        got = []
+        for _ in range(3):
+            outs.fill_(777)
+            for g in graphs:
+                g.replay()
+            got.append(outs.clone())
+            h.decode_dev(0, range(n), rows, fa.F32, big, fa.F32)
+        torch.cuda.synchronize()
+        h.check()
+        want, room, _, _ = _decode_want(torch, rows[:2], w, True, False, 0, [p, p], k.expand(2, -1, -1, -1), v.expand(2, -1, -1, -1))
+        ref.assert_near(got[0][1], want, room, "graph")
+        ref.assert_near(got[0][0, :1], want[:1], room[:1], "graph")
+        assert (got[0][0, 1] == 777).all()
+        assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
+@gpu
+@pytest.mark.parametrize("half,is_swa,first", [(False, False, 0), (False, True, 0), (True, True, 4)])
+def test_captures_refused(fa, half, is_swa, first):
+    """A prefill is not captured, nor a call that takes pages; the capture goes on and takes the calls that are allowed."""
+    import torch
+
+    paged = not is_swa
+    x, out = _rand(torch, 97, 40, 5120), torch.empty(40, 4096, device="cuda")
+    k, v = _history(torch, 99, 2, 64)
+    h, _ = _open(fa, torch, is_swa, True, 2, 400, kv_pages=6 if paged else 0, first_tokens=first, half=half)
+    with h:
+        h.store_kv_dev(0, [0], [0], 64, k[:1], v[:1], fa.F16)
+        h.set_pos(0, 63)
+        h.set_pos(1, 0)
+        h.decode_dev(0, [0], x, fa.F32, out, fa.F32)
+        want = out[0].clone()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            st = torch.cuda.current_stream().cuda_stream
+            with pytest.raises(fa.FlintAttnError, match="captured"):
+                h.prefill_dev(0, 0, 40, x, fa.F32, out, fa.F32, st)
+            if paged:
+                for call in (lambda: h.decode_dev(0, [0, 1], x, fa.F32, out, fa.F32, st),
+                             lambda: h.prefill_dev(0, 1, 1, x, fa.F32, out, fa.F32, st),
+                             lambda: h.store_kv_dev(0, [0], [60], 10, k, v, fa.F16, st)):
+                    with pytest.raises(fa.FlintAttnError, match="captured"):
+                        call()
+                assert h.pages_free() == 5
+            h.decode_dev(0, [0], x, fa.F32, out, fa.F32, st)
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        h.check()
+        assert torch.equal(out[0], want) and not out[1:].any()
+
+
+@gpu
 def test_positions_past_32_bits_of_bytes(fa):
     """A cache of more than 4 GB: block addresses of the last sequence lie beyond 32 bits."""
     import torch
