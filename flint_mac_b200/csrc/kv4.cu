@@ -81,6 +81,14 @@ __global__ void __launch_bounds__(256) k_half_load(const KvRowsParams p, const _
     const int kvh = int(w % kNHeadKv), r = int(w / kNHeadKv % p.n_rows), i = int(w / kNHeadKv / p.n_rows);
     const size_t at = size_t(i) * p.seq_stride + size_t(kvh) * p.head_stride + size_t(r) * kHeadDim + 4 * lane;
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.staging) {  // first tokens of a prefill
+        const size_t from = half_first_row(seqs.seq[i], kvh, seqs.pos0[i] + r) + 4 * lane;
+        uint2 k = *reinterpret_cast<const uint2 *>(p.first_k + from), v = *reinterpret_cast<const uint2 *>(p.first_v + from);
+        half_row_staged(k, v);
+        *reinterpret_cast<uint2 *>(static_cast<__half *>(p.k) + at) = k;
+        *reinterpret_cast<uint2 *>(static_cast<__half *>(p.v) + at) = v;
+        return;
+    }
     if (p.is_swa && seqs.pos0[i] + r < p.cache.first_tokens) {
         const size_t from = half_first_row(seqs.seq[i], kvh, seqs.pos0[i] + r) + 4 * lane;
         row_store4(p.k, p.dtype, at, row_load4(p.first_k, kDtypeF16, from));
@@ -238,7 +246,8 @@ __global__ void __launch_bounds__(kRowThreads, kType == kDtypeF32 ? 4 : 6) k_kv4
     }
 }
 
-template <int kType>
+// kStaging: see KvRowsParams; values that half precision does not reach are its largest there, as the products need them.
+template <int kType, bool kStaging = false>
 __global__ void __launch_bounds__(kRowThreads) k_kv4_load(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs) {
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // (after the wait: see the prefill prologue)
@@ -265,16 +274,19 @@ __global__ void __launch_bounds__(kRowThreads) k_kv4_load(const KvRowsParams p, 
 #pragma unroll
     for (int i = 0; i < kRowSteps; i++) {
         const int r = r0 + 16 * i;
+        const bool odd = kStaging && (vd[i] & 0x7c00u) == 0x7c00u;  // (the row's sixteen lanes are half a warp)
+        const bool bad = kStaging && (__ballot_sync(0xffffffffu, odd) >> (threadIdx.x & 16) & 0xffffu) != 0;
         if (!b.has(r)) continue;
         const size_t at = b.base + size_t(b.first + r) * kHeadDim + 8 * sub;
         float x[8];
+        auto reach = [](float y) { return kStaging && fabsf(y) > 65504.f ? copysignf(65504.f, y) : y; };
         const float2 dl = __half22float2(*reinterpret_cast<const __half2 *>(&kg[i]));
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = fmaf(float((kc[i] >> (4 * j)) & 15u), dl.x, dl.y);
+        for (int j = 0; j < 8; j++) x[j] = bad ? __uint_as_float(0x7fc00000u) : reach(fmaf(float((kc[i] >> (4 * j)) & 15u), dl.x, dl.y));
         Eight<kType>::store(p.k, at, x);
         const float d = __half2float(__ushort_as_half(vd[i])), lo = __half2float(__ushort_as_half(vl[i]));
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = fmaf(float((vc[i] >> (4 * j)) & 15u), d, lo);
+        for (int j = 0; j < 8; j++) x[j] = odd ? 0.f : reach(fmaf(float((vc[i] >> (4 * j)) & 15u), d, lo));
         Eight<kType>::store(p.v, at, x);
     }
 }
@@ -300,6 +312,7 @@ cudaError_t kv_rows_setup() {
     if (e == cudaSuccess) e = max_shared(k_kv4_load<kDtypeF32>);
     if (e == cudaSuccess) e = max_shared(k_kv4_load<kDtypeBf16>);
     if (e == cudaSuccess) e = max_shared(k_kv4_load<kDtypeF16>);
+    if (e == cudaSuccess) e = max_shared(k_kv4_load<kDtypeF16, true>);
     return e;
 }
 
@@ -318,6 +331,7 @@ cudaError_t launch_kv_load(const KvRowsParams &p, const KvRowsSeqs &seqs, int n,
     const dim3 grid = block_grid(p, n, 1);
     if (p.dtype == kDtypeF32) return launch_pdl(k_kv4_load<kDtypeF32>, grid, kRowThreads, 0, stream, p, seqs);
     if (p.dtype == kDtypeBf16) return launch_pdl(k_kv4_load<kDtypeBf16>, grid, kRowThreads, 0, stream, p, seqs);
+    if (p.staging) return launch_pdl(k_kv4_load<kDtypeF16, true>, grid, kRowThreads, 0, stream, p, seqs);
     return launch_pdl(k_kv4_load<kDtypeF16>, grid, kRowThreads, 0, stream, p, seqs);
 }
 

@@ -24,6 +24,18 @@ __device__ __forceinline__ int kv4_chunk(int row, int ch) { return row * kKv4Row
 __device__ __forceinline__ int kv4_k_group(int row, int g) { return kKv4KGroups + row * 16 + g * 4; }
 __device__ __forceinline__ int kv4_v_group(int row, int g) { return kKv4VGroups + (row >> 1) * 32 + g * 4 + (row & 1) * 2; }
 
+// A half-precision row's K and V, four values of each a lane, for the products of a prefill (see its prologue): infinities and
+// NaN of V become zeros, and the K row beside them NaN.
+__device__ __forceinline__ void half_row_staged(uint2 &k, uint2 &v) {
+    auto odd = [](uint32_t w) {  // 0xffff in each half that is an infinity or a NaN
+        return ((w & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((w & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
+    };
+    const uint32_t a = odd(v.x), b = odd(v.y);
+    if (!__any_sync(0xffffffffu, (a | b) != 0)) return;
+    v = make_uint2(v.x & ~a, v.y & ~b);
+    k = make_uint2(0x7fff7fffu, 0x7fff7fffu);
+}
+
 // d and lo of a group, packed {d, lo}, and 1 / d, from its least and largest value (halves; NaN if a value was one).  A group
 // that holds an infinity or a NaN gets d = NaN.  The quotient by 15, like those by d below, is the product with the
 // reciprocal and one correction step, which rounds it as a division does (Markstein 1990).

@@ -76,6 +76,7 @@ struct KvRowsParams {
     int is_swa = 0;
     int raw_slots = 0;          // ring layers: pos0 counts slots (the first tokens' rows from kSwaRing on), not positions
     int dtype = 0;              // of k and v
+    int staging = 0;            // load: V without infinities and NaN, K rows beside those NaN, for the products of a prefill
     int n_rows = 0;
     long long seq_stride = 0, head_stride = 0;  // elements of k and v
     void *k = nullptr, *v = nullptr;

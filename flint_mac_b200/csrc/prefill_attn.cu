@@ -90,6 +90,7 @@ struct PfArgs {
     // [0, first_tokens), the window's rows follow.
     int first_tokens, first_rows;  // (first_rows: 64)
 };
+static_assert(kNHead + kNHeadKv == 36 && kNHead == 32, "the prologue's warp 3 has a token's K and V rows");
 static_assert(kMaxFirstTokens == 64, "half a key tile");
 
 // What a query sees, beyond the causal limit; the attention kernel is compiled for each.
@@ -232,15 +233,26 @@ __device__ __forceinline__ void pf_norm_rope8(float (&x)[8], const unsigned long
     for (int i = 0; i < 4; i++) unpack_f32x2(v[i], x[2 * i], x[2 * i + 1]);
 }
 
+// Rows in the staging of a handle with a 4-bit cache or first tokens.  The products take every row of a tile, also for queries
+// that do not see it, and 0 times an infinity or a NaN is a NaN: so the staging has zeros in place of such values of V, and
+// the K row of that token (`bad`) is NaN, which reaches the scores of the queries that see it, and those only.
+__device__ __forceinline__ bool pf_not_finite(float x) { return !(fabsf(x) < 65520.f); }  // (as a half)
+__device__ __forceinline__ void pf_store_staged(__half *dst, const float (&x)[8], bool is_v, bool bad) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = is_v ? (pf_not_finite(x[i]) ? 0.f : x[i]) : bad ? __uint_as_float(0x7fc00000u) : x[i];
+    pf_store_half44(dst, y);
+}
+
 // A new token's K or V row with a 4-bit cache: half-precision values to the staging, codes to the cache.  The lane's eight
 // values belong to two groups: dims 4 sub .. + 3 to group sub / 8, the four 64 further on to the group two after it; each
 // group lives in eight neighbouring lanes.
 __device__ __forceinline__ void store_row_kv4(const PrologueArgs &a, const float (&x)[8], int pos, int t, int kvh, bool is_v,
-                                              int sub, bool to_cache) {
+                                              int sub, bool to_cache, bool bad) {
     __half *st = is_v ? a.v_st : a.k_st;
-    pf_store_half44(st + (size_t(kvh) * a.st_rows + a.st_new + t) * kHeadDim + 4 * sub, x);
+    pf_store_staged(st + (size_t(kvh) * a.st_rows + a.st_new + t) * kHeadDim + 4 * sub, x, is_v, bad);
     const bool to_first = pos < a.first_tokens;
-    if (to_first && a.first_rows > 0) pf_store_half44(st + (size_t(kvh) * a.st_rows + pos) * kHeadDim + 4 * sub, x);
+    if (to_first && a.first_rows > 0) pf_store_staged(st + (size_t(kvh) * a.st_rows + pos) * kHeadDim + 4 * sub, x, is_v, bad);
     if (!to_cache && !to_first) return;  // (the same for the whole token)
     unsigned char *block = kv4_block(a.kv4, a.seq, kvh, pos >> 6);
 #pragma unroll
@@ -321,6 +333,15 @@ __device__ __forceinline__ void prologue_rows(const PrologueArgs &a) {
 
 #pragma unroll
     for (int i = 0; i < kProRows / 2; i++) {
+        bool bad = false;  // (the V rows of a K row's token lie two passes on, in the same lanes)
+        if (kCache != kHalfCache && (i == 1 || i == 2) && warp == 3) {
+            float y[8];
+            raw[i + 2].unpack(y);
+            bool odd = false;
+#pragma unroll
+            for (int j = 0; j < 8; j++) odd = odd || pf_not_finite(y[j]);
+            bad = (__ballot_sync(0xffffffffu, odd) >> (16 * half) & 0xffffu) != 0;
+        }
         const int row = warp * kProRows + 2 * i + half;  // 0-31 q heads, 32-35 k heads, 36-39 v heads
         float x[8];
         raw[i].unpack(x);
@@ -339,7 +360,7 @@ __device__ __forceinline__ void prologue_rows(const PrologueArgs &a) {
             pf_norm_rope8(x, wk, cs, sn, nsn, rope, 1.0f);
         }
         if (kCache == kKv4Cache) {
-            store_row_kv4(a, x, pos, t, kvh, !is_k, sub, to_cache);
+            store_row_kv4(a, x, pos, t, kvh, !is_k, sub, to_cache, bad);
             continue;
         }
         if (to_cache) {
@@ -347,13 +368,15 @@ __device__ __forceinline__ void prologue_rows(const PrologueArgs &a) {
             const size_t crow = a.block_table ? (page * kNHeadKv + kvh) * 64 + (pos & 63) : size_t(kvh) * a.n_slots + slot;
             pf_store_half44(cache + crow * kHeadDim + 4 * sub, x);
         }
-        if (a.k_st) {
+        if (kCache == kHalfFirst) {
             __half *st = is_k ? a.k_st : a.v_st;
-            pf_store_half44(st + (size_t(kvh) * a.st_rows + a.st_new + t) * kHeadDim + 4 * sub, x);
-            if (kCache == kHalfFirst && pos < a.first_tokens) {
+            pf_store_staged(st + (size_t(kvh) * a.st_rows + a.st_new + t) * kHeadDim + 4 * sub, x, !is_k, bad);
+            if (pos < a.first_tokens) {
                 pf_store_half44((is_k ? a.first_k : a.first_v) + (size_t(kvh) * kMaxFirstTokens + pos) * kHeadDim + 4 * sub, x);
-                if (a.first_rows > 0) pf_store_half44(st + (size_t(kvh) * a.st_rows + pos) * kHeadDim + 4 * sub, x);
+                if (a.first_rows > 0) pf_store_staged(st + (size_t(kvh) * a.st_rows + pos) * kHeadDim + 4 * sub, x, !is_k, bad);
             }
+        } else if (a.k_st) {
+            pf_store_half44((is_k ? a.k_st : a.v_st) + (size_t(kvh) * a.st_rows + a.st_new + t) * kHeadDim + 4 * sub, x);
         }
     }
 }
@@ -370,8 +393,10 @@ __global__ void __launch_bounds__(256) k_prefill_history(const PrologueArgs a) {
     const int pos = a.p0 - a.n_hist + r, slot = pos & (kSwaRing - 1);
     const size_t src = (size_t(kvh) * a.n_slots + slot) * kHeadDim + 4 * lane;
     const size_t dst = (size_t(kvh) * a.st_rows + a.first_rows + r) * kHeadDim + 4 * lane;
-    *reinterpret_cast<uint2 *>(a.k_st + dst) = *reinterpret_cast<const uint2 *>(a.k_cache + src);
-    *reinterpret_cast<uint2 *>(a.v_st + dst) = *reinterpret_cast<const uint2 *>(a.v_cache + src);
+    uint2 k = *reinterpret_cast<const uint2 *>(a.k_cache + src), v = *reinterpret_cast<const uint2 *>(a.v_cache + src);
+    if (a.first_tokens > 0) half_row_staged(k, v);
+    *reinterpret_cast<uint2 *>(a.k_st + dst) = k;
+    *reinterpret_cast<uint2 *>(a.v_st + dst) = v;
 }
 
 // (one kernel per input type: the bf16 one holds half the registers in flight and fits eight CTAs on an SM)
@@ -1289,6 +1314,7 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
             rows.n_slots = p.n_slots;
             rows.is_swa = p.is_swa;
             rows.dtype = kDtypeF16;
+            rows.staging = 1;
             rows.head_stride = (long long)st_rows * kHeadDim;
             rows.n_rows = n;
             rows.k = k_st + size_t(to) * kHeadDim;

@@ -500,6 +500,51 @@ def test_prefill(fa, in_type, out_type, is_swa, first, paged, half, past, tokens
             assert np.array_equal(v16[:, 0].view(np.float16), want_v.float().to(torch.float16).cpu().numpy())
 
 
+@gpu
+@pytest.mark.parametrize("in_type", ["float32", "bfloat16"])
+@pytest.mark.parametrize("is_swa,first,half", [(False, 0, False), (True, 0, False), (True, 4, False), (True, 64, True)])
+@pytest.mark.parametrize("past,tokens", [(600, 300), (0, 700), (20, 560), (1400, 40)])
+def test_prefill_keeps_infinities_from_queries_that_do_not_see_them(fa, in_type, is_swa, first, half, past, tokens):
+    """Values that are not finite, in padding behind the prompt, in one row of it, in the window's history and in a first
+    token: queries that see one get NaN in its heads, all others what they get without them."""
+    import torch
+
+    dt = getattr(torch, in_type)
+    k, v = _history(torch, 45, 1, max(past, 1))
+    qkv = _rand(torch, 47, tokens, 5120, dtype=dt)
+    bad_at = {head: set() for head in range(4)}
+    k2, v2, qkv2 = k.clone(), v.clone(), qkv.clone()
+    mid, pad = tokens // 3, tokens - 10
+    qkv2[mid, 4608 + 128 + 77] = math.inf  # V of KV head 1, one value
+    bad_at[1].add(past + mid)
+    qkv2[pad:] = math.nan
+    for head in range(4):
+        bad_at[head].update(range(past + pad, past + tokens))
+    if past > 512:
+        v2[0, 0, past - 500, 5] = -math.inf
+        bad_at[0].add(past - 500)
+    if first and past:
+        v2[0, 3, 1, 127] = math.nan
+        bad_at[3].add(1)
+    outs = []
+    for kk, vv, x in ((k, v, qkv), (k2, v2, qkv2)):
+        h, _ = _open(fa, torch, is_swa, True, 1, past + tokens, first_tokens=first, half=half)
+        with h:
+            if past:
+                h.store_kv_dev(0, [0], [0], past, kk, vv, fa.F16)
+            h.set_pos(0, past)
+            out = torch.empty(tokens, 4096, device="cuda")
+            h.prefill_dev(0, 0, tokens, x, _kind(fa, torch, dt), out, fa.F32)
+            h.check()
+            outs.append(out.view(tokens, 4, 1024))
+    at, keys = torch.arange(past, past + tokens, device="cuda"), torch.arange(past + tokens, device="cuda")
+    sees = ref.visible(at, keys, is_swa, first)
+    for head in range(4):
+        hit = sees[:, sorted(bad_at[head])].any(1)
+        assert torch.isnan(outs[1][hit, head]).all(), head
+        assert torch.equal(outs[1][~hit, head], outs[0][~hit, head]), head
+
+
 # ------------------------------------------------------------------------------------------------ together
 @gpu
 @pytest.mark.parametrize("is_swa,first,paged,half", [(False, 0, True, False), (True, 4, False, False), (True, 4, False, True)])
