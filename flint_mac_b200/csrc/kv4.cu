@@ -121,6 +121,7 @@ struct Eight<kDtypeF32> {
     __device__ __forceinline__ uint4 get() const {
         return make_uint4(pack_half2(a.x, a.y), pack_half2(a.z, a.w), pack_half2(b.x, b.y), pack_half2(b.z, b.w));
     }
+    template <bool>
     static __device__ __forceinline__ void store(void *base, size_t elem, const float (&x)[8]) {
         float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(base) + elem);
         __stcs(p, make_float4(x[0], x[1], x[2], x[3]));
@@ -137,6 +138,7 @@ struct Eight<kDtypeBf16> {
         auto half2_of = [](uint32_t w) { return pack_half2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); };
         return make_uint4(half2_of(a.x), half2_of(a.y), half2_of(a.z), half2_of(a.w));
     }
+    template <bool>
     static __device__ __forceinline__ void store(void *base, size_t elem, const float (&x)[8]) {
         uint32_t w[4];
 #pragma unroll
@@ -154,9 +156,16 @@ struct Eight<kDtypeF16> {
         a = __ldcs(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + elem));
     }
     __device__ __forceinline__ uint4 get() const { return a; }
+    // kLimit: values past the largest finite one become it (lo + 15 d can be, by half a step of d, where the row reaches it)
+    template <bool kLimit>
     static __device__ __forceinline__ void store(void *base, size_t elem, const float (&x)[8]) {
-        __stcs(reinterpret_cast<uint4 *>(static_cast<uint16_t *>(base) + elem),
-               make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7])));
+        auto pack = [](float a, float b) {
+            if (!kLimit) return pack_half2(a, b);
+            uint32_t h;
+            asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;\n" : "=r"(h) : "f"(b), "f"(a));
+            return h;
+        };
+        __stcs(reinterpret_cast<uint4 *>(static_cast<uint16_t *>(base) + elem), make_uint4(pack(x[0], x[1]), pack(x[2], x[3]), pack(x[4], x[5]), pack(x[6], x[7])));
     }
 };
 
@@ -246,7 +255,7 @@ __global__ void __launch_bounds__(kRowThreads, kType == kDtypeF32 ? 4 : 6) k_kv4
     }
 }
 
-// kStaging: see KvRowsParams; values that half precision does not reach are its largest there, as the products need them.
+// kStaging: see KvRowsParams.
 template <int kType, bool kStaging = false>
 __global__ void __launch_bounds__(kRowThreads) k_kv4_load(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs) {
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
@@ -279,15 +288,15 @@ __global__ void __launch_bounds__(kRowThreads) k_kv4_load(const KvRowsParams p, 
         if (!b.has(r)) continue;
         const size_t at = b.base + size_t(b.first + r) * kHeadDim + 8 * sub;
         float x[8];
-        auto reach = [](float y) { return kStaging && fabsf(y) > 65504.f ? copysignf(65504.f, y) : y; };
         const float2 dl = __half22float2(*reinterpret_cast<const __half2 *>(&kg[i]));
+        const float k_lo = bad ? __uint_as_float(0x7fc00000u) : dl.y;
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = bad ? __uint_as_float(0x7fc00000u) : reach(fmaf(float((kc[i] >> (4 * j)) & 15u), dl.x, dl.y));
-        Eight<kType>::store(p.k, at, x);
-        const float d = __half2float(__ushort_as_half(vd[i])), lo = __half2float(__ushort_as_half(vl[i]));
+        for (int j = 0; j < 8; j++) x[j] = fmaf(float((kc[i] >> (4 * j)) & 15u), dl.x, k_lo);
+        Eight<kType>::template store<kStaging>(p.k, at, x);
+        const float d = odd ? 0.f : __half2float(__ushort_as_half(vd[i])), lo = odd ? 0.f : __half2float(__ushort_as_half(vl[i]));
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = odd ? 0.f : reach(fmaf(float((vc[i] >> (4 * j)) & 15u), d, lo));
-        Eight<kType>::store(p.v, at, x);
+        for (int j = 0; j < 8; j++) x[j] = fmaf(float((vc[i] >> (4 * j)) & 15u), d, lo);
+        Eight<kType>::template store<kStaging>(p.v, at, x);
     }
 }
 

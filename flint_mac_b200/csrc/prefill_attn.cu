@@ -233,32 +233,37 @@ __device__ __forceinline__ void pf_norm_rope8(float (&x)[8], const unsigned long
     for (int i = 0; i < 4; i++) unpack_f32x2(v[i], x[2 * i], x[2 * i + 1]);
 }
 
-// Rows in the staging of a handle with a 4-bit cache or first tokens.  The products take every row of a tile, also for queries
-// that do not see it, and 0 times an infinity or a NaN is a NaN: so the staging has zeros in place of such values of V, and
-// the K row of that token (`bad`) is NaN, which reaches the scores of the queries that see it, and those only.
-__device__ __forceinline__ bool pf_not_finite(float x) { return !(fabsf(x) < 65520.f); }  // (as a half)
-__device__ __forceinline__ void pf_store_staged(__half *dst, const float (&x)[8], bool is_v, bool bad) {
-    float y[8];
+// A lane's eight values of a row as halves: dims 4 sub .. + 3, then the four 64 further on.
+struct ProHalf {
+    uint32_t w[4];
+    __device__ __forceinline__ explicit ProHalf(const float (&x)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) y[i] = is_v ? (pf_not_finite(x[i]) ? 0.f : x[i]) : bad ? __uint_as_float(0x7fc00000u) : x[i];
-    pf_store_half44(dst, y);
-}
+        for (int i = 0; i < 4; i++) w[i] = pack_half2(x[2 * i], x[2 * i + 1]);
+    }
+    __device__ __forceinline__ void set(uint32_t v) { w[0] = w[1] = w[2] = w[3] = v; }
+    __device__ __forceinline__ void store(__half *dst) const {
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2 *>(dst + kHeadDim / 2) = make_uint2(w[2], w[3]);
+    }
+    __device__ __forceinline__ bool finite() const {
+        auto mag = [&](int i) { return __habs2(*reinterpret_cast<const __half2 *>(&w[i])); };
+        const __half2 m = __hmax2_nan(__hmax2_nan(mag(0), mag(1)), __hmax2_nan(mag(2), mag(3)));
+        const uint32_t u = *reinterpret_cast<const uint32_t *>(&m);
+        return (u & 0x7c00u) != 0x7c00u && (u & 0x7c000000u) != 0x7c000000u;
+    }
+};
 
-// A new token's K or V row with a 4-bit cache: half-precision values to the staging, codes to the cache.  The lane's eight
-// values belong to two groups: dims 4 sub .. + 3 to group sub / 8, the four 64 further on to the group two after it; each
-// group lives in eight neighbouring lanes.
-__device__ __forceinline__ void store_row_kv4(const PrologueArgs &a, const float (&x)[8], int pos, int t, int kvh, bool is_v,
-                                              int sub, bool to_cache, bool bad) {
-    __half *st = is_v ? a.v_st : a.k_st;
-    pf_store_staged(st + (size_t(kvh) * a.st_rows + a.st_new + t) * kHeadDim + 4 * sub, x, is_v, bad);
+// A new token's K or V row to a 4-bit cache.  The lane's eight values belong to two groups: dims 4 sub .. + 3 to group
+// sub / 8, the four 64 further on to the group two after it; each group lives in eight neighbouring lanes.
+__device__ __forceinline__ void store_row_kv4(const PrologueArgs &a, const ProHalf &x, int pos, int kvh, bool is_v, int sub,
+                                              bool to_cache) {
     const bool to_first = pos < a.first_tokens;
-    if (to_first && a.first_rows > 0) pf_store_staged(st + (size_t(kvh) * a.st_rows + pos) * kHeadDim + 4 * sub, x, is_v, bad);
     if (!to_cache && !to_first) return;  // (the same for the whole token)
     unsigned char *block = kv4_block(a.kv4, a.seq, kvh, pos >> 6);
 #pragma unroll
     for (int hi = 0; hi < 2; hi++) {
         uint32_t dl;
-        const uint32_t codes = kv4_quantise4(make_uint2(pack_half2(x[4 * hi], x[4 * hi + 1]), pack_half2(x[4 * hi + 2], x[4 * hi + 3])), dl);
+        const uint32_t codes = kv4_quantise4(make_uint2(x.w[2 * hi], x.w[2 * hi + 1]), dl);
         const int g = (sub >> 3) + 2 * hi;
         auto put = [&](unsigned char *blk, int row) {
             *reinterpret_cast<uint16_t *>(blk + (is_v ? kKv4VCodes : kKv4KCodes) + kv4_chunk(row, g) + (sub & 7) * 2) = uint16_t(codes);
@@ -331,17 +336,14 @@ __device__ __forceinline__ void prologue_rows(const PrologueArgs &a) {
         }
     }
 
+    // Staging of a handle with a 4-bit cache or first tokens: the products take every row of a tile, also for queries that do
+    // not see it, and 0 times an infinity or a NaN is a NaN.  So V has zeros in place of such values, and the K row beside
+    // them is NaN, which reaches the scores of the queries that see it, and those only.  (A token's K and V rows of a KV head
+    // are in the same lanes, two passes apart: V goes first.)
+    bool bad[2] = {false, false};
 #pragma unroll
-    for (int i = 0; i < kProRows / 2; i++) {
-        bool bad = false;  // (the V rows of a K row's token lie two passes on, in the same lanes)
-        if (kCache != kHalfCache && (i == 1 || i == 2) && warp == 3) {
-            float y[8];
-            raw[i + 2].unpack(y);
-            bool odd = false;
-#pragma unroll
-            for (int j = 0; j < 8; j++) odd = odd || pf_not_finite(y[j]);
-            bad = (__ballot_sync(0xffffffffu, odd) >> (16 * half) & 0xffffu) != 0;
-        }
+    for (int n = 0; n < kProRows / 2; n++) {
+        const int i = kCache == kHalfCache || n == 0 ? n : n < 3 ? n + 2 : n - 2;
         const int row = warp * kProRows + 2 * i + half;  // 0-31 q heads, 32-35 k heads, 36-39 v heads
         float x[8];
         raw[i].unpack(x);
@@ -359,23 +361,31 @@ __device__ __forceinline__ void prologue_rows(const PrologueArgs &a) {
                                               pack_f32x2(k1.z, k1.w)};
             pf_norm_rope8(x, wk, cs, sn, nsn, rope, 1.0f);
         }
-        if (kCache == kKv4Cache) {
-            store_row_kv4(a, x, pos, t, kvh, !is_k, sub, to_cache, bad);
-            continue;
+        if (kCache != kHalfCache) {
+            const ProHalf h(x);
+            ProHalf staged = h;
+            if (is_k) {
+                if (bad[i == 2]) staged.set(0x7fff7fffu);
+            } else {
+                const bool odd = !h.finite();
+                if (odd) staged.set(0u);
+                bad[i == 4] = (__ballot_sync(0xffffffffu, odd) >> (16 * half) & 0xffffu) != 0;
+            }
+            __half *st = (is_k ? a.k_st : a.v_st) + size_t(kvh) * a.st_rows * kHeadDim + 4 * sub;
+            staged.store(st + size_t(a.st_new + t) * kHeadDim);
+            if (pos < a.first_tokens && a.first_rows > 0) staged.store(st + size_t(pos) * kHeadDim);
+            if (kCache == kKv4Cache) {
+                store_row_kv4(a, h, pos, kvh, !is_k, sub, to_cache);
+                continue;
+            }
+            if (pos < a.first_tokens) h.store((is_k ? a.first_k : a.first_v) + (size_t(kvh) * kMaxFirstTokens + pos) * kHeadDim + 4 * sub);
         }
         if (to_cache) {
             __half *cache = is_k ? a.k_cache : a.v_cache;
             const size_t crow = a.block_table ? (page * kNHeadKv + kvh) * 64 + (pos & 63) : size_t(kvh) * a.n_slots + slot;
             pf_store_half44(cache + crow * kHeadDim + 4 * sub, x);
         }
-        if (kCache == kHalfFirst) {
-            __half *st = is_k ? a.k_st : a.v_st;
-            pf_store_staged(st + (size_t(kvh) * a.st_rows + a.st_new + t) * kHeadDim + 4 * sub, x, !is_k, bad);
-            if (pos < a.first_tokens) {
-                pf_store_half44((is_k ? a.first_k : a.first_v) + (size_t(kvh) * kMaxFirstTokens + pos) * kHeadDim + 4 * sub, x);
-                if (a.first_rows > 0) pf_store_staged(st + (size_t(kvh) * a.st_rows + pos) * kHeadDim + 4 * sub, x, !is_k, bad);
-            }
-        } else if (a.k_st) {
+        if (kCache == kHalfCache && a.k_st) {
             pf_store_half44((is_k ? a.k_st : a.v_st) + (size_t(kvh) * a.st_rows + a.st_new + t) * kHeadDim + 4 * sub, x);
         }
     }

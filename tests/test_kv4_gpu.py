@@ -513,6 +513,7 @@ def test_prefill_keeps_infinities_from_queries_that_do_not_see_them(fa, in_type,
     k, v = _history(torch, 45, 1, max(past, 1))
     qkv = _rand(torch, 47, tokens, 5120, dtype=dt)
     bad_at = {head: set() for head in range(4)}
+    v[0, 2, -1, 3], v[0, 2, -1, 4] = 65504, -65504  # d rounds up: lo + 15 d is 65536 in a 4-bit cache
     k2, v2, qkv2 = k.clone(), v.clone(), qkv.clone()
     mid, pad = tokens // 3, tokens - 10
     qkv2[mid, 4608 + 128 + 77] = math.inf  # V of KV head 1, one value
@@ -537,6 +538,7 @@ def test_prefill_keeps_infinities_from_queries_that_do_not_see_them(fa, in_type,
             h.prefill_dev(0, 0, tokens, x, _kind(fa, torch, dt), out, fa.F32)
             h.check()
             outs.append(out.view(tokens, 4, 1024))
+    assert torch.isfinite(outs[0]).all()
     at, keys = torch.arange(past, past + tokens, device="cuda"), torch.arange(past + tokens, device="cuda")
     sees = ref.visible(at, keys, is_swa, first)
     for head in range(4):
