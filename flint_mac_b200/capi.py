@@ -231,6 +231,8 @@ class Attn:
         fn = self._lib[name]  # a function object of its own, without argument types
         fn.restype = C.c_int32
         types = SYMBOLS[name][1]
+        if self._h is None:
+            raise FlintAttnError("the handle is closed")
         given = (self._h,) + args + (self._err, ERR_LEN)
         assert len(given) == len(types)
         simple = (C.c_int32, C.c_void_p)
@@ -299,6 +301,8 @@ class Attn:
                                     out_dtype, stream)
 
         def call(qkv_address: int):
+            if self._h is None:
+                raise FlintAttnError("the handle is closed")
             rows.value = qkv_address
             if fn(*args) != 0:
                 raise FlintAttnError(err.value.decode(errors="replace"))
@@ -402,15 +406,18 @@ class Attn:
         self._call("flint_attn_write_kv", layer, seq, slot0, k.shape[1], k.ctypes.data, v.ctypes.data)
 
     def _kv_rows(self, name, layer, seqs, pos0, n_rows, k_dev, v_dev, dtype, stream):
-        """f() that enqueues the call, with every argument converted once."""
+        """f() that enqueues the call, with every argument converted once (it keeps the handle and the arrays alive)."""
         if len(seqs) != len(pos0):
             raise ValueError("one start position per sequence")
         fn, args, err = self._bound(name, layer, len(seqs), _i32(seqs), _i32(pos0), n_rows, _ptr(k_dev), _ptr(v_dev), dtype, stream)
 
         def call():
+            if self._h is None:
+                raise FlintAttnError("the handle is closed")
             if fn(*args) != 0:
                 raise FlintAttnError(err.value.decode(errors="replace"))
 
+        call.arrays = (k_dev, v_dev)
         return call
 
     def store_kv_dev(self, layer, seqs, pos0, n_rows, k_dev, v_dev, dtype, stream: int = 0):

@@ -974,7 +974,7 @@ static void prefill_impl(flint_attn *a, int layer, int seq, int n_tok, const voi
     if (seq < 0 || seq >= a->max_seqs) throw std::runtime_error("sequence index out of range");
     if (n_tok <= 0) throw std::runtime_error("empty prefill");  // src/engine.mm:975
     const int p0 = a->pos[seq];
-    if (p0 + n_tok > a->n_ctx) throw std::runtime_error("context full");  // src/engine.mm:976
+    if (n_tok > a->n_ctx - p0) throw std::runtime_error("context full");  // src/engine.mm:976
     if (a->kv_ranks > 1 && !L.is_swa && !partial_o)
         throw std::runtime_error("full layers of a KV-sharded handle need prefill_partial + prefill_combine");
     if (partial_o && L.is_swa) throw std::runtime_error("sliding-window layers are not sharded: use prefill_dev");
@@ -1230,6 +1230,7 @@ int32_t flint_attn_n_slots(const flint_attn *a, int32_t layer) {
 // Rows of n sequences between a layer's cache and dense arrays [n][4][n_rows][128] on the device.
 static void kv_rows(flint_attn *a, int layer, int n, const int32_t *seqs, const int32_t *pos0, int n_rows, void *k, void *v,
                     int dtype, cudaStream_t st, bool store) {
+    if (!a) throw std::runtime_error("null handle");
     CK(cudaSetDevice(a->device));
     if (layer < 0 || layer >= int(a->layers.size())) throw std::runtime_error("layer index out of range");
     Layer &L = a->layers[layer];

@@ -30,6 +30,14 @@ def test_open_refuses(fa, kw, match):
         fa.Attn([True], [True], 1, 128, **kw)
 
 
+def test_rows_of_no_handle_are_refused(fa):
+    import ctypes as C
+
+    lib, err, zero = fa.load_library(), C.create_string_buffer(200), (C.c_int32 * 1)(0)
+    for fn in (lib.flint_attn_store_kv_dev, lib.flint_attn_load_kv_dev):
+        assert fn(None, 0, 1, zero, zero, 1, 16, 16, fa.F32, None, err, 200) == -1 and err.value == b"null handle"
+
+
 def test_statement_keeps_what_it_says():
     """The reference itself: every value within half a step of what it came from, the least and largest of a group exact
     to the rounding of d."""
@@ -267,10 +275,18 @@ def test_rows_refused(fa):
             h.decode_partial_dev(0, [0], big, fa.F32, big)
         with pytest.raises(fa.FlintAttnError, match="4-bit"):
             h.prefill_partial_dev(0, 0, 1, big, fa.F32, big, big)
+        h.set_pos(0, 9)
+        for n in (192, 2**31 - 1):
+            with pytest.raises(fa.FlintAttnError, match="context full"):
+                h.prefill_dev(0, 0, n, big, fa.F32, big, fa.F32)
+        prepared = h.prepared_store_kv_dev(0, [0], [0], 1, x, x, fa.F16), lambda f=h.prepared_decode_dev(0, [0], fa.F32, big, fa.F32): f(big.data_ptr())
         # a page that no sequence holds reads as zeros
         k, v = torch.ones(2, 1, 4, 10, 128, device="cuda")
         h.load_kv_dev(0, [1], [60], 10, k, v, fa.F32)
         assert not k.any() and not v.any()
+    for call in (*prepared, lambda: h.load_kv_dev(0, [1], [60], 10, k, v, fa.F32)):
+        with pytest.raises(fa.FlintAttnError, match="closed"):
+            call()
 
 
 @gpu
