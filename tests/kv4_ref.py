@@ -57,7 +57,12 @@ def attend(q, k, v, seen, sinks):
     The kernels round q, the keys of a call and probabilities to half (2^-11 relative each), and probabilities times d or
     the staged values once more.  A score's error is then at most 3 * 2^-11 * sum |q_i k_i| / sqrt(128) (keys that went
     through norm and rotation in 32 bits may land on the neighbouring half: 2 * 2^-11), which moves every probability by at
-    most twice that, relatively; three more roundings sit on the products p v.  32-bit sums add less than 2^-16."""
+    most twice that, relatively; three more roundings sit on the products p v.  32-bit sums add less than 2^-16.
+
+    A cached value is lo + d code, and its product the sum of p' lo and r(p' d) code, with p' the rounded probability and r
+    one more rounding: p' lo + p' d code (1 + e) = p' v + e p' (v - lo), |e| <= 2^-11.  So where lo and d code nearly cancel
+    (a query that sees two keys: v = 0.002 from terms of 1.3) the error is 2^-11 p |v - lo|, however small v is, and the
+    32-bit sums are relative to those terms too.  A group's least value has code 0, so lo is its minimum."""
     n, m = q.shape[0], k.shape[1]
     qh = q.view(n, KVH, GQA, DIM)
     s = torch.einsum("nhgd,hmd->nhgm", qh, k) / math.sqrt(DIM)
@@ -67,7 +72,9 @@ def attend(q, k, v, seen, sinks):
     sink = sinks.double().view(1, KVH, GQA, 1).expand(n, KVH, GQA, 1)
     p = torch.cat((s, sink), -1).softmax(-1)[..., :m]
     out = torch.einsum("nhgm,hmd->nhgd", p, v)
-    room = torch.einsum("nhgm,hmd->nhgd", p, v.abs()) * (2 * 3 * 2**-11 * mag.amax(-1, keepdim=True) + 3 * 2**-11 + 2**-16)
+    g = v.unflatten(-1, (DIM // GROUP, GROUP))
+    off = torch.einsum("nhgm,hmd->nhgd", p, (g - g.amin(-1, keepdim=True)).flatten(-2)) * (2**-11 + 2**-16)
+    room = off + torch.einsum("nhgm,hmd->nhgd", p, v.abs()) * (2 * 3 * 2**-11 * mag.amax(-1, keepdim=True) + 3 * 2**-11 + 2**-16)
     return out.reshape(n, 32, DIM), room.reshape(n, 32, DIM) + 1e-6
 
 

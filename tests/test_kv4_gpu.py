@@ -716,7 +716,8 @@ def test_captured_and_replayed(fa):
 
 @gpu
 def test_a_graph_outlives_larger_calls(fa):
-    """Two graphs of one handle, replayed in turn and after larger batches of the handle, give what they gave."""
+    """Graphs of one handle, one of them a launch of several rounds, replayed in turn and after larger batches of the
+    handle, give what they gave."""
     import torch
 
     n, p = 300, 1500
@@ -727,7 +728,7 @@ def test_a_graph_outlives_larger_calls(fa):
         for s in range(n):
             h.store_kv_dev(0, [s], [0], p, k, v, fa.F16)
             h.set_pos(s, p)
-        outs = torch.empty(2, 2, 4096, device="cuda")
+        outs, many = torch.empty(2, 2, 4096, device="cuda"), torch.empty(n - 50, 4096, device="cuda")
         side = torch.cuda.Stream()
         graphs = []
         for i in range(2):
@@ -735,6 +736,10 @@ def test_a_graph_outlives_larger_calls(fa):
             with torch.cuda.graph(g, stream=side):  # (no call of the handle before the first capture)
                 h.decode_dev(0, [0, 1][: i + 1], rows, fa.F32, outs[i], fa.F32, torch.cuda.current_stream().cuda_stream)
             graphs.append(g)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            h.decode_dev(0, range(n - 50), rows, fa.F32, many, fa.F32, torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
         big = torch.empty(n, 4096, device="cuda")
         got = []
         for _ in range(3):
@@ -742,6 +747,9 @@ def test_a_graph_outlives_larger_calls(fa):
             for g in graphs:
                 g.replay()
             got.append(outs.clone())
+            h.decode_dev(0, range(n - 50), rows, fa.F32, big, fa.F32)
+            assert torch.equal(many, big[: n - 50])
+            many.zero_()
             h.decode_dev(0, range(n), rows, fa.F32, big, fa.F32)
         torch.cuda.synchronize()
         h.check()
