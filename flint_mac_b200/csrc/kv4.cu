@@ -274,11 +274,13 @@ __global__ void __launch_bounds__(kRowThreads) k_kv4_load(const KvRowsParams p, 
         vd[i] = vl[i] = 0;
         const unsigned char *blk = front && b.first + r < p.cache.first_tokens ? front : block;
         if (!blk || !b.has(r)) continue;
-        kc[i] = __ldg(reinterpret_cast<const uint32_t *>(blk + kKv4KCodes + kv4_chunk(r, g) + (sub & 3) * 4));
-        kg[i] = __ldg(reinterpret_cast<const uint32_t *>(blk + kv4_k_group(r, g)));
-        vc[i] = __ldg(reinterpret_cast<const uint32_t *>(blk + kKv4VCodes + kv4_chunk(r, g) + (sub & 3) * 4));
-        vd[i] = __ldg(reinterpret_cast<const uint16_t *>(blk + kv4_v_group(r, g)));
-        vl[i] = __ldg(reinterpret_cast<const uint16_t *>(blk + kv4_v_group(r, g) + 16));
+        // (ordinary loads, which the wait above orders behind the stream's earlier kernels: one that writes the block may run
+        // beside this grid's beginning, so the block is not read-only for the grid's whole life, as __ldg takes it to be)
+        kc[i] = *reinterpret_cast<const uint32_t *>(blk + kKv4KCodes + kv4_chunk(r, g) + (sub & 3) * 4);
+        kg[i] = *reinterpret_cast<const uint32_t *>(blk + kv4_k_group(r, g));
+        vc[i] = *reinterpret_cast<const uint32_t *>(blk + kKv4VCodes + kv4_chunk(r, g) + (sub & 3) * 4);
+        vd[i] = *reinterpret_cast<const uint16_t *>(blk + kv4_v_group(r, g));
+        vl[i] = *reinterpret_cast<const uint16_t *>(blk + kv4_v_group(r, g) + 16);
     }
 #pragma unroll
     for (int i = 0; i < kRowSteps; i++) {
