@@ -446,9 +446,17 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
     // Per lane: reference maximum (replicated over g) and partial sum of heads 2 t4 and 2 t4 + 1; outputs o[2c] = dims
     // 32 c + 4 g (n0) and + 1 (n0 + 16 n1), o[2c + 1] = dims + 2 and + 3, each for the two heads; om = the part of lo, group
     // g & 3.
-    // The reference lies 1 under a maximum (base 2) and stays until one exceeds it by 2, so that few tiles have outputs to
-    // rescale.  Probabilities are then at most 4, and times d, which is at most 8736, they fit a half.
+    // The reference lies kUp + 1 under a maximum (base 2) and stays until one exceeds it by kUp + 2, so that few tiles have
+    // outputs to rescale; probabilities are then at most 2^(kUp + 2) = 2^13.  Their products with d are operands in half
+    // precision, and below 2^-14 a half loses bits, below 2^-25 all of them: a key would count as the least value of its
+    // group.  So the outputs o are kept times 2^b: d takes the factor where b > 0, which is exact, the probabilities where
+    // b < 0.  b stays while the largest d of a tile's visible rows, times 2^b, lies between 2^-6 and 4 (V rows whose groups
+    // span 0.25 to 60: b = 0, and nothing is multiplied), and goes back into [1/2, 1) or below 4 when it does not.  Products
+    // are then below 2^15, and normal halves for every row whose probability times d is above 2^-19 of the largest d times P,
+    // with P the probability that lies kUp above the reference, which some key seen exceeds twofold; where b < 0, the
+    // probabilities themselves lose bits below 2^(-25 - b) P (b >= -12).
     float m0 = -INFINITY, m1 = -INFINITY;
+    int b_exp = 0;
     uint64_t l01 = 0;  // (two zeros)
     float o[2 * kKv4Groups][4], om[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -520,8 +528,9 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
             mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
             mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
         }
-        if (__any_sync(0xffffffffu, mx0 > m0 + 2.f || mx1 > m1 + 2.f)) {
-            const float n0 = mx0 > m0 + 2.f ? mx0 - 1.f : m0, n1 = mx1 > m1 + 2.f ? mx1 - 1.f : m1;
+        constexpr float kUp = 11.f;
+        if (__any_sync(0xffffffffu, mx0 > m0 + (kUp + 2.f) || mx1 > m1 + (kUp + 2.f))) {
+            const float n0 = mx0 > m0 + (kUp + 2.f) ? mx0 - (kUp + 1.f) : m0, n1 = mx1 > m1 + (kUp + 2.f) ? mx1 - (kUp + 1.f) : m1;
             const float c0 = fast_exp2(m0 - n0), c1 = fast_exp2(m1 - n1);
             l01 = mul2(l01, pack2(c0, c1));
 #pragma unroll
@@ -550,9 +559,30 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
             break;
         }
         used++;
+        auto seen = [&](int r) {  // rows r and r + 1, as a mask of their halves
+            return (r >= r_lo && r < r_hi ? 0xffffu : 0u) | (r + 1 >= r_lo && r + 1 < r_hi ? 0xffff0000u : 0u);
+        };
+        {  // the largest d: a lane looks at two rows, a maximum passes over NaN
+            uint32_t w[4];
+            lds128(w, v_tile + (kKv4VGroups - kHalf) + lane * 32);
+            uint32_t top = as_u32(__hmax2(__hmax2(__hmax2(as_half2(w[0]), as_half2(w[1])), __hmax2(as_half2(w[2]), as_half2(w[3]))), as_half2(0u)));
+            if (edge) top &= seen(2 * lane);
+            top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+            const int e = int(top >> 10);  // d is in [2^(e - 15), 2^(e - 14)), for e = 0 below
+            if (top != 0 && (e + b_exp < 9 || e + b_exp > 16)) {
+                const int to = e + b_exp > 16 ? 16 - e : 14 - e;
+                const float c = __int_as_float((127 + to - b_exp) << 23);
+#pragma unroll
+                for (int i = 0; i < 2 * kKv4Groups; i++) {
+                    o[i][0] *= c; o[i][1] *= c; o[i][2] *= c; o[i][3] *= c;
+                }
+                b_exp = to;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t pb0 = pb[i][0], pb1 = pb[i][1];
+            uint32_t ps0 = pb0, ps1 = pb1;  // those that meet d
             uint32_t da[4], db[4];
             // d and lo of rows 16 i + 2 t4 and the next, and of those 8 rows on
             lds128(da, vg_at + i * 256);
@@ -560,9 +590,6 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
             uint32_t la = lds32(vg_at + i * 256 + 16 + 4 * (g & 3)), lb = lds32(vg_at + i * 256 + 144 + 4 * (g & 3));
             if (edge) {  // rows that the query does not see may hold anything: their d and lo count 0
                 const int ka = 16 * i + 2 * t4;
-                auto seen = [&](int r) {
-                    return (r >= r_lo && r < r_hi ? 0xffffu : 0u) | (r + 1 >= r_lo && r + 1 < r_hi ? 0xffff0000u : 0u);
-                };
                 const uint32_t va = seen(ka), vb = seen(ka + 8);
 #pragma unroll
                 for (int c = 0; c < kKv4Groups; c++) {
@@ -571,6 +598,16 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
                 }
                 la &= va;
                 lb &= vb;
+            }
+            if (b_exp != 0) {
+                const uint32_t fd = uint32_t(15 + max(b_exp, 0)) * 0x04000400u, fp = uint32_t(15 + min(b_exp, 0)) * 0x04000400u;  // powers of two
+                ps0 = mul_half2(ps0, fp);
+                ps1 = mul_half2(ps1, fp);
+#pragma unroll
+                for (int c = 0; c < kKv4Groups; c++) {
+                    da[c] = mul_half2(da[c], fd);
+                    db[c] = mul_half2(db[c], fd);
+                }
             }
             {
                 const uint32_t a[4] = {la, 0u, lb, 0u};
@@ -583,7 +620,7 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
 #pragma unroll
                 for (int q2 = 0; q2 < 2; q2++) {
                     const int c = 2 * hf + q2;
-                    const uint32_t b0v = mul_half2(pb0, da[c]), b1v = mul_half2(pb1, db[c]);
+                    const uint32_t b0v = mul_half2(ps0, da[c]), b1v = mul_half2(ps1, db[c]);
                     const Codes x = split_codes(w[2 * q2]), y = split_codes(w[2 * q2 + 1]);
                     const uint32_t a0[4] = {x.n0, x.n01, y.n0, y.n01}, a1[4] = {x.n2, x.n23, y.n2, y.n23};
                     mma_16816(o[2 * c], a0, b0v, b1v);
@@ -626,9 +663,9 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
         sm.red_m[warp][2 * t4] = m0; sm.red_m[warp][2 * t4 + 1] = m1;
         sm.red_l[warp][2 * t4] = l0; sm.red_l[warp][2 * t4 + 1] = l1;
     }
+    const float k0 = __int_as_float((127 + 24 - b_exp) << 23), k1 = __int_as_float((127 + 20 - b_exp) << 23);  // 2^24 / 2^b, and 2^20 / 2^b for the differences
 #pragma unroll
     for (int c = 0; c < kKv4Groups; c++) {
-        constexpr float k0 = 16777216.f, k1 = 1048576.f;  // 2^24, and 2^20 for the differences
         const float lo0 = __shfl_sync(0xffffffffu, om[0], 4 * c + t4), lo1 = __shfl_sync(0xffffffffu, om[1], 4 * c + t4);
         const float *e = o[2 * c], *f = o[2 * c + 1];
         *reinterpret_cast<float4 *>(&sm.o[warp][2 * t4][32 * c + 4 * g]) =
