@@ -13,6 +13,7 @@
 
 #include "../../include/flint_attn.h"
 #include "attn_common.h"
+#include "device_errors.h"
 #include "kv4.h"
 #include "prefill_attn.h"
 #include "proj.h"
@@ -1200,23 +1201,29 @@ int32_t flint_attn_check(flint_attn *a, char *err, int32_t err_len) {
     CK(cudaDeviceSynchronize());
     // Each device error word is reported once and cleared, the way the reference raises once per failed command
     // buffer (src/engine.mm:930-932): later, healthy launches on this handle are not failed by an old error.
-    int flag = 0;
-    CK(prefill_error_flag(a->pf, &flag));
-    if (flag) throw std::runtime_error("prefill kernel reported device error " + std::to_string(flag));
-    CK(cudaMemcpy(&flag, a->dec_err, sizeof(int), cudaMemcpyDeviceToHost));
-    if (flag) {
-        CK(cudaMemset(a->dec_err, 0, sizeof(int)));
-        if (a->tickets) CK(cudaMemset(a->tickets, 0, a->n_tickets * sizeof(int)));  // (a launch that gave up left them counted)
-        CK(cudaDeviceSynchronize());
-        throw std::runtime_error("decode kernel reported device error " + std::to_string(flag));
-    }
-    if (a->xchg) {
-        int *word = reinterpret_cast<int *>(a->xchg + kMaxPeers * sizeof(uint32_t));
-        CK(cudaMemcpy(&flag, word, sizeof(int), cudaMemcpyDeviceToHost));
-        if (flag) {
-            CK(cudaMemset(word, 0, sizeof(int)));
-            throw std::runtime_error("the wait for a peer's partial records ran out (exchange error " + std::to_string(flag) + ")");
+    struct Words {
+        flint_attn *a;
+        static int take(int *word) {
+            int flag = 0;
+            CK(cudaMemcpy(&flag, word, sizeof(int), cudaMemcpyDeviceToHost));
+            if (flag) CK(cudaMemset(word, 0, sizeof(int)));
+            return flag;
         }
+        int take_prefill() {
+            int flag = 0;
+            CK(prefill_error_flag(a->pf, &flag));
+            return flag;
+        }
+        int take_decode() { return take(a->dec_err); }
+        int take_exchange() { return a->xchg ? take(reinterpret_cast<int *>(a->xchg + kMaxPeers * sizeof(uint32_t))) : 0; }
+        void clear_counters() {
+            if (a->tickets) CK(cudaMemset(a->tickets, 0, a->n_tickets * sizeof(int)));
+        }
+    };
+    const std::string errors = take_device_errors(Words{a});
+    if (!errors.empty()) {
+        CK(cudaDeviceSynchronize());  // (a launch on a non-blocking stream does not wait for the default stream)
+        throw std::runtime_error(errors);
     }
     return 0;
     API_CATCH(-1)
