@@ -1461,7 +1461,7 @@ int32_t flint_attn_plan_decode(int32_t n, const int32_t *pos, int32_t is_swa, in
 int32_t flint_attn_plan_decode_int4(int32_t n, const int32_t *pos, int32_t is_swa, int32_t first_tokens,
                                     int32_t target_items, int32_t *out, int32_t cap) {
     try {
-        if (n <= 0 || first_tokens < 0 || !pos || !out) return -1;
+        if (n <= 0 || first_tokens < 0 || first_tokens > kMaxFirstTokens || !pos || !out) return -1;
         std::vector<int> tiles(n);
         std::vector<Dec4Piece> pieces;
         for (int i = 0; i < n; i++) {

@@ -271,7 +271,7 @@ int32_t flint_attn_plan_decode(int32_t n, const int32_t *pos, int32_t is_swa, in
 /* The same for decode over a 4-bit cache: one record of 8 int32 per piece of a token's visible keys, for each of the four
  * KV heads alike = { token, tile0, tile1, split, n_split, first_record, launch, records_of_launch }.  Tiles are 64 keys,
  * the first tokens' one in front where the token sees any; the pieces of a token tile all its tiles once.  Returns the
- * piece count, or -1 if cap is too small. */
+ * piece count, or -1 if cap is too small or first_tokens is not one that a handle opens with (0 to 64). */
 int32_t flint_attn_plan_decode_int4(int32_t n, const int32_t *pos, int32_t is_swa, int32_t first_tokens,
                                     int32_t target_items, int32_t *pieces, int32_t cap);
 /* Tuning knob: work items the planner aims for per launch (default: one wave of 2 CTAs on every SM). */
