@@ -38,6 +38,7 @@ _KV_ROWS = [C.c_void_p, C.c_int32, C.c_int32, C.POINTER(C.c_int32), C.POINTER(C.
 SYMBOLS = {
     "flint_attn_open_kv": (C.c_void_p, [C.POINTER(_Config), C.POINTER(_KvOptions), C.c_char_p, C.c_int32]),
     "flint_attn_plan_decode_int4": (C.c_int32, [C.c_int32, _I32P, C.c_int32, C.c_int32, C.c_int32, _I32P, C.c_int32]),
+    "flint_attn_plan_prefill_int4": (C.c_int32, [C.c_int32, C.c_int32, C.c_int32, _I32P, C.c_int32]),
     "flint_attn_store_kv_dev": (C.c_int32, _KV_ROWS),
     "flint_attn_load_kv_dev": (C.c_int32, _KV_ROWS),
     "flint_attn_open": (C.c_void_p, [C.POINTER(_Config), C.c_char_p, C.c_int32]),
@@ -167,6 +168,17 @@ def plan_decode_int4(pos: Sequence[int], is_swa: bool, first_tokens: int = 0, ta
     n = lib.flint_attn_plan_decode_int4(len(pos), _i32(pos), int(is_swa), first_tokens, target_items, out, cap)
     if n < 0:
         raise FlintAttnError("bad batch for a plan")
+    return np.ctypeslib.as_array(out)[: 8 * n].reshape(n, 8).copy()
+
+
+def plan_prefill_int4(n_tok: int, p0: int, n_sm: int = 148):
+    """Host-only: the pieces of a prefill on a full layer with a 4-bit cache as an int32 array [n][8] = (cta, unit, part, tile0,
+    tile1, tiles_of_unit, first_query, kv_head); empty where the call's units are not cut so that all CTAs end together."""
+    cap = 1024
+    out = (C.c_int32 * (8 * cap))()
+    n = load_library().flint_attn_plan_prefill_int4(n_tok, p0, n_sm, out, cap)
+    if n < 0:
+        raise FlintAttnError("bad prefill for a plan")
     return np.ctypeslib.as_array(out)[: 8 * n].reshape(n, 8).copy()
 
 

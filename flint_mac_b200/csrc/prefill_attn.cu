@@ -1190,7 +1190,51 @@ int whole_units_load(const PfArgs &a, int n_units, int grid) {
     return most;
 }
 
+// Ranges that the units of a full layer are cut into evenly: where they leave most of the SMs idle, as many of at least four
+// tiles as fit.
+int even_ksplit(int n_tok, int p0, int n_units, int sm_count, int kr_lo, int kr_hi) {
+    if (n_units * 2 > sm_count) return 1;
+    // the shortest unit's tiles (the first query block that has keys here)
+    const int min_tiles = unit_geom_of(n_units - 1, n_tok, p0, 0, 0, 1, kr_lo, kr_hi).n_tiles;
+    return std::max(1, std::min(sm_count / n_units, min_tiles / 4));
+}
+
+// A full layer with a 4-bit cache: units are cut so that all CTAs end together, where that gains more than the partials cost
+// (a piece is 131 KB of fp32 rows written and read again, about 0.05 us; a key tile takes a CTA 2.2 us).  Returns the parts of
+// the most divided unit, 0 where the units stay as n_ksplit has them.
+int choose_cuts(int n_tok, int p0, int n_units, int n_ksplit, int sm_count, int kr_lo, int kr_hi, PfCuts &cuts, int &n_pieces) {
+    PfArgs g{};
+    g.n_tok = n_tok; g.p0 = p0; g.key_row0 = kr_lo; g.kr_lo = kr_lo; g.kr_hi = kr_hi;
+    const int parts = plan_cuts(g, n_units, sm_count, cuts, n_pieces);
+    if (parts <= 1) return 0;
+    long long total = 0;
+    for (int u = 0; u < n_units; u++) total += unit_geom_of(u, n_tok, p0, 0, kr_lo, 1, kr_lo, kr_hi).n_tiles;
+    const double even = double(total) / sm_count + 2.0;
+    const double whole = n_ksplit > 1 ? unit_geom_of(0, n_tok, p0, 0, kr_lo, 1, kr_lo, kr_hi).n_tiles / double(n_ksplit) + 1.0
+                                      : double(whole_units_load(g, n_units, sm_count));
+    const double partials = 0.05 * (n_pieces - (n_ksplit > 1 ? n_units * n_ksplit : 0)) + (n_ksplit > 1 ? 0.0 : 6.0);
+    return (whole - even) * 2.2 > partials ? parts : 0;
+}
+
 }  // namespace
+
+int plan_prefill_kv4(int n_tok, int p0, int sm_count, std::vector<PrefillPiece> &pieces, int &n_units, int &parts) {
+    static thread_local PfCuts cuts;
+    constexpr int kAll = 0x7fffffff;
+    n_units = (n_tok + kCtaPos - 1) / kCtaPos * kNHeadKv;
+    const int n_ksplit = even_ksplit(n_tok, p0, n_units, sm_count, 0, kAll);
+    int n_pieces = 0;
+    parts = choose_cuts(n_tok, p0, n_units, n_ksplit, sm_count, 0, kAll, cuts, n_pieces);
+    pieces.clear();
+    if (parts == 0) return n_ksplit;
+    for (int b = 0; b < sm_count; b++)
+        for (int e = cuts.start[b]; e < cuts.start[b + 1]; e++) {
+            const PfCut &c = cuts.e[e];
+            const Unit u = unit_geom_of(c.unit, n_tok, p0, 0, 0, 1);
+            pieces.push_back(PrefillPiece{b, c.unit, c.part, c.tile0, c.tile1, u.n_tiles, u.q_first, u.kvh});
+        }
+    return n_ksplit;
+}
 
 cudaError_t prefill_kernel_setup() {
     if (!g_encode) {
@@ -1247,33 +1291,13 @@ cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStr
     if (n_units_q > 0 && (unit_geom_of(n_units_q - 1, T, p.p0, p.is_swa, p.is_swa ? p.p0 - n_hist : kr_lo, 1, kr_lo, kr_hi).n_keys <= 0 ||
                           unit_geom_of(0, T, p.p0, p.is_swa, p.is_swa ? p.p0 - n_hist : kr_lo, 1, kr_lo, kr_hi).n_keys <= 0))
         return cudaErrorInvalidValue;
-    int n_ksplit = 1;
-    if (!p.is_swa && n_units_q > 0 && n_units_q * 2 <= g_sm_count) {
-        // the shortest unit's tiles (the first query block that has keys here)
-        const int min_tiles = unit_geom_of(n_units_q - 1, T, p.p0, 0, 0, 1, kr_lo, kr_hi).n_tiles;
-        n_ksplit = std::max(1, std::min(g_sm_count / n_units_q, min_tiles / 4));
-    }
+    int n_ksplit = !p.is_swa && n_units_q > 0 ? even_ksplit(T, p.p0, n_units_q, g_sm_count, kr_lo, kr_hi) : 1;
     const int t_pad = (T + kCtaPos - 1) / kCtaPos * kCtaPos;
-    // A full layer with a 4-bit cache: units are cut so that all CTAs end together, where that gains more than the partials
-    // cost (a piece is 131 KB of fp32 rows written and read again, about 0.05 us; a key tile takes a CTA 2.2 us).
     static thread_local PfCuts cuts;
     int n_cut_pieces = 0;
-    bool cut = false;
-    if (kv4 && !p.is_swa && n_units_q > 0) {
-        PfArgs g{};
-        g.n_tok = T; g.p0 = p.p0; g.key_row0 = kr_lo; g.kr_lo = kr_lo; g.kr_hi = kr_hi;
-        const int parts = plan_cuts(g, n_units_q, g_sm_count, cuts, n_cut_pieces);
-        if (parts > 1) {
-            long long total = 0;
-            for (int u = 0; u < n_units_q; u++) total += unit_geom_of(u, T, p.p0, 0, kr_lo, 1, kr_lo, kr_hi).n_tiles;
-            const double even = double(total) / g_sm_count + 2.0;
-            const double whole = n_ksplit > 1 ? unit_geom_of(0, T, p.p0, 0, kr_lo, 1, kr_lo, kr_hi).n_tiles / double(n_ksplit) + 1.0
-                                              : double(whole_units_load(g, n_units_q, g_sm_count));
-            const double partials = 0.05 * (n_cut_pieces - (n_ksplit > 1 ? n_units_q * n_ksplit : 0)) + (n_ksplit > 1 ? 0.0 : 6.0);
-            cut = (whole - even) * 2.2 > partials;
-            if (cut) n_ksplit = parts;
-        }
-    }
+    const int cut_parts = kv4 && !p.is_swa && n_units_q > 0 ? choose_cuts(T, p.p0, n_units_q, n_ksplit, g_sm_count, kr_lo, kr_hi, cuts, n_cut_pieces) : 0;
+    const bool cut = cut_parts > 0;
+    if (cut) n_ksplit = cut_parts;
     const size_t part_o_bytes = n_ksplit > 1 ? up(size_t(n_ksplit) * t_pad * kQDim * sizeof(float)) : 0;
     const size_t part_ml_bytes = n_ksplit > 1 ? up(size_t(n_ksplit) * t_pad * kNHead * sizeof(float2)) : 0;
     const size_t need = q_bytes + 2 * kv_bytes + part_o_bytes + part_ml_bytes + 1024;

@@ -274,6 +274,12 @@ int32_t flint_attn_plan_decode(int32_t n, const int32_t *pos, int32_t is_swa, in
  * piece count, or -1 if cap is too small or first_tokens is not one that a handle opens with (0 to 64). */
 int32_t flint_attn_plan_decode_int4(int32_t n, const int32_t *pos, int32_t is_swa, int32_t first_tokens,
                                     int32_t target_items, int32_t *pieces, int32_t cap);
+/* The work list of a prefill of n_tok tokens behind p0 cached ones on a full layer with a 4-bit cache, on a GPU of n_sm
+ * multiprocessors: one record of 8 int32 per piece = { cta, unit, part, tile0, tile1, tiles_of_unit, first_query, kv_head },
+ * CTA by CTA in the order in which they take them.  A unit is 32 query positions of a KV head, its tiles are 128 keys.
+ * Returns the piece count, 0 where the call's units are not cut this way, or -1 if an argument is out of range or cap is too
+ * small. */
+int32_t flint_attn_plan_prefill_int4(int32_t n_tok, int32_t p0, int32_t n_sm, int32_t *pieces, int32_t cap);
 /* Tuning knob: work items the planner aims for per launch (default: one wave of 2 CTAs on every SM). */
 int32_t flint_attn_set_target_items(flint_attn *a, int32_t target_items);
 /* Number of kernel launches this handle has enqueued so far. */
