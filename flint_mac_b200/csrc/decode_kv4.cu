@@ -16,10 +16,9 @@
 // of the difference of two outputs.  On the K side d multiplies the 32-dim partial scores (4 groups per key), on the V side
 // it multiplies the probabilities (4 operand pairs per 16 keys), and lo enters through one more product each.
 //
-// A CTA works on pieces (kv4_plan.h), one after the other: its own, then, in launches of several rounds, those of CTAs that
-// have not started.  Its warps (four, eight or sixteen) take the tiles of a piece in turn and work alone: a tile is one 5 KB
-// bulk copy for K and one for V, on mbarriers of the warp's own; the next tile's K comes in while this one's V is worked on,
-// and the other way round, and the raw rows and the first K of the next piece while this one is worked on and ended.
+// A CTA works on one piece (kv4_plan.h).  Its warps (four, eight or sixteen) take the piece's tiles in turn and work alone: a
+// tile is one 5 KB bulk copy for K and one for V, on mbarriers of the warp's own; the next tile's K comes in while this one's
+// V is worked on, and the other way round.
 //
 // Bytes per tile of 64 keys: 10240, against about 800 instructions of the warp, 72 of them products.  64 x 8192 keys (337 MB)
 // take 59 us, 5.7 TB/s or 0.88 of a copy's rate, in short runs, and 68 us when the GPU's power limit holds the clocks down
@@ -48,13 +47,11 @@ struct __align__(128) Dec4Smem {
         float o[kWarps][kGqa][kORow];  // the warps' outputs of a piece, once all are through with its tiles
     };
     alignas(8) unsigned long long full_bar[kWarps][2];  // the K part, the V part has landed
-    alignas(16) uint4 next;                // answer of the scheduler: the next piece, if there is one
-    alignas(8) unsigned long long next_bar;
-    alignas(16) unsigned char raw[kGqa + 2][kHeadDim * 4];  // raw rows of the next piece: q heads, new k, new v
+    alignas(16) unsigned char raw[kGqa + 2][kHeadDim * 4];  // raw rows: q heads, new k, new v
     alignas(16) __half q[kGqa][kHeadDim];  // normalised, rotated, scaled by log2(e) / sqrt(128)
     float red_m[kWarps][kGqa], red_l[kWarps][kGqa];
     alignas(16) __half knew[kHeadDim];
-    alignas(16) __half vnew[2][kHeadDim];  // (the present piece's is read while the next one's is written)
+    alignas(16) __half vnew[kHeadDim];
     alignas(16) float rope_cos[kHeadDim / 2], rope_sin[kHeadDim / 2];
     alignas(16) float q_norm[kHeadDim], k_norm[kHeadDim], sinks[kNHead];
 };
@@ -184,35 +181,12 @@ __device__ __forceinline__ void store_out4(void *out, int dtype, size_t idx, flo
     }
 }
 
-// Asks the scheduler for a CTA of this grid that has not started: it then never starts, and its work is the asker's.
-__device__ __forceinline__ void ask_next(uint32_t dst, uint32_t bar) {
-    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-    mbar_expect_tx(bar, 16);
-    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n" ::"r"(dst), "r"(bar)
-                 : "memory");
-}
-// The answer: the block index of the CTA, or -1 if none was left.
-__device__ __forceinline__ int next_index(uint32_t src) {
-    uint32_t ok, x;
-    asm volatile(
-        "{\n.reg .pred p;\n.reg .b128 r;\n.reg .b64 a, b;\n"
-        "ld.shared.v2.b64 {a, b}, [%2];\n"
-        "mov.b128 r, {a, b};\n"
-        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n"
-        "selp.b32 %0, 1, 0, p;\n"
-        "mov.b32 %1, 0;\n"
-        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n}\n"
-        : "=r"(ok), "=r"(x)
-        : "r"(src)
-        : "memory");
-    return ok ? int(x) : -1;
-}
 __device__ __forceinline__ void cp_async8(uint32_t dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(dst), "l"(src) : "memory");
 }
 
 template <int kWarps>
-__device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Piece *pieces) {
+__device__ __forceinline__ void decode_piece(const Dec4Params &p, const Dec4Piece &piece, int kvh) {
     extern __shared__ __align__(128) unsigned char smem_raw[];
     Dec4Smem<kWarps> &sm = *reinterpret_cast<Dec4Smem<kWarps> *>(smem_raw);
     constexpr int kThreads = kWarps * 32;
@@ -228,7 +202,7 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
     float freq = 0.f;
     const bool rope_warp = rope && rope_at >= 0 && rope_at < kHeadDim / 2;
     if (rope_warp) freq = p.inv_freq[rope_at];
-    // the layer's constants: read from shared memory at every piece (a load past a busy memory system takes microseconds)
+    // the layer's constants, early: a load past a busy memory system takes microseconds
     for (int i = tid; i < kHeadDim; i += kThreads) {
         sm.q_norm[i] = p.q_norm[i];
         sm.k_norm[i] = p.k_norm[i];
@@ -239,7 +213,6 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
     if (lane == 0) {
         mbar_init(k_bar, 1);
         mbar_init(v_bar, 1);
-        if (warp == 0) mbar_init(smem_u32(&sm.next_bar), 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
 
@@ -249,23 +222,14 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
     const uint32_t v_at = v_tile + (((lane >> 3) & 1) * 8 + (lane & 7)) * kKv4RowBytes + (((lane >> 4) ^ sw) << 4);
     const uint32_t kg_at = k_tile + kKv4KGroups + g * 16, vg_at = v_tile + (kKv4VGroups - kHalf) + t4 * 32;
 
-    // the present piece
-    Dec4Piece pc;
-    Dec4Range rg;
-    int kvh, ta, tb;
-    const unsigned char *seq_blocks;  // contiguous caches: the group's first block
-    bool ends;  // it ends its group: it also takes the new token
-    auto get_piece = [&](int index) {
-        pc = pieces[index >> 2];
-        kvh = index & 3;
-        rg = dec4_range(pc.pos, p.is_swa, p.cache.first_tokens);
-        ta = pc.t0;
-        tb = ta + pc.n;
-        ends = pc.split == pc.n_split - 1;
-        seq_blocks = p.cache.blocks + (size_t(pc.seq) * kNHeadKv + kvh) * p.cache.blocks_per_seq * kKv4BlockBytes;
-    };
+    const Dec4Piece pc = piece;
+    const Dec4Range rg = dec4_range(pc.pos, p.is_swa, p.cache.first_tokens);
+    const int ta = pc.t0, tb = ta + pc.n;
+    const bool ends = pc.split == pc.n_split - 1;  // the piece ends its group: it also takes the new token
+    const int extra = rg.n_first > 0 ? 1 : 0;
+    const unsigned char *seq_blocks = p.cache.blocks + (size_t(pc.seq) * kNHeadKv + kvh) * p.cache.blocks_per_seq * kKv4BlockBytes;  // contiguous caches: the group's first block
     auto load_part = [&](int t, int is_v) {  // one lane
-        const int extra = rg.n_first > 0 ? 1 : 0, b = (rg.j0 >> 6) + t - extra;
+        const int b = (rg.j0 >> 6) + t - extra;
         const unsigned char *block;
         if (p.cache.block_table) block = kv4_block(p.cache, pc.seq, kvh, b);
         else block = seq_blocks + size_t(t < extra ? uint32_t(kKv4RingBlocks) : uint32_t(b) & p.cache.block_mask) * kKv4BlockBytes;
@@ -275,9 +239,8 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
         bulk_load(is_v ? v_tile : k_tile, block + is_v * kHalf, kHalf, bar);
     };
     // Raw rows: its heads of the group by each warp, the new k and v by the last two warps too.  A warp reads what it fetched.
-    auto fetch_rows = [&](int index) {
-        const Dec4Piece &w = pieces[index >> 2];
-        const int head0 = (index & 3) * kGqa, tok = p.tok0 + w.tok;
+    auto fetch_rows = [&] {
+        const int head0 = kvh * kGqa, tok = p.tok0 + pc.tok;
         const size_t es = p.qkv_dtype == kDtypeF32 ? 4 : 2;
         const unsigned char *row = static_cast<const unsigned char *>(p.qkv) + size_t(tok) * kQkvDim * es;
         auto fetch = [&](int at, int i) {
@@ -288,17 +251,16 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
 #pragma unroll
         for (int i = 0; i < kHeads; i++)
             if (has_heads) fetch((head0 + warp * kHeads + i) * kHeadDim, warp * kHeads + i);
-        if (w.split == w.n_split - 1 && nw >= 0) fetch(kQDim + nw * kKvDim + (index & 3) * kHeadDim, kGqa + nw);
+        if (ends && nw >= 0) fetch(kQDim + nw * kKvDim + kvh * kHeadDim, kGqa + nw);
         cp_async_commit();
     };
-    auto rope_table = [&](int index) {
+    auto rope_table = [&] {
         if (!rope_warp) return;
         float sn, cs;
-        sincos_reduced(float(pieces[index >> 2].pos) * freq, &sn, &cs);
+        sincos_reduced(float(pc.pos) * freq, &sn, &cs);
         sm.rope_cos[rope_at] = cs;
         sm.rope_sin[rope_at] = sn;
     };
-    int flip = 0;
     auto finish_rows = [&] {  // raw rows (and the rotation table, visible already) -> sm.q, the new token's rows, the cache
         cp_async_wait<0>();
         __syncwarp();
@@ -320,81 +282,28 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
             float4 x = load_row4(&sm.raw[kGqa + nw][0], p.qkv_dtype, 0, lane);
             if (nw == 0) x = norm_rope(x, reinterpret_cast<const float4 *>(sm.k_norm)[lane], cs, sn, lane, rope);
             const uint2 h = make_uint2(pack_half2(x.x, x.y), pack_half2(x.z, x.w));
-            *reinterpret_cast<uint2 *>(nw == 0 ? &sm.knew[d0] : &sm.vnew[flip][d0]) = h;
+            *reinterpret_cast<uint2 *>(nw == 0 ? &sm.knew[d0] : &sm.vnew[d0]) = h;
         }
     };
     auto store_new = [&] {  // the new token's rows -> the cache
         if (!ends || nw < 0) return;
-        const uint2 h = *reinterpret_cast<const uint2 *>(nw == 0 ? &sm.knew[d0] : &sm.vnew[flip][d0]);
+        const uint2 h = *reinterpret_cast<const uint2 *>(nw == 0 ? &sm.knew[d0] : &sm.vnew[d0]);
         kv4_store_lane(kv4_block(p.cache, pc.seq, kvh, pc.pos >> 6), pc.pos & 63, nw == 1, lane, h);
         if (p.is_swa && pc.pos < p.cache.first_tokens)
             kv4_store_lane(kv4_first_block(p.cache, pc.seq, kvh), pc.pos, nw == 1, lane, h);
     };
-    // Split-K, per query head: a warp that has written its record of a head counts it; the one that finds itself the last of
-    // its run of records merges the run, and if that was the last run of the head, the runs.  (The record's stores are ordered
-    // before lane 0's ticket by the warp's barrier; the ticket is an acquire-release atomic at device scope, cumulative over
-    // them; the readers go past L1.)  The first ticket's answer is looked at after the next piece, if there is one: no piece
-    // waits for the round trip.
-    struct Out {
-        int rec0, split, n_split, kvh, row;
-    } out = {};
-    int arrived[kHeads];
-    auto count_record = [&] {
-        const int fan = dec4_fan(out.n_split);
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kHeads; i++)
-            if (lane == 0) arrived[i] = ticket_acq_rel(&p.tickets[(out.rec0 + out.split / fan * kNHeadKv) * kGqa + warp * kHeads + i]);
-    };
-    auto merge_runs = [&] {
-        const int fan = dec4_fan(out.n_split), sub = out.split / fan, n_sub = (out.n_split + fan - 1) / fan;
-        const int n = min(fan, out.n_split - sub * fan);
-        __syncwarp();  // lane 0's tickets come before the other lanes' reads
-#pragma unroll
-        for (int i = 0; i < kHeads; i++) {
-            const int h = warp * kHeads + i, head = out.kvh * kGqa + h;
-            auto record = [&](float *base, int k) { return base + (size_t(out.rec0 + k * kNHeadKv) * kGqa + h) * kRecStride; };
-            if (__shfl_sync(0xffffffffu, arrived[i], 0) != n - 1) continue;
-            if (lane == 0) p.tickets[(out.rec0 + sub * kNHeadKv) * kGqa + h] = 0;  // ready for the next launch
-            Merged4 r = merge_records4([&](int k) { return record(p.scratch, sub * fan + k); }, n, d0);
-            if (n_sub > 1) {
-                float *rec = record(p.scratch2, sub);
-                *reinterpret_cast<float4 *>(rec + d0) = make_float4(r.a[0], r.a[1], r.a[2], r.a[3]);
-                if (lane == 0) *reinterpret_cast<float2 *>(rec + kHeadDim) = make_float2(r.M, r.L);
-                __syncwarp();
-                int last = 0;
-                int *ticket = &p.tickets2[out.rec0 * kGqa + h];
-                if (lane == 0) {
-                    last = ticket_acq_rel(ticket) == n_sub - 1;
-                    if (last) *ticket = 0;
-                }
-                __syncwarp();
-                if (!__shfl_sync(0xffffffffu, last, 0)) continue;
-                r = merge_records4([&](int k) { return record(p.scratch2, k); }, n_sub, d0);
-            }
-            const float sink2 = sm.sinks[head] * kLog2e;
-            const float Mf = fmaxf(r.M, sink2), cf = fast_exp2(r.M - Mf);
-            const float inv = cf / (r.L * cf + fast_exp2(sink2 - Mf));
-            store_out4(p.out, p.out_dtype, size_t(out.row) * kQDim + head * kHeadDim + d0, r.a[0] * inv, r.a[1] * inv, r.a[2] * inv, r.a[3] * inv);
-        }
-    };
-
-    get_piece(int(blockIdx.x));
     // Nothing an earlier kernel of the stream produces (rows, cache contents, split-K records and counters) is read or
     // written before this wait.
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    fetch_rows(int(blockIdx.x));
+    fetch_rows();
     if (lane == 0 && ta + warp < tb) load_part(ta + warp, 0);
-    if (p.several_rounds && tid == 0) ask_next(smem_u32(&sm.next), smem_u32(&sm.next_bar));
-    rope_table(int(blockIdx.x));
+    rope_table();
     __syncthreads();
     finish_rows();
     __syncthreads();
 
     const uint64_t two22 = pack2(4194304.f, 4194304.f);
-    bool waiting = false;  // the last piece's record is out, its run not yet merged
     int used = 0;  // tiles this warp has been through: the phase of its barriers
-    for (uint32_t turn = 0;; turn++) {
     if (lane == 0 && ta + warp < tb) load_part(ta + warp, 1);
     store_new();
     float s_new[kHeads];  // the new token's score with the warp's heads
@@ -461,14 +370,7 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
     float o[2 * kKv4Groups][4], om[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 2 * kKv4Groups; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    // what comes next (asked for a piece ago): its rows are fetched while this piece is worked on
-    bool late = p.several_rounds && !__all_sync(0xffffffffu, wait_bar(smem_u32(&sm.next_bar), turn & 1u));
-    const int next = !p.several_rounds || late ? -1 : next_index(smem_u32(&sm.next));
-    if (next >= 0) {
-        fetch_rows(next);
-        rope_table(next);
-    }
-    const int extra = rg.n_first > 0 ? 1 : 0;
+    bool late = false;  // a wait ran out
     for (int t = ta + warp; t < tb; t += kWarps) {
         if (!__all_sync(0xffffffffu, wait_bar(k_bar, uint32_t(used) & 1u))) {
             late = true;
@@ -631,26 +533,11 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
         __syncwarp();  // the whole warp is done with the V part
         if (lane == 0 && t + kWarps < tb) load_part(t + kWarps, 1);
     }
-    const int row = p.tok0 + pc.tok;
-    const bool with_new = ends, more = next >= 0;
-    const int split = pc.split, n_split = pc.n_split, kv_head = kvh, rec0 = pc.part0 * kNHeadKv + kvh;  // this KV head's records: every fourth
-    if (more) {
-        get_piece(next);
-        if (lane == 0 && ta + warp < tb && !late) load_part(ta + warp, 0);
-    }
     if (__syncthreads_or(late)) {  // (and every warp is through with its V part: they become the merge buffer)
         if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 4);
-        cp_async_wait<0>();
         if (lane == 0)
             for (int i = 0; i < 4; i++) wait_bar(i & 1 ? v_bar : k_bar, uint32_t(i >> 1) & 1u);
-        if (p.several_rounds && tid == 0)
-            for (uint32_t i = 0; i < 2; i++) wait_bar(smem_u32(&sm.next_bar), i);
         return;
-    }
-    if (more) {
-        if (tid == 0) ask_next(smem_u32(&sm.next), smem_u32(&sm.next_bar));
-        flip ^= 1;
-        finish_rows();
     }
     float l0, l1;
     asm("mov.b64 {%0, %1}, %2;\n" : "=f"(l0), "=f"(l1) : "l"(l01));
@@ -676,17 +563,18 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
     __syncthreads();
 
     // ---- merge of the warps and the new token: a lane owns four dims of each of the warp's heads
-    const int old = more ? flip ^ 1 : flip;
+    const int n_split = pc.n_split, split = pc.split, rec0 = pc.part0 * kNHeadKv + kvh;  // this KV head's records: every fourth
+    const size_t out_row = size_t(p.tok0 + pc.tok) * kQDim;
 #pragma unroll
     for (int i = 0; i < kHeads; i++) {
         if (!has_heads) break;
-        const int h = warp * kHeads + i, head = kv_head * kGqa + h;
+        const int h = warp * kHeads + i, head = kvh * kGqa + h;
         float M = s_new[i];
 #pragma unroll
         for (int w = 0; w < kWarps; w++) M = fmaxf(M, sm.red_m[w][h]);
-        float L = with_new ? fast_exp2(s_new[i] - M) : 0.f, A[4] = {0.f, 0.f, 0.f, 0.f};
-        if (with_new) {
-            const uint2 hv = *reinterpret_cast<const uint2 *>(&sm.vnew[old][d0]);
+        float L = ends ? fast_exp2(s_new[i] - M) : 0.f, A[4] = {0.f, 0.f, 0.f, 0.f};
+        if (ends) {
+            const uint2 hv = *reinterpret_cast<const uint2 *>(&sm.vnew[d0]);
             const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&hv.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&hv.y));
             A[0] = L * a.x; A[1] = L * a.y; A[2] = L * b.x; A[3] = L * b.y;
         }
@@ -702,23 +590,53 @@ __device__ __forceinline__ void decode_pieces(const Dec4Params &p, const Dec4Pie
             const float sink2 = sm.sinks[head] * kLog2e;
             const float Mf = fmaxf(M, sink2), cf = fast_exp2(M - Mf);
             const float inv = cf / (L * cf + fast_exp2(sink2 - Mf));
-            store_out4(p.out, p.out_dtype, size_t(row) * kQDim + head * kHeadDim + d0, A[0] * inv, A[1] * inv, A[2] * inv, A[3] * inv);
+            store_out4(p.out, p.out_dtype, out_row + head * kHeadDim + d0, A[0] * inv, A[1] * inv, A[2] * inv, A[3] * inv);
         } else {  // this piece's record: acc, m (base 2), l
             float *rec = p.scratch + (size_t(rec0 + split * kNHeadKv) * kGqa + h) * kRecStride;
             *reinterpret_cast<float4 *>(rec + d0) = make_float4(A[0], A[1], A[2], A[3]);
             if (lane == 0) *reinterpret_cast<float2 *>(rec + kHeadDim) = make_float2(M, L);
         }
     }
-    if (waiting) merge_runs();
-    waiting = n_split > 1 && has_heads;
-    if (waiting) {
-        out = {rec0, split, n_split, kv_head, row};
-        count_record();
+    if (n_split == 1 || !has_heads) return;
+
+    // ---- split-K, per query head: a warp that has written its record of a head counts it; the one that finds itself the last of
+    // its run of records merges the run, and if that was the last run of the head, the runs.  (The record's stores are ordered
+    // before lane 0's ticket by the warp's barrier; the ticket is an acquire-release atomic at device scope, cumulative over
+    // them; the readers go past L1.)
+    const int fan = dec4_fan(n_split), sub = split / fan, n_sub = (n_split + fan - 1) / fan, n = min(fan, n_split - sub * fan);
+    int arrived[kHeads];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kHeads; i++)
+        if (lane == 0) arrived[i] = ticket_acq_rel(&p.tickets[(rec0 + sub * kNHeadKv) * kGqa + warp * kHeads + i]);
+    __syncwarp();  // lane 0's tickets come before the other lanes' reads
+#pragma unroll
+    for (int i = 0; i < kHeads; i++) {
+        const int h = warp * kHeads + i, head = kvh * kGqa + h;
+        auto record = [&](float *base, int k) { return base + (size_t(rec0 + k * kNHeadKv) * kGqa + h) * kRecStride; };
+        if (__shfl_sync(0xffffffffu, arrived[i], 0) != n - 1) continue;
+        if (lane == 0) p.tickets[(rec0 + sub * kNHeadKv) * kGqa + h] = 0;  // ready for the next launch
+        Merged4 r = merge_records4([&](int k) { return record(p.scratch, sub * fan + k); }, n, d0);
+        if (n_sub > 1) {
+            float *rec = record(p.scratch2, sub);
+            *reinterpret_cast<float4 *>(rec + d0) = make_float4(r.a[0], r.a[1], r.a[2], r.a[3]);
+            if (lane == 0) *reinterpret_cast<float2 *>(rec + kHeadDim) = make_float2(r.M, r.L);
+            __syncwarp();
+            int last = 0;
+            int *ticket = &p.tickets2[rec0 * kGqa + h];
+            if (lane == 0) {
+                last = ticket_acq_rel(ticket) == n_sub - 1;
+                if (last) *ticket = 0;
+            }
+            __syncwarp();
+            if (!__shfl_sync(0xffffffffu, last, 0)) continue;
+            r = merge_records4([&](int k) { return record(p.scratch2, k); }, n_sub, d0);
+        }
+        const float sink2 = sm.sinks[head] * kLog2e;
+        const float Mf = fmaxf(r.M, sink2), cf = fast_exp2(r.M - Mf);
+        const float inv = cf / (r.L * cf + fast_exp2(sink2 - Mf));
+        store_out4(p.out, p.out_dtype, out_row + head * kHeadDim + d0, r.a[0] * inv, r.a[1] * inv, r.a[2] * inv, r.a[3] * inv);
     }
-    if (!more) break;
-    __syncthreads();  // the merge buffer is free, the next piece's rows are there
-    }  // pieces
-    if (waiting) merge_runs();
 }
 
 template <int kCap>
@@ -729,7 +647,7 @@ struct Dec4List {
 template <int kCap, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, 16 / kWarps)
     k_decode_kv4(const __grid_constant__ Dec4Params p, const __grid_constant__ Dec4List<kCap> list) {
-    decode_pieces<kWarps>(p, list.pieces);
+    decode_piece<kWarps>(p, list.pieces[blockIdx.x >> 2], int(blockIdx.x & 3));
 }
 
 // The parameter block is copied at every launch, so the kernel comes in three capacities and a launch takes the smallest

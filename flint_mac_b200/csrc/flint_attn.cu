@@ -465,8 +465,6 @@ struct flint_attn {
             const int m = plan_decode_kv4(n - i0, seqs + i0, p + i0, kv4_tiles.data() + i0, target_items, kv4_pieces, n_records, n_warps);
             dp.scratch = scratch; dp.scratch2 = scratch2;
             dp.tickets = tickets; dp.tickets2 = tickets + n_tickets / 2;
-            // (a CTA of four warps takes half the room of one of eight)
-            dp.several_rounds = int(kv4_pieces.size()) * kNHeadKv * n_warps > sm_count * kDec4CtasPerSm * 8;
             dp.tok0 = i0;
             CK(launch_decode_kv4(dp, kv4_pieces.data(), int(kv4_pieces.size()), n_warps, st));
             launches++;

@@ -53,7 +53,6 @@ struct Dec4Params {
     Kv4Cache cache;
     float *scratch, *scratch2;  // split-K records of both merge levels, [n_records][4 KV heads][8][kRecStride]
     int *tickets, *tickets2;    // arrival counters, [n_records][4][8]; zero between launches (and graph replays)
-    int several_rounds;         // more CTAs than the GPU holds at a time: the first ones take over the others' pieces
     int tok0;                   // row of qkv and out that the launch's token 0 has
     int is_swa, has_rope, qkv_dtype, out_dtype;
     int *error_flag;

@@ -1,10 +1,11 @@
 // The work list of a decode launch over 4-bit caches (host side, and what host and device share).
 //
 // The visible keys of a (token, KV head) group are tiles of 64; a token's tiles are cut into equal pieces, and the launch
-// has one CTA per piece and KV head, longest first.  The CTAs that fit the GPU at a time stay and take the pieces of those
-// that have not started (the hardware's scheduler hands them out), so that an SM that gets less of the memory's bandwidth
-// than others takes fewer pieces: with equal shares, dealt beforehand, the SMs of a 64 x 8192 batch ended between 42 and
-// 62 us.
+// has one CTA per piece and KV head, longest first.  Where there are more than the GPU holds at a time, the hardware starts
+// the next one on the SM that is through first, so that an SM that gets less of the memory's bandwidth than others takes
+// fewer pieces.  (CTAs that stay and take over the pieces of those that have not started, the next piece's rows fetched
+// ahead, were slower on every batch: 256 windows of a mixed batch 27.4 against 20.7 us, 128 sequences of 8192 keys 137
+// against 130, 400 of 0 to 3000 46.1 against 43.1.)
 #pragma once
 
 #include <algorithm>
@@ -57,10 +58,11 @@ __host__ __device__ inline int dec4_fan(int n_split) {
 // While every token's four groups fit the slots the launch is one round: the tokens are cut so that the longest piece is as
 // short as the slots allow.  A piece costs some 5 us beside its tiles (rows, norm and rotation, the merges), so nothing is
 // cut below kLeast tiles, and a window never.  Larger batches go in several rounds, cut only where a token is longer than a
-// slot's share.  Eight warps a piece: 64 x 8192 keys take 68 us (four warps: 73), one 131072-key sequence 28 (33); many
-// short pieces are over sooner with four, whose CTAs overlap each other's beginnings and ends (256 windows: 33 against
-// 40 us), and pieces that leave half of the GPU idle with sixteen, if they have tiles for them (32 windows: 7.5 against
-// 10.2 us).
+// slot's share.  Warps of a CTA (each the others' time in long runs): eight, as 64 x 8192 keys take 66.7 us (four 110, sixteen
+// 67.1), one 131072-key sequence 22.0 (28, 28.6), 32 sequences of 0 to 32768 keys 23.7 (45, 27).  Many short pieces are over
+// sooner with four, whose CTAs overlap each other's beginnings and ends: 256 windows 28.6 (eight 34.6), 256 x 600 keys 28.3
+// (33.4).  Pieces that leave half of the GPU idle have sixteen, if they have tiles for them: 32 windows 7.2 (eight 10.0, four
+// 14.6), 4 x 8192 keys 9.7 (12.8, 21.7).
 inline int plan_decode_kv4(int n, const int32_t *seqs, const int32_t *pos, const int *tiles, int slots,
                            std::vector<Dec4Piece> &pieces, int &n_records, int &n_warps) {
     constexpr int kLeast = 16;
