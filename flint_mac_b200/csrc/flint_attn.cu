@@ -1485,7 +1485,7 @@ int32_t flint_attn_plan_decode_int4(int32_t n, const int32_t *pos, int32_t is_sw
 
 int32_t flint_attn_plan_prefill_int4(int32_t n_tok, int32_t p0, int32_t n_sm, int32_t *out, int32_t cap) {
     try {
-        if (n_tok <= 0 || p0 < 0 || n_sm < 1 || n_tok > INT32_MAX - p0 || !out) return -1;
+        if (n_tok <= 0 || p0 < 0 || n_sm < 1 || n_tok > INT32_MAX - 256 - p0 || !out) return -1;  // (room for the rounding up to units and tiles)
         std::vector<PrefillPiece> pieces;
         int n_units = 0, parts = 0;
         plan_prefill_kv4(n_tok, p0, n_sm, pieces, n_units, parts);

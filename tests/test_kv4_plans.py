@@ -64,7 +64,7 @@ def test_prefill_plan_covers_every_tile_once(fa):
     assert seen > 300
 
 
-@pytest.mark.parametrize("n_tok,p0,n_sm", [(0, 5, 148), (-1, 5, 148), (5, -1, 148), (5, 5, 0), (2147483647, 1, 148)])
+@pytest.mark.parametrize("n_tok,p0,n_sm", [(0, 5, 148), (-1, 5, 148), (5, -1, 148), (5, 5, 0), (2147483647, 1, 148), (2147483647, 0, 148), (1, 2147483647, 148)])
 def test_prefill_plan_refuses(fa, n_tok, p0, n_sm):
     with pytest.raises(fa.FlintAttnError):
         fa.plan_prefill_int4(n_tok, p0, n_sm)
