@@ -38,7 +38,8 @@ __device__ __forceinline__ void half_row_staged(uint2 &k, uint2 &v) {
 
 // d and lo of a group, packed {d, lo}, and 1 / d, from its least and largest value (halves; NaN if a value was one).  A group
 // that holds an infinity or a NaN gets d = NaN.  The quotient by 15, like those by d below, is the product with the
-// reciprocal and one correction step, which rounds it as a division does (Markstein 1990).
+// reciprocal and one correction step, which rounds it as a division does (Markstein 1990).  32 bits, not exact, because exact
+// codes would ask each value how near it is to a border, some 15 % more instructions of a store by count, for one code in billions.
 struct Kv4Scale {
     uint32_t dl;
     float d, lo, inv;

@@ -2,7 +2,9 @@
 //
 // A cache row is the 128 values x of one token and KV head, K or V, rounded to half, in four groups of 32.  A group keeps
 //   lo = min x,   d = half((max x - lo) / 15),   code = round-half-even((x - lo) / d) limited to 0..15   (0 where d = 0)
-// and stands for lo + code * d.  A group that holds an infinity or a NaN gets d = NaN and reads back as NaN throughout.
+// and stands for lo + code * d.  Differences and quotients are those of 32 bits, so a value within 2^-19 of a step of the border
+// between two codes may get either: where one of x and lo is far smaller than the other, their difference has more bits than a
+// float.  A group that holds an infinity or a NaN gets d = NaN and reads back as NaN throughout.
 // Codes are 64 bytes a row, d and lo 2 + 2 bytes a group: 80 bytes, where the half-precision cache takes 256.
 //
 // 64 consecutive positions of one sequence and KV head make one block of 10240 bytes, K and V together, so that one bulk

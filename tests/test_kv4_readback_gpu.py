@@ -92,3 +92,38 @@ def test_chunk_behind_a_chunk(fa, is_swa, first):
     for x, y in zip(*outs):
         assert torch.isfinite(x).all() and torch.equal(x, y)
     assert not torch.equal(outs[0][1][0], outs[0][1][1])
+
+
+def test_codes_beside_a_border(fa):
+    """Values as near to the border between two codes as halves get, tiny ones beside a large least value: whichever code they
+    get, they are within half a step and 2^-19 of one of what it stands for (the difference x - lo and its quotient by d are
+    below 16 steps and rounded to 32 bits, 2^-24 relative each: 2^-19 steps)."""
+    import torch
+
+    g = torch.Generator().manual_seed(101)
+    n = 6400
+    code = torch.randint(1, 14, (n, 4, 1), generator=g).double() + 0.5
+    d = (0.1 + 0.4 * torch.rand(n, 4, 1, generator=g)).half().double()
+    lo = (-code * d).half().double()
+    x = torch.empty(n, 4, 32, dtype=torch.float64)
+    x[..., 0:1], x[..., 1:2] = lo, (lo + 15 * d).half().double()
+    c = torch.arange(1, 15) + 0.5
+    x[..., 2:16] = (lo + c * d).half().double()          # beside every border
+    x[..., 16:32] = (lo + code * d).half().double()      # beside the one that lies next to zero
+    rows = x.reshape(n, 128).half()
+    rows[-1, :2] = torch.tensor([-2.01171875, 1.5390625])
+    rows[-1, 2:32] = 0.00018322467803955078              # x - lo is a tie of 32-bit floats, on a border of d = 0.2366943359375
+    back = torch.empty(2, 1, 4, n // 4, 128, device="cuda")
+    given = rows.cuda().view(1, 4, n // 4, 128)
+    with _open(fa, torch, False, 1, n // 4) as h:
+        h.store_kv_dev(0, [0], [0], n // 4, given, given, fa.F16)
+        h.load_kv_dev(0, [0], [0], n // 4, back[0], back[1], fa.F32)
+        h.check()
+    assert torch.equal(back[0], back[1])
+    _, d, lo = ref.quantise(given)
+    value, x = back[0].double().unflatten(-1, (4, 32)), given.double().unflatten(-1, (4, 32))
+    inside = (x - lo) / d <= 14.5  # (beyond it the last code's value may lie further off by the rounding of d)
+    assert float(inside.double().mean()) > 0.9
+    off = (value - x).abs() - d * (0.5 + 2.0**-19) - 2.0**-24 * value.abs()
+    assert float(off[inside].max()) <= 0, float((off / d)[inside].max())
+    assert float(d[0, -1, -1, 0, 0]) == 0.2366943359375
