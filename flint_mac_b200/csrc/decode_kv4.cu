@@ -20,12 +20,16 @@
 // tile is one 5 KB bulk copy for K and one for V, on mbarriers of the warp's own; the next tile's K comes in while this one's
 // V is worked on, and the other way round.
 //
-// Bytes per tile of 64 keys: 10240, against about 800 instructions of the warp, 72 of them products.  64 x 8192 keys (337 MB)
-// take 59 us, 5.7 TB/s or 0.88 of a copy's rate, in short runs, and 68 us when the GPU's power limit holds the clocks down
-// in a long one: the SMs issue 2.1 instructions a cycle (46 % of the logical unit's rate, 34 % of the tensor pipe's) and
-// DRAM is 67 % busy, so memory and issue bound it together.  Shorter launches are bound by latency: about 1.8 us from the
-// wait to the first tile (rows, norm, rotation), 2 us a tile and warp, 1.2 us for the merge of the warps, 4 to 5 us for that
-// of the splits.  One 131072-key sequence takes 23.2 us (its bytes 13), 32 windows 7.5, 256 windows 25.7, 317 keys 5.9.
+// Roundings to half, 2^-11 relative each, which the products' operands need: the rows of q after norm, rotation and scale;
+// their operands q0 - q1 / 16 once more; the probabilities (the denominator adds them up unrounded); a probability times d.
+// Sums, maxima, records and the parts of lo are in 32 bits.
+//
+// Bytes per tile of 64 keys: 10240, against 885 instructions of the warp, 72 of them products.  64 x 8192 keys (337 MB) take
+// 58.2 us, 5.8 TB/s or 0.90 of a copy's rate, in short runs, and 66.7 us when the GPU's power limit holds the clocks down in
+// a long one: the SMs issue 2.1 instructions a cycle (46 % of the logical unit's rate, 35 % of the tensor pipe's) and DRAM is
+// 69 % busy, so memory and issue bound it together.  Shorter launches are bound by latency: about 1.8 us from the wait to the
+// first tile (rows, norm, rotation), 2 us a tile and warp, 1.2 us for the merge of the warps, 4 to 5 us for that of the
+// splits.  One 131072-key sequence takes 22.0 us (its bytes 13), 32 windows 7.2, 256 windows of a mixed batch 21, 317 keys 5.7.
 #include <cstring>
 
 #include "decode_common.cuh"

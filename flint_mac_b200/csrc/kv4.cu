@@ -50,7 +50,9 @@ __device__ __forceinline__ size_t half_first_row(int seq, int kvh, int pos) {
     return ((size_t(seq) * kNHeadKv + kvh) * kMaxFirstTokens + pos) * kHeadDim;
 }
 
-// ---- half-precision caches: one warp per (sequence, row, KV head)
+// ---- half-precision caches: one warp per (sequence, row, KV head).  Bound by memory: 131071 rows of one sequence from half
+// (537 MB read and written) are stored in 115 us and read back in 118, 0.72 and 0.70 of a copy's rate (one or two loads in
+// flight a lane); 16384 rows in 14.2 and 12.9 us (their bytes 10.4), 64 rows in 4.2 and 4.0.
 __global__ void __launch_bounds__(256) k_half_store(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs, int n) {
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // (after the wait: see the prefill prologue)
@@ -103,8 +105,8 @@ __global__ void __launch_bounds__(256) k_half_load(const KvRowsParams p, const _
 // ---- 4-bit caches: one CTA per (sequence, KV head, block of 64 positions), so that a block's codes are written or read by
 // one CTA.  Eight neighbouring values a lane (one 16-byte access in half precision, four bytes of codes): 16 lanes a row,
 // four lanes a group, two neighbouring rows a warp; a thread's loads are all in flight before the first is used.
-// Loading is bound by memory: 131071 rows of one sequence to half (84 MB read, 268 MB written) take 56.7 us, 6.2 TB/s or
-// 0.96 of a copy's rate.
+// Loading is bound by memory: 131071 rows of one sequence to half (84 MB read, 268 MB written) take 57.0 us, 6.2 TB/s or
+// 0.95 of a copy's rate.
 constexpr int kRowThreads = 256;
 constexpr int kRowSteps = kKv4BlockKeys * 16 / kRowThreads;  // rows of a lane in a block
 
@@ -192,9 +194,11 @@ __device__ __forceinline__ unsigned char *block_of(const KvRowsParams &p, const 
     return p.cache.blocks + ((size_t(b.seq) * kNHeadKv + b.kvh) * p.cache.blocks_per_seq + b.block) * kKv4BlockBytes;
 }
 
-// Storing is bound by instructions, so a lane has sixteen values here (half a group: one exchange between lanes, d and lo
-// worked out by two lanes instead of four: 13.1 instead of 17 us for 16384 rows), eight lanes a row, and K and V of a block
-// are separate CTAs.  16384 rows of one sequence from half (34 MB read, 10 MB written) take 10.4 us: 4.2 TB/s.
+// Storing takes most instructions per byte, so a lane has sixteen values here (half a group: one exchange between lanes, d and
+// lo worked out by two lanes instead of four: 13.1 instead of 17 us for 16384 rows, 10.4 with whole blocks apart), eight lanes
+// a row, and K and V of a block are separate CTAs.  16384 rows of one sequence from half (34 MB read, 10 MB written) take
+// 10.0 us: 4.4 TB/s, 0.68 of a copy's rate.  No unit is full (2.6 instructions a cycle of 4, the logical unit 45 %, DRAM 33 %,
+// as what is written stays in L2): 2056 CTAs are 2.3 times what the GPU holds, and each waits for its rows once.
 constexpr int kStoreSteps = kKv4BlockKeys * 8 / kRowThreads;
 template <int kType>
 __global__ void __launch_bounds__(kRowThreads, kType == kDtypeF32 ? 4 : 6) k_kv4_store(const KvRowsParams p, const __grid_constant__ KvRowsSeqs seqs) {

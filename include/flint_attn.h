@@ -72,14 +72,20 @@ void flint_attn_close(flint_attn *a);
  *     A row is one token's 128 values of one KV head, K after norm and rotation, rounded to half as in a half-precision
  *     cache, in four groups of 32.  A group keeps lo = min, d = half((max - lo) / 15) and codes
  *     round-half-even((x - lo) / d) limited to 0..15 (0 where d is 0), and stands for lo + code d.  A group with an
- *     infinity or a NaN in it reads back as NaN.  All calls below work as on a half-precision handle, contiguous and
+ *     infinity or a NaN in it reads back as NaN.  Differences and quotients are rounded to 32 bits: a value within 2^-19 of a
+ *     step of the border between two codes may get either.  All calls below work as on a half-precision handle, contiguous and
  *     paged; a call's own tokens are attended as their half-precision rows, what the cache held before the call as the
  *     values that it stands for.  Not with kv_ranks > 1, and no partial records (decode_partial, prefill_partial, xchg).
  *     A prefill behind a cached context on a full layer brings that context into half-precision scratch of the handle
  *     (n_ctx rows, 2 KB each, once for all layers).
  *   first_tokens  0 to 64, with either format: on sliding-window layers a query at position p sees, besides the last 513
  *     positions, positions below first_tokens.  Each sequence keeps those rows outside the ring; n_slots is
- *     1024 + first_tokens there, slots from 1024 on being the first tokens' rows.
+ *     1024 + first_tokens there, slots from 1024 on being the first tokens' rows.  Their keys keep the rotation of their own
+ *     positions, and queries that of theirs: nothing is re-numbered as the window moves on.  Decode, prefill and
+ *     flint_attn_store_kv_dev write a position below first_tokens to both places; flint_attn_write_kv writes the slots it is
+ *     given, so a caller who fills such a cache by slot fills both (0 .. first_tokens - 1 and 1024 .. 1023 + first_tokens), as
+ *     flint_attn_load_kv_dev and a prefill over a 4-bit cache read those positions from the rows behind the ring even while
+ *     the window holds them.
  * A 4-bit cache's device memory (flint_attn_kv_dev, which = 0; which = 1 is NULL) is in the library's own block format. */
 enum { FLINT_ATTN_KV_F16 = 0, FLINT_ATTN_KV_INT4 = 1 };
 typedef struct {
