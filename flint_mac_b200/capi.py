@@ -315,7 +315,10 @@ class Attn:
         def call(qkv_address: int):
             if self._h is None:
                 raise FlintAttnError("the handle is closed")
-            rows.value = qkv_address
+            try:
+                rows.value = qkv_address
+            except TypeError:  # a ctypes pointer, as a call that converts its arguments takes it
+                rows.value = qkv_address.value if isinstance(qkv_address, C.c_void_p) else C.cast(qkv_address, C.c_void_p).value
             if fn(*args) != 0:
                 raise FlintAttnError(err.value.decode(errors="replace"))
 
