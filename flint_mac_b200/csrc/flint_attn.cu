@@ -1486,9 +1486,7 @@ int32_t flint_attn_plan_decode_int4(int32_t n, const int32_t *pos, int32_t is_sw
 int32_t flint_attn_plan_prefill_int4(int32_t n_tok, int32_t p0, int32_t n_sm, int32_t *out, int32_t cap) {
     try {
         if (n_tok <= 0 || p0 < 0 || n_sm < 1 || n_tok > INT32_MAX - 256 - p0 || !out) return -1;  // (room for the rounding up to units and tiles)
-        std::vector<PrefillPiece> pieces;
-        int n_units = 0, parts = 0;
-        plan_prefill_kv4(n_tok, p0, n_sm, pieces, n_units, parts);
+        const std::vector<PrefillPiece> pieces = plan_prefill_kv4(n_tok, p0, n_sm);
         if (int64_t(pieces.size()) > cap) return -1;
         static_assert(sizeof(PrefillPiece) == 8 * sizeof(int32_t), "a record");
         if (!pieces.empty()) memcpy(out, pieces.data(), pieces.size() * sizeof(PrefillPiece));

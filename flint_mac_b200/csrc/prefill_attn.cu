@@ -1218,22 +1218,21 @@ int choose_cuts(int n_tok, int p0, int n_units, int n_ksplit, int sm_count, int 
 
 }  // namespace
 
-int plan_prefill_kv4(int n_tok, int p0, int sm_count, std::vector<PrefillPiece> &pieces, int &n_units, int &parts) {
+std::vector<PrefillPiece> plan_prefill_kv4(int n_tok, int p0, int sm_count) {
     static thread_local PfCuts cuts;
     constexpr int kAll = 0x7fffffff;
-    n_units = (n_tok + kCtaPos - 1) / kCtaPos * kNHeadKv;
+    std::vector<PrefillPiece> pieces;
+    const int n_units = (n_tok + kCtaPos - 1) / kCtaPos * kNHeadKv;
     const int n_ksplit = even_ksplit(n_tok, p0, n_units, sm_count, 0, kAll);
     int n_pieces = 0;
-    parts = choose_cuts(n_tok, p0, n_units, n_ksplit, sm_count, 0, kAll, cuts, n_pieces);
-    pieces.clear();
-    if (parts == 0) return n_ksplit;
+    if (choose_cuts(n_tok, p0, n_units, n_ksplit, sm_count, 0, kAll, cuts, n_pieces) == 0) return pieces;
     for (int b = 0; b < sm_count; b++)
         for (int e = cuts.start[b]; e < cuts.start[b + 1]; e++) {
             const PfCut &c = cuts.e[e];
             const Unit u = unit_geom_of(c.unit, n_tok, p0, 0, 0, 1);
             pieces.push_back(PrefillPiece{b, c.unit, c.part, c.tile0, c.tile1, u.n_tiles, u.q_first, u.kvh});
         }
-    return n_ksplit;
+    return pieces;
 }
 
 cudaError_t prefill_kernel_setup() {

@@ -61,11 +61,11 @@ cudaError_t make_kv_rows_map(void *map_out, const void *base, long long n_rows);
 cudaError_t launch_prefill(const PrefillParams &p, PrefillWorkspace &ws, cudaStream_t stream, int *n_launches);
 // The work list of a full layer with a 4-bit cache whose units (32 query positions of a KV head) are cut so that all CTAs end
 // together, as launch_prefill makes it: CTA `cta` takes key tiles [tile0, tile1) of the unit_tiles of unit `unit`, its part
-// `part`.  No pieces (parts = 0) where the units stay whole or are cut evenly; the number of even ranges is returned.
+// `part`.  No pieces where the units stay whole or are cut evenly.
 struct PrefillPiece {
     int cta, unit, part, tile0, tile1, unit_tiles, q_first, kvh;
 };
-int plan_prefill_kv4(int n_tok, int p0, int sm_count, std::vector<PrefillPiece> &pieces, int &n_units, int &parts);
+std::vector<PrefillPiece> plan_prefill_kv4(int n_tok, int p0, int sm_count);
 void prefill_workspace_free(PrefillWorkspace &ws);
 // parts_o [n_parts][n_tok][4096] fp32, parts_ml [n_parts][n_tok][32][2] -> out [n_tok][4096]: log-sum-exp merge of the
 // devices' partials (src/metal/fused.metal:332-350 applied to prefill rows; the sink is inside one part's l).
